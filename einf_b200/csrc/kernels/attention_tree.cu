@@ -1,0 +1,265 @@
+// Attention of drafted trees over the paged cache with 32-bit products: the 32-bit path, and in bfloat16 the head and
+// page sizes that the tensor-core kernel (attention_tree_tcgen05.cu) does not take.
+//
+//   o_i = sum_j p_ij v_j,  p_ij = softmax_j(cap(scale q_i . k_j)) over the keys that node i sees
+//
+// One pass over the keys, 32 at a time, with the running maximum and sum of every row.  Four warps have eight
+// rows each.  Scores: lane j has key j, whose elements it reads once for its eight rows; the rows come as broadcasts.
+// Sums: a lane has a few elements of the head, whose values it reads once for its eight rows.  Both products read 12
+// 16-byte words of shared memory for 32 fused multiply-adds, so shared memory bounds the kernel at two thirds of
+// the FMA rate.  Keys that no row of a tile is kept from run without masks; in the other tiles a value is added
+// to the rows that see it and to no others, so that what stands in a masked place (a sibling's value, a row behind the
+// last node) may be anything.
+#include "attention_tree.cuh"
+
+namespace einf {
+
+constexpr int kKeys = 32;
+constexpr int kWarps = 4;
+constexpr int kRowsPerWarp = 8;
+constexpr int kRows = kWarps * kRowsPerWarp;
+
+// VEC: elements of the head that a lane has (2, 4 or 8: heads of up to 64, 128, 256)
+template <typename T, int VEC>
+__global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams p) {
+  extern __shared__ __align__(16) float smem[];
+  const int size4 = (p.size + 3) & ~3, pitch = size4 + 4;
+  float* ks = smem;                                 // [keys][pitch]
+  float* vs = ks + kKeys * pitch;                   // [keys][32 * VEC]
+  float* qs = vs + kKeys * 32 * VEC;                // [rows][size4]
+  float* ps = qs + kRows * size4;                   // [rows][keys]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_launch_dependents();
+  pdl_wait();
+  const T* q = static_cast<const T*>(p.q);
+  const T* k_cache = static_cast<const T*>(p.k_cache);
+  const T* v_cache = static_cast<const T*>(p.v_cache);
+  TreeWalk w;
+  bool any = tree_first(p, &w);
+  tree_note(p, w, any);
+  const float scale_log2 = p.scale * 1.4426950408889634f, cap_log2 = p.softcap * 1.4426950408889634f;
+  for (; any; any = tree_next(p, &w)) {
+    const TreeUnit u = tree_unit(p, w.t, w.unit);
+    const int rows = u.nodes * u.heads;
+    __syncthreads();
+    for (int e = threadIdx.x; e < kRows * size4; e += 32 * kWarps) {
+      const int row = e / size4, d = e - row * size4;
+      float v = 0.f;
+      if (row < rows && d < p.size)
+        v = to_float(q[((size_t)(w.t.first + u.first_node + row / u.heads) * p.heads + u.first_head + row % u.heads) * p.size + d]);
+      qs[e] = v;
+    }
+    float m[kRowsPerWarp], l[kRowsPerWarp], acc[kRowsPerWarp][VEC];
+#pragma unroll
+    for (int i = 0; i < kRowsPerWarp; ++i) {
+      m[i] = -INFINITY;
+      l[i] = 0.f;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) acc[i][e] = 0.f;
+    }
+    const int keys_end = w.t.cached + w.t.nodes;
+    const int* table = p.block_table + (size_t)w.request * p.table_width;
+    for (int tile = w.tile_begin; tile < w.tile_end; ++tile) {
+      const int key0 = w.t.begin + tile * kKeys;
+      __syncthreads();
+      // four threads a key; a key beyond the end is zeros
+      {
+        const int key = key0 + (threadIdx.x >> 2), part = threadIdx.x & 3;
+        size_t at = 0;
+        bool live = key < keys_end;
+        if (live) {
+          const int page = table[key / p.page_size];
+          if (page < 0 || page >= p.num_pages) {
+            atomicOr(p.status, kStatusBadPage);
+            live = false;
+          } else {
+            at = (((size_t)page * p.kv_heads + u.kv_head) * p.page_size + key % p.page_size) * p.size;
+          }
+        }
+        float* kr = ks + (threadIdx.x >> 2) * pitch;
+        float* vr = vs + (threadIdx.x >> 2) * 32 * VEC;
+        for (int d = part; d < size4; d += 4) kr[d] = live && d < p.size ? to_float(k_cache[at + d]) : 0.f;
+        for (int d = part; d < 32 * VEC; d += 4) vr[d] = live && d < p.size ? to_float(v_cache[at + d]) : 0.f;
+      }
+      __syncthreads();
+      const int my_rows = min(kRowsPerWarp, rows - warp * kRowsPerWarp);
+      if (my_rows <= 0) continue;
+      float s[kRowsPerWarp];
+#pragma unroll
+      for (int i = 0; i < kRowsPerWarp; ++i) s[i] = 0.f;
+      const float* kr = ks + lane * pitch;
+      const float* qr = qs + warp * kRowsPerWarp * size4;
+#pragma unroll 2
+      for (int d = 0; d < size4; d += 4) {
+        const float4 k4 = *reinterpret_cast<const float4*>(kr + d);
+#pragma unroll
+        for (int i = 0; i < kRowsPerWarp; ++i) {
+          const float4 q4 = *reinterpret_cast<const float4*>(qr + i * size4 + d);
+          s[i] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[i]))));
+        }
+      }
+      uint32_t seen[kRowsPerWarp];
+      uint32_t all = 0xffffffffu;
+#pragma unroll
+      for (int i = 0; i < kRowsPerWarp; ++i) {
+        const int row = warp * kRowsPerWarp + i;
+        uint32_t bits = 0u;
+        if (row < rows) {
+          const int token = w.t.first + u.first_node + row / u.heads;
+          const int position = tree_position(p, w.t, token);
+          bits = tree_visible(p, w.t, token, tree_lowest(p, position), position, key0);
+        }
+        seen[i] = bits;
+        all &= row < rows ? bits : 0xffffffffu;
+        float x = p.softcap > 0.f ? cap_log2 * tanhf(s[i] * p.scale / p.softcap) : s[i] * scale_log2;
+        if (!(bits >> lane & 1u)) x = -INFINITY;
+        const float top = fmaxf(m[i], warp_max(x));
+        const float keep = m[i] == -INFINITY ? 0.f : exp2f(m[i] - top);
+        const float e = (bits >> lane & 1u) && x != -INFINITY ? exp2f(x - top) : 0.f;
+        l[i] = (l[i] == 0.f ? 0.f : l[i] * keep) + warp_sum(e);
+        m[i] = top;
+        ps[row * kKeys + lane] = e;
+#pragma unroll
+        for (int d = 0; d < VEC; ++d) acc[i][d] *= keep;
+      }
+      __syncwarp();
+      const float* pr = ps + warp * kRowsPerWarp * kKeys;
+      auto value = [&](int j, float* v) {
+        const float* vr = vs + j * 32 * VEC;
+        if (VEC == 2) {
+          const float2 a = *reinterpret_cast<const float2*>(vr + 2 * lane);
+          v[0] = a.x, v[1] = a.y;
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; e += 4) {
+            const float4 a = *reinterpret_cast<const float4*>(vr + e * 32 + 4 * lane);
+            v[e] = a.x, v[e + 1] = a.y, v[e + 2] = a.z, v[e + 3] = a.w;
+          }
+        }
+      };
+      if (all == 0xffffffffu) {
+#pragma unroll 1
+        for (int j = 0; j < kKeys; j += 4) {
+          float4 e4[kRowsPerWarp];
+#pragma unroll
+          for (int i = 0; i < kRowsPerWarp; ++i) e4[i] = *reinterpret_cast<const float4*>(pr + i * kKeys + j);
+#pragma unroll
+          for (int jj = 0; jj < 4; ++jj) {
+            float v[VEC];
+            value(j + jj, v);
+#pragma unroll
+            for (int i = 0; i < kRowsPerWarp; ++i) {
+              const float e = jj == 0 ? e4[i].x : jj == 1 ? e4[i].y : jj == 2 ? e4[i].z : e4[i].w;
+#pragma unroll
+              for (int d = 0; d < VEC; ++d) acc[i][d] = fmaf(e, v[d], acc[i][d]);
+            }
+          }
+        }
+      } else {
+        uint32_t some = 0u;
+#pragma unroll
+        for (int i = 0; i < kRowsPerWarp; ++i) some |= seen[i];
+        for (; some; some &= some - 1) {
+          const int j = __ffs(some) - 1;
+          float v[VEC];
+          value(j, v);
+#pragma unroll
+          for (int i = 0; i < kRowsPerWarp; ++i)
+            if (seen[i] >> j & 1u) {
+              const float e = pr[i * kKeys + j];
+#pragma unroll
+              for (int d = 0; d < VEC; ++d) acc[i][d] = fmaf(e, v[d], acc[i][d]);
+            }
+        }
+      }
+      __syncwarp();
+    }
+#pragma unroll
+    for (int i = 0; i < kRowsPerWarp; ++i) {
+      const int row = warp * kRowsPerWarp + i;
+      if (row >= rows) break;
+      const size_t at = ((size_t)(w.t.first + u.first_node + row / u.heads) * p.heads + u.first_head + row % u.heads) * p.size;
+      const size_t share = (size_t)w.share * p.unit_rows + row;
+      const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int d = VEC == 2 ? 2 * lane + e : (e >> 2) * 128 + 4 * lane + (e & 3);
+        if (w.whole) {
+          if (d < p.size) static_cast<T*>(p.out)[at + d] = from_float<T>(acc[i][e] * inv);
+        } else if (d < p.padded) {
+          p.part_o[share * p.padded + d] = acc[i][e];
+        }
+      }
+      if (!w.whole && lane == 0) p.part_ml[share] = make_float2(m[i], l[i]);
+    }
+  }
+}
+
+template <typename T, int VEC>
+int launch_tree(const TreeParams& p, cudaStream_t stream) {
+  const int size4 = (p.size + 3) & ~3;
+  const size_t smem = sizeof(float) * ((size_t)kKeys * (size4 + 4) + kKeys * 32 * VEC + kRows * size4 + kRows * kKeys);
+  cudaError_t e = cudaFuncSetAttribute(tree_attention_kernel<T, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return (int)e;
+  e = launch_pdl(tree_attention_kernel<T, VEC>, dim3(p.ctas), dim3(32 * kWarps), smem, stream, p);
+  if (e != cudaSuccess) return (int)e;
+  return tree_merge<T>(p, stream);
+}
+
+template <typename T>
+int dispatch_tree(const TreeParams& p, cudaStream_t stream) {
+  return p.size <= 64 ? launch_tree<T, 2>(p, stream) : p.size <= 128 ? launch_tree<T, 4>(p, stream) : launch_tree<T, 8>(p, stream);
+}
+
+}  // namespace einf
+
+using namespace einf;
+
+extern "C" int einf_tree_attention_rows() { return kRows; }
+
+// part_o: [2 * ctas][32][padded] floats, part_ml: [2 * ctas][32][2], notes: [ctas][4]; padded: size rounded up to four.
+extern "C" int einf_tree_attention(const void* q, const void* k_cache, const void* v_cache, int dtype, const int* block_table,
+                                   const int* q_start, const int* cached_lens, const void* mask, const int* positions, void* out,
+                                   float* part_o, float* part_ml, int* notes, int requests, int tokens, int heads, int kv_heads,
+                                   int size, int page_size, int num_pages, int table_width, int words, int window, float scale,
+                                   float softcap, int ctas, int min_chunk, int* status, cudaStream_t stream) {
+  if (requests == 0 || tokens == 0) return 0;
+  if (size < 1 || size > 256 || ctas < 1 || min_chunk < 1 || kv_heads < 1 || heads % kv_heads || page_size < 1 || words < 1 ||
+      (window > 0 && !positions))
+    return (int)cudaErrorInvalidValue;
+  TreeParams p = {};
+  p.q = q;
+  p.k_cache = k_cache;
+  p.v_cache = v_cache;
+  p.block_table = block_table;
+  p.q_start = q_start;
+  p.cached_lens = cached_lens;
+  p.mask = static_cast<const uint32_t*>(mask);
+  p.positions = positions;
+  p.out = out;
+  p.part_o = part_o;
+  p.part_ml = reinterpret_cast<float2*>(part_ml);
+  p.notes = reinterpret_cast<int4*>(notes);
+  p.status = status;
+  p.requests = requests;
+  p.tokens = tokens;
+  p.heads = heads;
+  p.kv_heads = kv_heads;
+  p.size = size;
+  p.page_size = page_size;
+  p.num_pages = num_pages;
+  p.table_width = table_width;
+  p.words = words;
+  p.window = window;
+  p.scale = scale;
+  p.softcap = softcap;
+  p.unit_heads = heads / kv_heads < kRows ? heads / kv_heads : kRows;
+  p.unit_nodes = kRows / p.unit_heads;
+  p.unit_rows = kRows;
+  p.padded = (size + 3) & ~3;
+  p.tile_keys = kKeys;
+  p.min_chunk = min_chunk;
+  p.ctas = ctas;
+  EINF_DISPATCH_2(dtype, T, return dispatch_tree<T>(p, stream);)
+  return 0;
+}

@@ -21,6 +21,7 @@ enum Status : int {
   kStatusBadToken = 1,      // a token id outside the embedding table
   kStatusBadPage = 2,       // a block-table entry outside the page pool
   kStatusWaitExpired = 4,   // a bounded wait on a barrier gave up
+  kStatusBadIndex = 8,      // an index outside what it points into (a mask's row, a node of a path)
 };
 
 template <typename T>

@@ -321,4 +321,6 @@ class ModelRunner:
             faults.append("a block-table entry outside the page pool")
         if status & ops.STATUS_WAIT_EXPIRED:
             faults.append("a bounded wait inside a kernel expired")
+        if status & ops.STATUS_BAD_INDEX:
+            faults.append("an index outside what it points into")
         raise StepError("the step's kernels reported: " + "; ".join(faults or [f"status {status}"]))

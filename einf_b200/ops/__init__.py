@@ -26,6 +26,7 @@ _DTYPE_CODES = {torch.float32: FLOAT32, torch.bfloat16: BFLOAT16}
 STATUS_BAD_TOKEN = 1
 STATUS_BAD_PAGE = 2
 STATUS_WAIT_EXPIRED = 4
+STATUS_BAD_INDEX = 8
 
 MAX_HEAD_SIZE = 256
 #: the general attention kernel alone takes larger heads (a latent cache row)
@@ -3492,10 +3493,317 @@ def sample(
     )
 
 
+# ---------------------------------------------------------------------------
+# Drafted trees.  A request's draft is a tree of nodes behind its cached tokens: node 0 is the last token that was answered,
+# every other node hangs on one before it.  The nodes of all requests are packed (``q_start``), node ``k`` of a request is
+# run as its token number ``cached_lens + k`` (so ``rope_kv_write`` puts its key and value at that place) at the position
+# ``cached_lens + depth``; ``tree_attention`` lets it see its ancestors alone, ``shape_logits`` counts their tokens,
+# ``accept_drafts`` walks the tree by the tokens that the model gave, and ``move_accepted`` closes the gaps in the cache.
+
+
+def _here(device: torch.device, *tensors: Optional[torch.Tensor]) -> None:
+    """Every tensor lies on ``device``, and a launch goes there."""
+    if device.type != "cuda":
+        raise KernelError(f"a tensor is on {device}: the kernels run on a CUDA device only and have no CPU path")
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors on {t.device} and on {device} in one call")
+    if device.index != _get_device():
+        raise ValueError(f"the tensors are on {device}, which is not the current device")
+
+
+def _check_mask(tree_mask: torch.Tensor, rows: int) -> int:
+    """Words of a node's mask."""
+    if tree_mask.dtype != torch.int64 or tree_mask.dim() != 2 or tree_mask.shape[0] != rows or tree_mask.shape[1] < 1:
+        raise ValueError(f"tree_mask must be int64 [{rows}, words], got {tree_mask.dtype} {tuple(tree_mask.shape)}")
+    return tree_mask.shape[1]
+
+
+#: keys and rows that a CTA of the tree attention kernel with 32-bit products works on at a time
+TREE_KEYS, TREE_ROWS = 32, 32
+
+
+def _tree_ctas(requests: int, units: int, tiles: int, device_ctas: int, min_chunk: int) -> int:
+    """CTAs of a tree attention launch: what the device holds at once, or fewer where the requests' most key tiles, at
+    least ``min_chunk`` to a CTA, do not need as many."""
+    return max(1, min(device_ctas, -(-requests * units * tiles // min_chunk)))
+
+
+def tree_attention(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    q_start: torch.Tensor,
+    cached_lens: torch.Tensor,
+    tree_mask: torch.Tensor,
+    out: torch.Tensor,
+    scale: float,
+    status: torch.Tensor,
+    positions: Optional[torch.Tensor] = None,
+    window: Optional[int] = None,
+    softcap: Optional[float] = None,
+    max_nodes: Optional[int] = None,
+    max_cached: Optional[int] = None,
+) -> None:
+    """Attention of drafted nodes over the paged cache.  ``q`` and ``out`` are ``[tokens, heads, head_size]``, float32 or
+    bfloat16 like the caches ``[pages, kv_heads, page_size, head_size]`` (heads of up to 256); request ``r`` has the nodes
+    ``q_start[r] .. q_start[r + 1] - 1`` (int32), ``cached_lens[r]`` (int32) cached tokens and, behind them in its pages,
+    its nodes' keys and values.  A node sees every cached token and node ``k`` of its own request where bit ``k % 64`` of
+    ``tree_mask[node, k // 64]`` (int64) is set: its ancestors and itself, in a tree.  With ``window`` it sees
+    only what stands less than ``window`` before its position (``positions``, int32 per node, then needed; nodes
+    stand at their request's cached length at least).  ``softcap`` as in :func:`paged_attention_generic`.  A node that sees
+    nothing gets zeros, rows that belong to no request keep what they hold.
+
+    Scores, softmax and sums are 32-bit.  ``max_nodes`` and ``max_cached``, the most nodes and cached tokens of a request as
+    far as the caller knows them, only size the launch: any request's nodes are computed whole."""
+    tokens, heads, size = q.shape
+    num_pages, kv_heads, page_size, cache_size = k_cache.shape
+    requests = cached_lens.shape[0]
+    if out.shape != q.shape or v_cache.shape != k_cache.shape or cache_size != size:
+        raise ValueError(f"q {tuple(q.shape)}, out {tuple(out.shape)} and caches {tuple(k_cache.shape)}, {tuple(v_cache.shape)} do not "
+                         "fit together")
+    if not q.dtype == k_cache.dtype == v_cache.dtype == out.dtype:
+        raise TypeError("q, caches and out must have one dtype")
+    if kv_heads < 1 or heads % kv_heads:
+        raise UnsupportedSize(f"{heads} query heads are not a multiple of {kv_heads} key/value heads")
+    if not 1 <= size <= MAX_HEAD_SIZE:
+        raise UnsupportedSize(f"tree attention takes heads of up to {MAX_HEAD_SIZE}, not {size}")
+    if q_start.shape != (requests + 1,) or block_table.dim() != 2 or block_table.shape[0] < requests:
+        raise ValueError(f"q_start must hold {requests + 1} entries and block_table a row for each of {requests} requests")
+    words = _check_mask(tree_mask, tokens)
+    if window is not None and window < 1:
+        raise ValueError(f"a window holds at least one token, not {window}")
+    if softcap is not None and not softcap > 0:
+        raise ValueError(f"a soft cap is positive, not {softcap}")
+    if not scale > 0:
+        raise ValueError(f"the scale is positive, not {scale}")
+    if window:
+        if positions is None or positions.shape != (tokens,):
+            raise ValueError("a window needs the position of every node")
+    else:
+        positions = None
+    _here(q.device, k_cache, v_cache, block_table, q_start, cached_lens, tree_mask, out, status, positions)
+    if tokens == 0 or requests == 0:
+        return
+    group, width = heads // kv_heads, block_table.shape[1]
+    nodes = min(tokens, max(1, int(max_nodes))) if max_nodes is not None else min(tokens, 64 * words)
+    context = width * page_size
+    if max_cached is not None:
+        context = min(context, max(0, int(max_cached)) + nodes)
+    if window:
+        context = min(context, window + nodes + page_size)
+    unit_heads = min(group, TREE_ROWS)
+    units = kv_heads * -(-group // unit_heads) * -(-nodes // (TREE_ROWS // unit_heads))
+    ctas = _tree_ctas(requests, units, -(-context // TREE_KEYS), 3 * _sm_count(), 2)
+    shares, padded = 2 * ctas * TREE_ROWS, -(-size // 4) * 4
+    scratch = torch.empty(4 * ctas + shares * (padded + 2), dtype=torch.float32, device=q.device)
+    notes = scratch.data_ptr()
+    sums = notes + 16 * ctas
+    fn = _fn("einf_tree_attention", [c_void_p] * 3 + [c_int] + [c_void_p] * 9 + [c_int] * 10 + [c_float] * 2 + [c_int] * 2 + [c_void_p] * 2)
+    _check(
+        fn(_dev(q, "q"), _dev(k_cache, "k_cache"), _dev(v_cache, "v_cache"), _code(q), _opt(block_table, "block_table", torch.int32),
+           _opt(q_start, "q_start", torch.int32), _opt(cached_lens, "cached_lens", torch.int32), _dev(tree_mask, "tree_mask"),
+           _opt(positions, "positions", torch.int32), _dev(out, "out"), sums, sums + 4 * shares * padded, notes, requests, tokens,
+           heads, kv_heads, size, page_size, num_pages, width, words, int(window or 0), float(scale), float(softcap or 0.0), ctas, 2,
+           _opt(status, "status", torch.int32), _stream()),
+        "tree_attention",
+    )
+
+
+def shape_logits(
+    logits: torch.Tensor,
+    out: torch.Tensor,
+    row_start: Optional[torch.Tensor],
+    status: torch.Tensor,
+    history: Optional[torch.Tensor] = None,
+    history_lens: Optional[torch.Tensor] = None,
+    prompt_lens: Optional[torch.Tensor] = None,
+    repetition: Optional[torch.Tensor] = None,
+    presence: Optional[torch.Tensor] = None,
+    frequency: Optional[torch.Tensor] = None,
+    node_tokens: Optional[torch.Tensor] = None,
+    tree_mask: Optional[torch.Tensor] = None,
+    bias_ids: Optional[torch.Tensor] = None,
+    bias: Optional[torch.Tensor] = None,
+    allowed: Optional[torch.Tensor] = None,
+    allowed_rows: Optional[torch.Tensor] = None,
+) -> None:
+    """Penalties, biases and masks on rows of logits (float32 ``[rows, vocab]``; ``out`` may be ``logits``), before
+    :func:`argmax` or :func:`sample`.  Request ``r`` has the rows ``row_start[r] .. row_start[r + 1] - 1`` (int32; None: one
+    row each).  With ``c`` the number of times a token was answered, of a logit ``x``
+
+    ``x / repetition[r]`` if positive, else ``x * repetition[r]``, where the token stands in the prompt or ``c > 0``; then
+    ``x - (frequency[r] * c + presence[r] * (c > 0))``; then ``x + bias``; then ``-inf`` where the mask has no bit.
+
+    ``history`` (int32 ``[requests, capacity]``) holds the first ``history_lens[r]`` tokens of a request, of which the first
+    ``prompt_lens[r]`` (None: none) are its prompt.  For drafted trees ``node_tokens`` (int32 ``[rows]``) are the rows' own
+    tokens and ``tree_mask`` their ancestors and themselves, as in :func:`tree_attention`: these count as answered.
+    ``bias_ids`` (int32 ``[requests, n]``, negative: none) and ``bias`` (float32) are added to single tokens, the last entry
+    of a token that stands twice.  ``allowed`` (int32 ``[masks, (vocab + 31) // 32]``) has bit ``v % 32`` of word
+    ``v // 32`` set for tokens that may come; row ``i`` has mask ``i``, or mask ``allowed_rows[i]`` (int32, negative: none).
+    A token outside the vocabulary and a mask that is not there set the status word and count for nothing."""
+    rows, vocab = logits.shape
+    if logits.dtype != torch.float32 or out.dtype != torch.float32 or out.shape != logits.shape:
+        raise TypeError("shape_logits takes float32 logits and a result like them")
+    requests = rows if row_start is None else row_start.shape[0] - 1
+    if requests < 0:
+        raise ValueError("row_start must hold one more entry than there are requests")
+    if (history is None) != (history_lens is None) or (prompt_lens is not None and history is None):
+        raise ValueError("a history comes with its lengths")
+    if (node_tokens is None) != (tree_mask is None):
+        raise ValueError("the nodes' tokens come with their mask")
+    if (bias_ids is None) != (bias is None):
+        raise ValueError("bias_ids come with bias")
+    for t, name in ((history_lens, "history_lens"), (prompt_lens, "prompt_lens"), (repetition, "repetition"), (presence, "presence"),
+                    (frequency, "frequency")):
+        if t is not None and t.shape != (requests,):
+            raise ValueError(f"{name} is {tuple(t.shape)}, expected ({requests},)")
+    capacity = words = biases = masks = mask_words = 0
+    if history is not None:
+        if history.dim() != 2 or history.shape[0] != requests:
+            raise ValueError(f"history is {tuple(history.shape)}, expected [{requests}, capacity]")
+        capacity = history.shape[1]
+    if node_tokens is not None:
+        if node_tokens.shape != (rows,):
+            raise ValueError(f"node_tokens is {tuple(node_tokens.shape)}, expected ({rows},)")
+        words = _check_mask(tree_mask, rows)
+    if bias is not None:
+        if bias.dim() != 2 or bias.shape[0] != requests or bias_ids.shape != bias.shape:
+            raise ValueError(f"bias_ids {tuple(bias_ids.shape)} and bias {tuple(bias.shape)} must be [{requests}, n]")
+        biases = bias.shape[1]
+    if allowed is not None:
+        masks, mask_words = allowed.shape
+        if mask_words != -(-vocab // 32):
+            raise ValueError(f"allowed has {mask_words} words a mask, expected {-(-vocab // 32)}")
+        if (allowed_rows is None and masks != rows) or (allowed_rows is not None and allowed_rows.shape != (rows,)):
+            raise ValueError("allowed has a mask per row, or allowed_rows says which mask a row has")
+    elif allowed_rows is not None:
+        raise ValueError("allowed_rows needs allowed")
+    _here(logits.device, out, row_start, status, history, history_lens, prompt_lens, repetition, presence, frequency, node_tokens,
+          tree_mask, bias_ids, bias, allowed, allowed_rows)
+    if rows == 0 or requests == 0 or vocab == 0:
+        return
+    if requests > 65535:
+        raise UnsupportedSize(f"shape_logits takes up to 65535 requests, not {requests}")
+    piece, row_ways = _shape_pieces(rows, requests, vocab)
+    fn = _fn("einf_shape_logits", [c_void_p] * 15 + [c_int] * 10 + [c_void_p] * 2)
+    _check(
+        fn(_dev(logits, "logits"), _dev(out, "out"), _opt(row_start, "row_start", torch.int32), _opt(history, "history", torch.int32),
+           _opt(history_lens, "history_lens", torch.int32), _opt(prompt_lens, "prompt_lens", torch.int32),
+           _opt(repetition, "repetition", torch.float32), _opt(presence, "presence", torch.float32),
+           _opt(frequency, "frequency", torch.float32), _opt(node_tokens, "node_tokens", torch.int32),
+           _opt(tree_mask, "tree_mask", torch.int64), _opt(bias_ids, "bias_ids", torch.int32), _opt(bias, "bias", torch.float32),
+           _opt(allowed, "allowed", torch.int32), _opt(allowed_rows, "allowed_rows", torch.int32), rows, vocab, requests, capacity,
+           words, biases, masks, mask_words, piece, row_ways, _opt(status, "status", torch.int32), _stream()),
+        "shape_logits",
+    )
+
+
+def _shape_pieces(rows: int, requests: int, vocab: int) -> tuple[int, int]:
+    """Places of the vocabulary that a CTA of :func:`shape_logits` has, and how many CTAs take a request's rows in turn."""
+    piece = 4096
+    while piece > 1024 and requests * -(-vocab // piece) < 4 * _sm_count():
+        piece //= 2
+    ways = 1
+    while ways < -(-rows // requests) and ways * requests * -(-vocab // piece) < 4 * _sm_count():
+        ways *= 2
+    return piece, ways
+
+
+def accept_drafts(node_tokens: torch.Tensor, targets: torch.Tensor, parents: torch.Tensor, q_start: torch.Tensor,
+                  path: torch.Tensor, answer: torch.Tensor, counts: torch.Tensor) -> None:
+    """The longest path from the root (node 0) of every request's tree on which each node's token is the one that the model
+    gave behind its parent: ``targets[n]``, the argmax or the sample of node ``n``'s logits, so that what is answered is
+    what decoding token by token would answer.  All int32: ``node_tokens``, ``targets`` and ``parents`` ``[rows]`` (a parent is
+    an index within the request, before the node's own; a node with any other, but the root, is not reached), of children that agree the first is
+    taken.  ``path[r, i]`` becomes the path's nodes and ``answer[r, i]`` the targets behind them (the tokens of this step: the
+    last is the next root), -1 behind the last, ``counts[r]`` how many there are; a path ends where its row
+    (``[requests, depth]``) is full."""
+    rows, requests = node_tokens.shape[0], counts.shape[0]
+    if targets.shape != node_tokens.shape or parents.shape != node_tokens.shape or node_tokens.dim() != 1:
+        raise ValueError("node_tokens, targets and parents must be [rows]")
+    if q_start.shape != (requests + 1,):
+        raise ValueError(f"q_start must hold {requests + 1} entries")
+    if path.dim() != 2 or path.shape[0] != requests or path.shape[1] < 1 or answer.shape != path.shape:
+        raise ValueError(f"path {tuple(path.shape)} and answer {tuple(answer.shape)} must be [{requests}, depth]")
+    _here(node_tokens.device, targets, parents, q_start, path, answer, counts)
+    if requests == 0:
+        return
+    fn = _fn("einf_accept_drafts", [c_void_p] * 7 + [c_int] * 3 + [c_void_p])
+    _check(
+        fn(_opt(node_tokens, "node_tokens", torch.int32), _opt(targets, "targets", torch.int32), _opt(parents, "parents", torch.int32),
+           _opt(q_start, "q_start", torch.int32), _opt(path, "path", torch.int32), _opt(answer, "answer", torch.int32),
+           _opt(counts, "counts", torch.int32), rows, requests, path.shape[1], _stream()),
+        "accept_drafts",
+    )
+
+
+class CacheRows:
+    """The cache tensors (``[pages, kv_heads, page_size, size]``; keys and values of every layer that share one
+    block table) whose rows :func:`move_accepted` moves in one launch, looked at once."""
+
+    MAX_TENSORS = 192
+
+    def __init__(self, caches: Sequence[torch.Tensor]) -> None:
+        self.caches = tuple(caches)
+        if not self.caches:
+            raise ValueError("CacheRows needs at least one cache tensor")
+        first = self.caches[0]
+        self.device, self.num_pages, self.page_size = first.device, first.shape[0], first.shape[2]
+        unit = 16
+        for t in self.caches:
+            if t.dim() != 4 or (t.shape[0], t.shape[2]) != (self.num_pages, self.page_size):
+                raise ValueError(f"caches must be [{self.num_pages}, kv_heads, {self.page_size}, size], got {tuple(t.shape)}")
+            if t.device != self.device:
+                raise ValueError(f"cache tensors on {t.device} and on {self.device}")
+            if t.numel() == 0:
+                raise ValueError("a cache tensor is empty")
+            _code(t)
+            while _dev(t, "cache") % unit or t.shape[3] * t.element_size() % unit:
+                unit //= 2
+        self.unit = unit
+        self._parts = []
+        for start in range(0, len(self.caches), self.MAX_TENSORS):
+            part = self.caches[start:start + self.MAX_TENSORS]
+            n = len(part)
+            self._parts.append((
+                (c_void_p * n)(*(t.data_ptr() for t in part)), (c_int * n)(*(t.shape[1] for t in part)),
+                (c_int * n)(*(t.shape[3] * t.element_size() // unit for t in part)), n,
+            ))
+
+
+def move_accepted(caches: CacheRows, block_table: torch.Tensor, cached_lens: torch.Tensor, path: torch.Tensor, counts: torch.Tensor,
+                  status: torch.Tensor) -> None:
+    """Close the gaps that refused nodes leave in the cache: in every tensor of ``caches`` the row at place
+    ``cached_lens[r] + path[r, i]`` of request ``r`` goes to place ``cached_lens[r] + i``, for ``i = 1 .. counts[r] - 1`` (all
+    int32, as :func:`accept_drafts` writes them), as if every row were read before any is written.  A path's nodes rise; one
+    that does not, or a place without a page, sets the status word and is not moved."""
+    requests = cached_lens.shape[0]
+    if path.dim() != 2 or path.shape[0] != requests or counts.shape != (requests,):
+        raise ValueError(f"path must be [{requests}, depth] and counts ({requests},)")
+    if block_table.dim() != 2 or block_table.shape[0] < requests:
+        raise ValueError(f"block_table needs a row for each of {requests} requests")
+    _here(caches.device, block_table, cached_lens, path, counts, status)
+    if requests == 0 or path.shape[1] < 2:
+        return
+    fn = _fn("einf_move_accepted", [c_void_p] * 3 + [c_int] * 2 + [c_void_p] * 4 + [c_int] * 5 + [c_void_p] * 2)
+    table, lens = _opt(block_table, "block_table", torch.int32), _opt(cached_lens, "cached_lens", torch.int32)
+    steps, kept, word = _opt(path, "path", torch.int32), _opt(counts, "counts", torch.int32), _opt(status, "status", torch.int32)
+    for bases, heads, units, count in caches._parts:
+        _check(
+            fn(bases, heads, units, count, caches.unit, table, lens, steps, kept, requests, path.shape[1], caches.page_size,
+               caches.num_pages, block_table.shape[1], word, _stream()),
+            "move_accepted",
+        )
+
+
 __all__ = [
+    "CacheRows",
     "KernelError",
     "KernelLibraryError",
     "UnsupportedSize",
+    "accept_drafts",
     "add_bias",
     "add_rmsnorm",
     "argmax",
@@ -3505,6 +3813,7 @@ __all__ = [
     "gemm_tcgen05",
     "gemm_tcgen05_splits",
     "linear",
+    "move_accepted",
     "paged_attention_generic",
     "paged_decode_attention",
     "decode_plan",
@@ -3516,6 +3825,8 @@ __all__ = [
     "project",
     "rope_kv_write",
     "sample",
+    "shape_logits",
     "silu_mul",
+    "tree_attention",
     "zero_fresh_state",
 ]

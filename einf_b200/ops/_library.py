@@ -78,6 +78,10 @@ LAUNCHERS = {
     "einf_argmax": "sampling",
     "einf_sample": "sampling",
     "einf_report": "sampling",
+    "einf_tree_attention": "attention_tree",
+    "einf_shape_logits": "logits",
+    "einf_accept_drafts": "drafts",
+    "einf_move_accepted": "drafts",
 }
 
 

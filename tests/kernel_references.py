@@ -785,3 +785,123 @@ def emulate_kernels():
         for name, function in saved_ops.items():
             setattr(ops, name, function)
         ModelRunner._check_device, ModelRunner._guard, ModelRunner.synchronize, ModelRunner._graphable = saved
+
+
+# ---------------------------------------------------------------------------
+# Drafted trees, in 64 bits and in loops.
+def _node_bits(tree_mask, row):
+    return sum((int(w) & (1 << 64) - 1) << 64 * i for i, w in enumerate(tree_mask[row].tolist()))
+
+
+def tree_visible(table, q_start, cached_lens, tree_mask, page, positions=None, window=None):
+    """Per request: (rows, the pages' places of its keys in order, which keys its nodes see)."""
+    for r, cached in enumerate(cached_lens.tolist()):
+        first, last = int(q_start[r]), int(q_start[r + 1])
+        count = cached + last - first
+        slots = [int(table[r, j // page]) * page + j % page for j in range(count)]
+        seen = torch.zeros((last - first, count), dtype=torch.bool)
+        for i in range(last - first):
+            bits = _node_bits(tree_mask, first + i)
+            for j in range(count):
+                seen[i, j] = j < cached or bool(bits >> (j - cached) & 1)
+                if window:
+                    here = max(int(positions[first + i]), cached)
+                    there = j if j < cached else max(int(positions[first + j - cached]), cached)
+                    seen[i, j] &= here - there < window
+        yield range(first, last), slots, seen
+
+
+def tree_attention(q, k_cache, v_cache, table, q_start, cached_lens, tree_mask, scale, positions=None, window=None, softcap=None):
+    """The mixed rows, and how far a sum in 32 bits may be off: both ``[tokens, heads, head_size]`` in 64 bits, NaN in
+    rows of no request."""
+    kv_heads, page, size = k_cache.shape[1], k_cache.shape[2], q.shape[2]
+    out = torch.full(q.shape, float("nan"), dtype=torch.float64)
+    bound = out.clone()
+    keys = k_cache.double().cpu().permute(0, 2, 1, 3).reshape(-1, kv_heads, size)
+    values = v_cache.double().cpu().permute(0, 2, 1, 3).reshape(-1, kv_heads, size)
+    queries, eps = q.double().cpu(), 2.0 ** -24
+    for rows, slots, seen in tree_visible(table.cpu(), q_start.cpu(), cached_lens.cpu(), tree_mask.cpu(), page, positions, window):
+        for i, row in enumerate(rows):
+            at = [s for s, visible in zip(slots, seen[i].tolist()) if visible]
+            for h in range(q.shape[1]):
+                k, v = keys[at][:, h // (q.shape[1] // kv_heads)], values[at][:, h // (q.shape[1] // kv_heads)]
+                raw = k @ queries[row, h] * scale
+                s = softcap * torch.tanh(raw / softcap) if softcap else raw
+                if not at:
+                    out[row, h], bound[row, h] = 0.0, 0.0
+                    continue
+                p = torch.softmax(s, 0)
+                out[row, h] = p @ v
+                # A score is a sum of `size` rounded products; a weight is 2^x with x rounded and the exponential's two
+                # units; sums of so many weights and products, rescaled once per tile, and one division.
+                score = (size + 4) * eps * (k.abs() @ queries[row, h].abs() * scale) + 8 * eps * (softcap or 0.0)
+                weight = score + eps * (s - s.max()).abs() * 2 + 4 * eps
+                worst = float(weight.max()) if weight.numel() else 0.0
+                bound[row, h] = (weight[:, None] * p[:, None] * v.abs()).sum(0) + (p[:, None] * v.abs()).sum(0) * (
+                    worst + (2 * len(at) + len(at) / 16 + 8) * eps)
+    return out, bound
+
+
+def shape_logits(logits, row_start, history=None, history_lens=None, prompt_lens=None, repetition=None, presence=None, frequency=None,
+                 node_tokens=None, tree_mask=None, bias_ids=None, bias=None, allowed=None, allowed_rows=None):
+    """In 64 bits; rows of no request are NaN."""
+    rows, vocab = logits.shape
+    starts = list(range(rows + 1)) if row_start is None else row_start.tolist()
+    out = torch.full((rows, vocab), float("nan"), dtype=torch.float64)
+    for r in range(len(starts) - 1):
+        tokens = history[r, :int(history_lens[r])].tolist() if history is not None else []
+        prompt = int(prompt_lens[r]) if prompt_lens is not None else 0
+        rep, pres, freq = (float(t[r]) if t is not None else off for t, off in ((repetition, 1.0), (presence, 0.0), (frequency, 0.0)))
+        biases = {}
+        if bias is not None:
+            biases = {i: b for i, b in zip(bias_ids[r].tolist(), bias[r].tolist()) if 0 <= i < vocab}
+        for row in range(starts[r], starts[r + 1]):
+            answered = tokens[prompt:]
+            if node_tokens is not None:
+                bits = _node_bits(tree_mask, row)
+                answered = answered + [int(node_tokens[starts[r] + k]) for k in range(starts[r + 1] - starts[r]) if bits >> k & 1]
+            counts = {}
+            for t in answered:
+                counts[t] = counts.get(t, 0) + 1
+            mask = row if allowed_rows is None else int(allowed_rows[row])
+            x = logits[row].double().cpu().tolist()
+            for v in range(vocab):
+                c = counts.get(v, 0)
+                if c or v in tokens[:prompt]:
+                    x[v] = x[v] / rep if x[v] > 0 else x[v] * rep
+                if c:
+                    x[v] -= freq * c + pres
+                x[v] += biases.get(v, 0.0)
+                if allowed is not None and 0 <= mask < allowed.shape[0] and not int(allowed[mask, v // 32]) >> v % 32 & 1:
+                    x[v] = float("-inf")
+            out[row] = torch.tensor(x, dtype=torch.float64)
+    return out
+
+
+def accept_drafts(node_tokens, targets, parents, q_start, depth):
+    path, answer, counts = [], [], []
+    starts = q_start.tolist()
+    for a, b in zip(starts, starts[1:]):
+        walk = [0] if b > a else []
+        while walk and len(walk) < depth:
+            after = [k for k in range(walk[-1] + 1, b - a)
+                     if int(parents[a + k]) == walk[-1] and int(node_tokens[a + k]) == int(targets[a + walk[-1]])]
+            if not after:
+                break
+            walk.append(after[0])
+        path.append(walk + [-1] * (depth - len(walk)))
+        answer.append([int(targets[a + k]) for k in walk] + [-1] * (depth - len(walk)))
+        counts.append(len(walk))
+    return path, answer, counts
+
+
+def move_accepted(caches, table, cached_lens, path, counts):
+    """What the caches hold afterwards."""
+    after = [c.clone() for c in caches]
+    page = caches[0].shape[2]
+    for r, cached in enumerate(cached_lens.tolist()):
+        for i in range(1, int(counts[r])):
+            a, b = cached + int(path[r, i]), cached + i
+            for before, c in zip(caches, after):
+                c[int(table[r, b // page]), :, b % page] = before[int(table[r, a // page]), :, a % page]
+    return after

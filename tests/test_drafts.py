@@ -1,0 +1,188 @@
+"""What the operators of drafted trees refuse, how their launches are cut, on a machine without a GPU."""
+import pytest
+import torch
+
+from einf_b200 import ops
+
+
+@pytest.fixture
+def on_this_machine(monkeypatch):
+    """Tensors of the CPU pass for tensors of the current device, and a launch is recorded instead of made."""
+    calls = []
+
+    def fn(symbol, argtypes, variant=""):
+        def launch(*args):
+            assert len(args) == len(argtypes)
+            calls.append(symbol)
+            return 0
+        return launch
+
+    def pointer(t, name="", dtype=None):
+        if t is None:
+            return 0
+        if dtype is not None and t.dtype != dtype:
+            raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+        return t.data_ptr()
+
+    monkeypatch.setattr(ops, "_fn", fn)
+    monkeypatch.setattr(ops, "_dev", pointer)
+    monkeypatch.setattr(ops, "_opt", pointer)
+    monkeypatch.setattr(ops, "_here", lambda device, *tensors: None)
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(ops, "_sm_count", lambda: 148)
+    return calls
+
+
+def ints(*shape):
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+def attention_arguments(**change):
+    given = dict(
+        q=torch.zeros(5, 4, 48), k_cache=torch.zeros(6, 2, 4, 48), v_cache=torch.zeros(6, 2, 4, 48), block_table=ints(2, 3),
+        q_start=ints(3), cached_lens=ints(2), tree_mask=torch.zeros(5, 1, dtype=torch.int64), out=torch.zeros(5, 4, 48), scale=0.1,
+        status=ints(1))
+    given.update(change)
+    return given
+
+
+@pytest.mark.parametrize("change, error", [
+    (dict(out=torch.zeros(5, 4, 32)), ValueError),
+    (dict(v_cache=torch.zeros(6, 2, 8, 48)), ValueError),
+    (dict(out=torch.zeros(5, 4, 48, dtype=torch.bfloat16)), TypeError),
+    (dict(q=torch.zeros(5, 4, 48).half(), k_cache=torch.zeros(6, 2, 4, 48).half(), v_cache=torch.zeros(6, 2, 4, 48).half(),
+          out=torch.zeros(5, 4, 48).half()), TypeError),
+    (dict(q=torch.zeros(5, 3, 48), out=torch.zeros(5, 3, 48)), ops.UnsupportedSize),
+    (dict(q=torch.zeros(5, 4, 260), out=torch.zeros(5, 4, 260), k_cache=torch.zeros(6, 2, 4, 260), v_cache=torch.zeros(6, 2, 4, 260)),
+     ops.UnsupportedSize),
+    (dict(q_start=ints(2)), ValueError),
+    (dict(block_table=ints(1, 3)), ValueError),
+    (dict(tree_mask=ints(5, 1)), ValueError),
+    (dict(tree_mask=torch.zeros(4, 1, dtype=torch.int64)), ValueError),
+    (dict(tree_mask=torch.zeros(5, 0, dtype=torch.int64)), ValueError),
+    (dict(window=0), ValueError),
+    (dict(window=7), ValueError),
+    (dict(window=7, positions=ints(4)), ValueError),
+    (dict(softcap=0.0), ValueError),
+    (dict(softcap=float("nan")), ValueError),
+    (dict(scale=0.0), ValueError),
+    (dict(cached_lens=torch.zeros(2, dtype=torch.int64)), TypeError),
+    (dict(status=torch.zeros(1)), TypeError),
+    (dict(q=torch.zeros(4, 5, 48).transpose(0, 1)), ValueError),
+])
+def test_tree_attention_refuses(on_this_machine, change, error):
+    with pytest.raises(error):
+        ops.tree_attention(**attention_arguments(**change))
+    assert on_this_machine == []
+
+
+def test_tree_attention_launches(on_this_machine):
+    ops.tree_attention(**attention_arguments())
+    assert on_this_machine == ["einf_tree_attention"]
+    ops.tree_attention(**attention_arguments(window=3, positions=ints(5), softcap=5.0, max_nodes=3, max_cached=0))
+    none = dict(q=torch.zeros(0, 4, 48), out=torch.zeros(0, 4, 48), tree_mask=torch.zeros(0, 1, dtype=torch.int64))
+    ops.tree_attention(**attention_arguments(**none))
+    assert len(on_this_machine) == 2
+
+
+def logits_arguments(**change):
+    given = dict(logits=torch.zeros(6, 50), out=torch.zeros(6, 50), row_start=ints(3), status=ints(1), history=ints(2, 9),
+                 history_lens=ints(2), prompt_lens=ints(2), repetition=torch.ones(2), presence=torch.ones(2), frequency=torch.ones(2),
+                 node_tokens=ints(6), tree_mask=torch.zeros(6, 1, dtype=torch.int64), bias_ids=ints(2, 3), bias=torch.zeros(2, 3),
+                 allowed=ints(6, 2))
+    given.update(change)
+    return given
+
+
+@pytest.mark.parametrize("change, error", [
+    (dict(logits=torch.zeros(6, 50, dtype=torch.bfloat16)), TypeError),
+    (dict(out=torch.zeros(6, 51)), TypeError),
+    (dict(row_start=ints(0)), ValueError),
+    (dict(history=None), ValueError),
+    (dict(history=None, history_lens=None), ValueError),
+    (dict(history=ints(3, 9)), ValueError),
+    (dict(history_lens=ints(3)), ValueError),
+    (dict(prompt_lens=ints(1)), ValueError),
+    (dict(repetition=torch.ones(6)), ValueError),
+    (dict(repetition=torch.ones(2, dtype=torch.float64)), TypeError),
+    (dict(node_tokens=None), ValueError),
+    (dict(tree_mask=None), ValueError),
+    (dict(node_tokens=ints(5)), ValueError),
+    (dict(bias=None), ValueError),
+    (dict(bias=torch.zeros(2, 4)), ValueError),
+    (dict(allowed=ints(6, 1)), ValueError),
+    (dict(allowed=ints(5, 2)), ValueError),
+    (dict(allowed_rows=ints(5)), ValueError),
+    (dict(allowed=None, allowed_rows=ints(6)), ValueError),
+    (dict(allowed=torch.zeros(6, 2, dtype=torch.int64)), TypeError),
+])
+def test_shape_logits_refuses(on_this_machine, change, error):
+    with pytest.raises(error):
+        ops.shape_logits(**logits_arguments(**change))
+    assert on_this_machine == []
+
+
+def test_shape_logits_launches(on_this_machine):
+    ops.shape_logits(**logits_arguments())
+    ops.shape_logits(torch.zeros(4, 7), torch.zeros(4, 7), None, ints(1))
+    ops.shape_logits(**logits_arguments(allowed=ints(1, 2), allowed_rows=ints(6)))
+    assert on_this_machine == ["einf_shape_logits"] * 3
+    ops.shape_logits(torch.zeros(0, 7), torch.zeros(0, 7), None, ints(1))
+    assert len(on_this_machine) == 3
+
+
+@pytest.mark.parametrize("change, error", [
+    (dict(targets=ints(5)), ValueError),
+    (dict(parents=ints(7)), ValueError),
+    (dict(q_start=ints(2)), ValueError),
+    (dict(path=ints(2, 0), answer=ints(2, 0)), ValueError),
+    (dict(answer=ints(2, 5)), ValueError),
+    (dict(path=ints(3, 4), answer=ints(3, 4)), ValueError),
+    (dict(targets=torch.zeros(6, dtype=torch.int64)), TypeError),
+])
+def test_accept_drafts_refuses(on_this_machine, change, error):
+    given = dict(node_tokens=ints(6), targets=ints(6), parents=ints(6), q_start=ints(3), path=ints(2, 4), answer=ints(2, 4), counts=ints(2))
+    ops.accept_drafts(**given)
+    with pytest.raises(error):
+        ops.accept_drafts(**dict(given, **change))
+    assert on_this_machine == ["einf_accept_drafts"]
+
+
+def test_cache_rows_refuses(on_this_machine):
+    good = [torch.zeros(6, 2, 4, 8), torch.zeros(6, 1, 4, 3, dtype=torch.bfloat16)]
+    assert ops.CacheRows(good[:1]).unit == 16 and ops.CacheRows(good).unit == 2
+    for caches, error in (([], ValueError), ([torch.zeros(6, 2, 4)], ValueError), ([good[0], torch.zeros(5, 2, 4, 8)], ValueError),
+                          ([good[0], torch.zeros(6, 2, 8, 8)], ValueError), ([torch.zeros(6, 2, 4, 8, dtype=torch.int32)], TypeError),
+                          ([torch.zeros(2, 6, 4, 8).transpose(0, 1)], ValueError), ([torch.zeros(0, 2, 4, 8)], ValueError)):
+        with pytest.raises(error):
+            ops.CacheRows(caches)
+
+
+@pytest.mark.parametrize("change, error", [
+    (dict(path=ints(3, 4)), ValueError),
+    (dict(counts=ints(3)), ValueError),
+    (dict(block_table=ints(1, 2)), ValueError),
+    (dict(path=torch.zeros(2, 4, dtype=torch.int64)), TypeError),
+])
+def test_move_accepted_refuses(on_this_machine, change, error):
+    caches = ops.CacheRows([torch.zeros(6, 2, 4, 8)] * 200)
+    given = dict(caches=caches, block_table=ints(2, 2), cached_lens=ints(2), path=ints(2, 4), counts=ints(2), status=ints(1))
+    ops.move_accepted(**given)
+    assert on_this_machine == ["einf_move_accepted"] * 2      # 200 tensors: two launches
+    ops.move_accepted(**dict(given, path=ints(2, 1)))         # a path of roots alone moves nothing
+    with pytest.raises(error):
+        ops.move_accepted(**dict(given, **change))
+    assert len(on_this_machine) == 2
+
+
+def test_tensors_of_the_cpu_are_refused():
+    with pytest.raises(ops.KernelError):
+        ops.tree_attention(**attention_arguments())
+    with pytest.raises(ops.KernelError):
+        ops.shape_logits(**logits_arguments())
+    with pytest.raises(ops.KernelError):
+        ops.accept_drafts(ints(6), ints(6), ints(6), ints(3), ints(2, 4), ints(2, 4), ints(2))
+    with pytest.raises(ops.KernelError):
+        ops.CacheRows([torch.zeros(6, 2, 4, 8)])
