@@ -104,30 +104,6 @@ static_assert(kShareOff % 16 == 0 && kShareOff + (128 * (D + 1) + 2 * 128) * 4 <
 
 // The 256 softmax threads meet (the producer and MMA warps do not take part).
 __device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
-// A raw score (q . k) as the exponent of 2 the softmax takes: score * scale * log2(e), or with a soft cap z
-// z * tanh(score * scale / z) * log2(e).  tanh(x) = 1 - 2 / (2^(2 x log2 e) + 1): the hardware's exponential
-// and reciprocal, good to about 1e-6 of the cap (its own tanh.approx is good to 5e-4 only).
-struct ScoreScale {
-  float scale_log2;     // scale * log2(e)
-  float tanh_in;        // 2 * log2(e) * scale / cap, or 0 without a cap
-  float cap_log2;       // cap * log2(e)
-};
-__device__ __forceinline__ float capped(float raw, const ScoreScale& c) {
-  const float e = fast_exp2(raw * c.tanh_in);
-  float inv;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(e + 1.f));
-  return fmaf(-2.f * c.cap_log2, inv, c.cap_log2);
-}
-__device__ __forceinline__ float score_log2(float raw, const ScoreScale& c) {
-  return c.tanh_in != 0.f ? capped(raw, c) : raw * c.scale_log2;
-}
-__device__ __forceinline__ ScoreScale make_score_scale(float scale, float softcap) {
-  ScoreScale c;
-  c.scale_log2 = scale * 1.4426950408889634f;
-  c.tanh_in = softcap > 0.f ? 2.f * 1.4426950408889634f * scale / softcap : 0.f;
-  c.cap_log2 = softcap * 1.4426950408889634f;
-  return c;
-}
 // The first position a token at `pos` may see: the later of its window's and its chunk's start.
 __device__ __forceinline__ int first_visible(int pos, int window, int chunk) {
   int lo = (window > 0 && pos - window + 1 > 0) ? pos - window + 1 : 0;
@@ -1309,23 +1285,6 @@ paged_decode_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k,
 }  // namespace einf
 
 using namespace einf;
-
-// The cache [pages, kv_heads, page_size, cols] as a four-dimensional map whose box is one head's 64-dim
-// slice of `box_pages` consecutive pages: box_pages * page_size rows land in shared memory one after the other.
-static int make_run_map(CUtensorMap* map, const void* base, long long pages, int kv_heads, int page_size, long long cols,
-                        int box_pages) {
-  EncodeTiledFn encode = encode_tiled();
-  if (!encode) return (int)cudaErrorNotSupported;
-  cuuint64_t dims[4] = {(cuuint64_t)cols, (cuuint64_t)page_size, (cuuint64_t)kv_heads, (cuuint64_t)pages};
-  cuuint64_t strides[3] = {(cuuint64_t)cols * 2, (cuuint64_t)page_size * cols * 2,
-                           (cuuint64_t)kv_heads * page_size * cols * 2};
-  cuuint32_t box[4] = {64, (cuuint32_t)page_size, 1, (cuuint32_t)box_pages};
-  cuuint32_t element_strides[4] = {1, 1, 1, 1};
-  CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box,
-                      element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
-}
 
 extern "C" int einf_attention_tcgen05_head_size() { return D; }
 

@@ -227,39 +227,14 @@ extern "C" int einf_tree_attention(const void* q, const void* k_cache, const voi
   if (size < 1 || size > 256 || ctas < 1 || min_chunk < 1 || kv_heads < 1 || heads % kv_heads || page_size < 1 || words < 1 ||
       (window > 0 && !positions))
     return (int)cudaErrorInvalidValue;
-  TreeParams p = {};
-  p.q = q;
-  p.k_cache = k_cache;
-  p.v_cache = v_cache;
-  p.block_table = block_table;
-  p.q_start = q_start;
-  p.cached_lens = cached_lens;
-  p.mask = static_cast<const uint32_t*>(mask);
-  p.positions = positions;
-  p.out = out;
-  p.part_o = part_o;
-  p.part_ml = reinterpret_cast<float2*>(part_ml);
-  p.notes = reinterpret_cast<int4*>(notes);
-  p.status = status;
-  p.requests = requests;
-  p.tokens = tokens;
-  p.heads = heads;
-  p.kv_heads = kv_heads;
-  p.size = size;
-  p.page_size = page_size;
-  p.num_pages = num_pages;
-  p.table_width = table_width;
-  p.words = words;
-  p.window = window;
-  p.scale = scale;
-  p.softcap = softcap;
+  TreeParams p = tree_params(q, k_cache, v_cache, block_table, q_start, cached_lens, mask, positions, out, part_o, part_ml, notes,
+                             requests, tokens, heads, kv_heads, size, page_size, num_pages, table_width, words, window, scale, softcap,
+                             ctas, min_chunk, status);
   p.unit_heads = heads / kv_heads < kRows ? heads / kv_heads : kRows;
   p.unit_nodes = kRows / p.unit_heads;
   p.unit_rows = kRows;
   p.padded = (size + 3) & ~3;
   p.tile_keys = kKeys;
-  p.min_chunk = min_chunk;
-  p.ctas = ctas;
   EINF_DISPATCH_2(dtype, T, return dispatch_tree<T>(p, stream);)
   return 0;
 }

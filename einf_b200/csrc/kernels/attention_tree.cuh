@@ -40,6 +40,42 @@ struct TreeParams {
   int tile_keys, min_chunk, ctas;
 };
 
+inline TreeParams tree_params(const void* q, const void* k_cache, const void* v_cache, const int* block_table, const int* q_start,
+                              const int* cached_lens, const void* mask, const int* positions, void* out, float* part_o,
+                              float* part_ml, int* notes, int requests, int tokens, int heads, int kv_heads, int size, int page_size,
+                              int num_pages, int table_width, int words, int window, float scale, float softcap, int ctas,
+                              int min_chunk, int* status) {
+  TreeParams p = {};
+  p.q = q;
+  p.k_cache = k_cache;
+  p.v_cache = v_cache;
+  p.block_table = block_table;
+  p.q_start = q_start;
+  p.cached_lens = cached_lens;
+  p.mask = static_cast<const uint32_t*>(mask);
+  p.positions = positions;
+  p.out = out;
+  p.part_o = part_o;
+  p.part_ml = reinterpret_cast<float2*>(part_ml);
+  p.notes = reinterpret_cast<int4*>(notes);
+  p.status = status;
+  p.requests = requests;
+  p.tokens = tokens;
+  p.heads = heads;
+  p.kv_heads = kv_heads;
+  p.size = size;
+  p.page_size = page_size;
+  p.num_pages = num_pages;
+  p.table_width = table_width;
+  p.words = words;
+  p.window = window;
+  p.scale = scale;
+  p.softcap = softcap;
+  p.ctas = ctas;
+  p.min_chunk = min_chunk;
+  return p;
+}
+
 // One request's figures, out of step inputs that are held to what memory there is.
 struct TreeRequest {
   int first, nodes, cached, begin, units, tiles, node_blocks;

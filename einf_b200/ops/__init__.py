@@ -3521,6 +3521,18 @@ def _check_mask(tree_mask: torch.Tensor, rows: int) -> int:
 
 #: keys and rows that a CTA of the tree attention kernel with 32-bit products works on at a time
 TREE_KEYS, TREE_ROWS = 32, 32
+#: the same of the tensor-core kernel, whose units have two such tiles of rows
+TREE_TILE = 128
+
+
+def tree_takes_tcgen05(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor) -> bool:
+    """Whether :func:`tree_attention` runs on the tensor cores: bfloat16 heads and pages that the tcgen05 kernels take, all
+    heads of a key/value head in one tile of rows, rows that start on 16 bytes."""
+    return (
+        q.dtype == torch.bfloat16 and has_tcgen05_attention(q.shape[2], k_cache.shape[2])
+        and q.shape[1] <= TREE_TILE * k_cache.shape[1]
+        and not (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr() | out.data_ptr()) & 15
+    )
 
 
 def _tree_ctas(requests: int, units: int, tiles: int, device_ctas: int, min_chunk: int) -> int:
@@ -3593,20 +3605,26 @@ def tree_attention(
         context = min(context, max(0, int(max_cached)) + nodes)
     if window:
         context = min(context, window + nodes + page_size)
-    unit_heads = min(group, TREE_ROWS)
-    units = kv_heads * -(-group // unit_heads) * -(-nodes // (TREE_ROWS // unit_heads))
-    ctas = _tree_ctas(requests, units, -(-context // TREE_KEYS), 3 * _sm_count(), 2)
-    shares, padded = 2 * ctas * TREE_ROWS, -(-size // 4) * 4
+    if tree_takes_tcgen05(q, k_cache, v_cache, out):
+        symbol, code, keys, min_chunk, device_ctas = "einf_tree_attention_tcgen05", (), TREE_TILE, 2, _sm_count()
+        unit_nodes = 2 * (TREE_TILE // group)
+        rows, units, padded = unit_nodes * group, kv_heads * -(-nodes // unit_nodes), size
+    else:
+        symbol, code, keys, min_chunk, device_ctas = "einf_tree_attention", (_code(q),), TREE_KEYS, 2, 3 * _sm_count()
+        unit_heads = min(group, TREE_ROWS)
+        rows, units, padded = TREE_ROWS, kv_heads * -(-group // unit_heads) * -(-nodes // (TREE_ROWS // unit_heads)), -(-size // 4) * 4
+    ctas = _tree_ctas(requests, units, -(-context // keys), device_ctas, min_chunk)
+    shares = 2 * ctas * rows
     scratch = torch.empty(4 * ctas + shares * (padded + 2), dtype=torch.float32, device=q.device)
     notes = scratch.data_ptr()
     sums = notes + 16 * ctas
-    fn = _fn("einf_tree_attention", [c_void_p] * 3 + [c_int] + [c_void_p] * 9 + [c_int] * 10 + [c_float] * 2 + [c_int] * 2 + [c_void_p] * 2)
+    fn = _fn(symbol, [c_void_p] * 3 + [c_int] * len(code) + [c_void_p] * 9 + [c_int] * 10 + [c_float] * 2 + [c_int] * 2 + [c_void_p] * 2)
     _check(
-        fn(_dev(q, "q"), _dev(k_cache, "k_cache"), _dev(v_cache, "v_cache"), _code(q), _opt(block_table, "block_table", torch.int32),
+        fn(_dev(q, "q"), _dev(k_cache, "k_cache"), _dev(v_cache, "v_cache"), *code, _opt(block_table, "block_table", torch.int32),
            _opt(q_start, "q_start", torch.int32), _opt(cached_lens, "cached_lens", torch.int32), _dev(tree_mask, "tree_mask"),
            _opt(positions, "positions", torch.int32), _dev(out, "out"), sums, sums + 4 * shares * padded, notes, requests, tokens,
-           heads, kv_heads, size, page_size, num_pages, width, words, int(window or 0), float(scale), float(softcap or 0.0), ctas, 2,
-           _opt(status, "status", torch.int32), _stream()),
+           heads, kv_heads, size, page_size, num_pages, width, words, int(window or 0), float(scale), float(softcap or 0.0), ctas,
+           min_chunk, _opt(status, "status", torch.int32), _stream()),
         "tree_attention",
     )
 
