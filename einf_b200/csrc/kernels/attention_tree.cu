@@ -35,10 +35,10 @@ __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams 
   const T* k_cache = static_cast<const T*>(p.k_cache);
   const T* v_cache = static_cast<const T*>(p.v_cache);
   TreeWalk w;
-  bool any = tree_first(p, &w);
-  tree_note(p, w, any);
+  bool any = tree_first(p, blockIdx.x, &w);
+  if (threadIdx.x == 0) tree_note(p, blockIdx.x, w, any);
   const float scale_log2 = p.scale * 1.4426950408889634f, cap_log2 = p.softcap * 1.4426950408889634f;
-  for (; any; any = tree_next(p, &w)) {
+  for (; any; any = tree_next(p, blockIdx.x, &w)) {
     const TreeUnit u = tree_unit(p, w.t, w.unit);
     const int rows = u.nodes * u.heads;
     __syncthreads();
@@ -179,7 +179,6 @@ __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams 
       const int row = warp * kRowsPerWarp + i;
       if (row >= rows) break;
       const size_t at = ((size_t)(w.t.first + u.first_node + row / u.heads) * p.heads + u.first_head + row % u.heads) * p.size;
-      const size_t share = (size_t)w.share * p.unit_rows + row;
       const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
@@ -187,10 +186,10 @@ __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams 
         if (w.whole) {
           if (d < p.size) static_cast<T*>(p.out)[at + d] = from_float<T>(acc[i][e] * inv);
         } else if (d < p.padded) {
-          p.part_o[share * p.padded + d] = acc[i][e];
+          tree_share(p, w.share, row, d)[d & 3] = acc[i][e];
         }
       }
-      if (!w.whole && lane == 0) p.part_ml[share] = make_float2(m[i], l[i]);
+      if (!w.whole && lane == 0) p.part_ml[(size_t)w.share * p.unit_rows + row] = make_float2(m[i], l[i]);
     }
   }
 }
@@ -201,7 +200,7 @@ int launch_tree(const TreeParams& p, cudaStream_t stream) {
   const size_t smem = sizeof(float) * ((size_t)kKeys * (size4 + 4) + kKeys * 32 * VEC + kRows * size4 + kRows * kKeys);
   cudaError_t e = cudaFuncSetAttribute(tree_attention_kernel<T, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
-  e = launch_pdl(tree_attention_kernel<T, VEC>, dim3(p.ctas), dim3(32 * kWarps), smem, stream, p);
+  e = launch_pdl(tree_attention_kernel<T, VEC>, dim3(p.workers), dim3(32 * kWarps), smem, stream, p);
   if (e != cudaSuccess) return (int)e;
   return tree_merge<T>(p, stream);
 }
@@ -215,26 +214,21 @@ int dispatch_tree(const TreeParams& p, cudaStream_t stream) {
 
 using namespace einf;
 
-extern "C" int einf_tree_attention_rows() { return kRows; }
-
-// part_o: [2 * ctas][32][padded] floats, part_ml: [2 * ctas][32][2], notes: [ctas][4]; padded: size rounded up to four.
-extern "C" int einf_tree_attention(const void* q, const void* k_cache, const void* v_cache, int dtype, const int* block_table,
-                                   const int* q_start, const int* cached_lens, const void* mask, const int* positions, void* out,
-                                   float* part_o, float* part_ml, int* notes, int requests, int tokens, int heads, int kv_heads,
-                                   int size, int page_size, int num_pages, int table_width, int words, int window, float scale,
-                                   float softcap, int ctas, int min_chunk, int* status, cudaStream_t stream) {
-  if (requests == 0 || tokens == 0) return 0;
-  if (size < 1 || size > 256 || ctas < 1 || min_chunk < 1 || kv_heads < 1 || heads % kv_heads || page_size < 1 || words < 1 ||
-      (window > 0 && !positions))
-    return (int)cudaErrorInvalidValue;
-  TreeParams p = tree_params(q, k_cache, v_cache, block_table, q_start, cached_lens, mask, positions, out, part_o, part_ml, notes,
-                             requests, tokens, heads, kv_heads, size, page_size, num_pages, table_width, words, window, scale, softcap,
-                             ctas, min_chunk, status);
-  p.unit_heads = heads / kv_heads < kRows ? heads / kv_heads : kRows;
+// call: a TreeCall, on the host; a worker is a CTA.  part_o: [2 * workers][32][padded] floats with the size rounded up to four, part_ml:
+// [2 * workers][32][2], notes: [workers][8].
+extern "C" int einf_tree_attention(const char* call, cudaStream_t stream) {
+  const TreeCall& c = *reinterpret_cast<const TreeCall*>(call);
+  if (c.requests == 0 || c.tokens == 0) return 0;
+  if (!tree_call_fits(c) || c.size > 256 || c.cluster != 1) return (int)cudaErrorInvalidValue;
+  TreeParams p = tree_params(c);
+  p.unit_heads = c.heads / c.kv_heads < kRows ? c.heads / c.kv_heads : kRows;
   p.unit_nodes = kRows / p.unit_heads;
+  p.group = c.heads / c.kv_heads;
+  p.head_blocks = (p.group + p.unit_heads - 1) / p.unit_heads;
   p.unit_rows = kRows;
-  p.padded = (size + 3) & ~3;
-  p.tile_keys = kKeys;
-  EINF_DISPATCH_2(dtype, T, return dispatch_tree<T>(p, stream);)
+  p.padded = (c.size + 3) & ~3;
+  p.tile_shift = 5;
+  static_assert(kKeys == 32, "a tile of keys");
+  EINF_DISPATCH_2(c.dtype, T, return dispatch_tree<T>(p, stream);)
   return 0;
 }

@@ -7,15 +7,29 @@
 //
 // The rows of a unit are those of some nodes x the query heads that share one key/value head, so that a tile of keys is
 // read once for all of them; with trees of 8 to 64 nodes that is what makes the work more than a read of the cache.  A
-// launch's work is the list of all (unit, key tile) pairs in the order of requests, and CTA b takes an equal piece of that
-// list: one long context spreads over the whole device, a batch of unequal ones leaves no CTA behind, and at
-// most the first and the last unit of a piece are shared with other CTAs.  Those go to scratch memory
-// as (sums, reference, sum of weights), and a second launch puts them together in the order of the keys.
+// worker is a CTA or a thread-block cluster.  A launch's work is cut over its workers in one of three ways:
+//   whole    a unit to a worker (a cluster shares its key tiles out among its CTAs), nothing is put together afterwards
+//   aligned  no more units than workers: a unit is cut into pieces of `chunk` key tiles, a piece to a worker
+//   list     more units than workers: worker w takes an equal piece of the list of all (unit, key tile) pairs, in the order
+//            of requests, so that a batch of unequal contexts leaves no worker behind; at most the first and the last
+//            unit of a piece are shared with other workers
+// The first is the caller's choice, who says how many workers there are; between the others the kernel chooses, who
+// knows the lengths.  Shares of a unit go to scratch memory as (sums, reference, sum of weights), and a second
+// launch puts them together in the order of the keys.
 #pragma once
 
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace einf {
+
+// What the second launch has to know where a worker's first piece goes on with a unit that began with another worker.
+struct __align__(16) TreeNote {
+  int places;                // workers less one that have the unit; 0: nothing to put together here
+  int place;                 // which of them this one is, from 0
+  int second;                // the unit was not the first piece of its first worker
+  int token;                 // the unit's first token, its nodes, heads and first head
+  int nodes, heads, first_head, more;
+};
 
 struct TreeParams {
   const void* q;             // [tokens, heads, D]
@@ -27,53 +41,82 @@ struct TreeParams {
   const uint32_t* mask;      // [tokens, 2 * words]: bit k of a row's words is node k of its request
   const int* positions;      // [tokens], read with a window alone
   void* out;                 // [tokens, heads, D]
-  float* part_o;             // [2 * ctas][rows of a unit][padded D]
-  float2* part_ml;           // [2 * ctas][rows of a unit]: reference (exponent of 2) and sum
-  int4* notes;               // [ctas], see tree_note
+  float* part_o;             // [2 * workers][rows of a unit / 32][padded D / 4][32][4]
+  float2* part_ml;           // [2 * workers][rows of a unit]: reference (exponent of 2) and sum
+  TreeNote* notes;           // [workers]
   int* status;
   int requests, tokens, heads, kv_heads, size, page_size, num_pages, table_width, words, window;
   float scale, softcap;
   int unit_heads;            // query heads of a unit: all of a key/value head, or a block of them
   int unit_nodes;            // at most that many nodes
-  int unit_rows;             // rows of a share in scratch memory
+  int unit_rows;             // rows of a share in scratch memory, a multiple of 32
   int padded;                // elements of a share's row
-  int tile_keys, min_chunk, ctas;
+  int tile_shift;            // a tile is 1 << tile_shift keys
+  int group, head_blocks;    // query heads of a key/value head, and blocks of them
+  int min_chunk, workers, cluster, whole;
 };
 
-inline TreeParams tree_params(const void* q, const void* k_cache, const void* v_cache, const int* block_table, const int* q_start,
-                              const int* cached_lens, const void* mask, const int* positions, void* out, float* part_o,
-                              float* part_ml, int* notes, int requests, int tokens, int heads, int kv_heads, int size, int page_size,
-                              int num_pages, int table_width, int words, int window, float scale, float softcap, int ctas,
-                              int min_chunk, int* status) {
+// The arguments of a launcher, as the caller packs them.
+struct TreeCall {
+  const void *q, *k_cache, *v_cache;
+  const int *block_table, *q_start, *cached_lens;
+  const uint32_t* mask;
+  const int* positions;
+  void* out;
+  int* status;
+  float* part_o;
+  float2* part_ml;
+  TreeNote* notes;
+  int requests, tokens, heads, kv_heads, size, page_size, num_pages, table_width, words, window, dtype, workers, cluster, whole, min_chunk;
+  float scale, softcap;
+};
+static_assert(sizeof(TreeCall) == 13 * 8 + 17 * 4 + 4, "as packed");
+
+inline bool tree_call_fits(const TreeCall& c) {
+  return c.workers >= 1 && c.cluster >= 1 && c.min_chunk >= 1 && c.kv_heads >= 1 && c.heads % c.kv_heads == 0 && c.size >= 1 && c.page_size >= 1 && c.words >= 1 &&
+         (c.window <= 0 || c.positions);
+}
+inline TreeParams tree_params(const TreeCall& c) {
   TreeParams p = {};
-  p.q = q;
-  p.k_cache = k_cache;
-  p.v_cache = v_cache;
-  p.block_table = block_table;
-  p.q_start = q_start;
-  p.cached_lens = cached_lens;
-  p.mask = static_cast<const uint32_t*>(mask);
-  p.positions = positions;
-  p.out = out;
-  p.part_o = part_o;
-  p.part_ml = reinterpret_cast<float2*>(part_ml);
-  p.notes = reinterpret_cast<int4*>(notes);
-  p.status = status;
-  p.requests = requests;
-  p.tokens = tokens;
-  p.heads = heads;
-  p.kv_heads = kv_heads;
-  p.size = size;
-  p.page_size = page_size;
-  p.num_pages = num_pages;
-  p.table_width = table_width;
-  p.words = words;
-  p.window = window;
-  p.scale = scale;
-  p.softcap = softcap;
-  p.ctas = ctas;
-  p.min_chunk = min_chunk;
+  p.q = c.q;
+  p.k_cache = c.k_cache;
+  p.v_cache = c.v_cache;
+  p.block_table = c.block_table;
+  p.q_start = c.q_start;
+  p.cached_lens = c.cached_lens;
+  p.mask = c.mask;
+  p.positions = c.positions;
+  p.out = c.out;
+  p.part_o = c.part_o;
+  p.part_ml = c.part_ml;
+  p.notes = c.notes;
+  p.status = c.status;
+  p.requests = c.requests;
+  p.tokens = c.tokens;
+  p.heads = c.heads;
+  p.kv_heads = c.kv_heads;
+  p.size = c.size;
+  p.page_size = c.page_size;
+  p.num_pages = c.num_pages;
+  p.table_width = c.table_width;
+  p.words = c.words;
+  p.window = c.window;
+  p.scale = c.scale;
+  p.softcap = c.softcap;
+  p.workers = c.workers;
+  p.cluster = c.cluster;
+  p.whole = c.whole;
+  p.min_chunk = c.min_chunk;
   return p;
+}
+
+// a / b for a >= 0, b > 0 and a quotient below 2^20.  (The compiler's own takes three times the instructions, and in kernels of a few
+// microseconds an instruction that a launch comes to for the first time costs more to fetch than to run.)
+__device__ __forceinline__ int divide(int a, int b) {
+  int q = (int)__fdividef((float)a, (float)b);
+  const int rest = a - q * b;
+  q += rest >= b ? 1 : 0;
+  return q - (rest < 0 ? 1 : 0);
 }
 
 // One request's figures, out of step inputs that are held to what memory there is.
@@ -94,10 +137,9 @@ __device__ __forceinline__ TreeRequest tree_request(const TreeParams& p, int r) 
   }
   // no node stands before its request's cached tokens, so none sees a key before this one
   t.begin = p.window > 0 ? max(0, t.cached - p.window + 1) / p.page_size * p.page_size : 0;
-  t.node_blocks = (t.nodes + p.unit_nodes - 1) / p.unit_nodes;
-  const int group = p.heads / p.kv_heads;
-  t.units = t.node_blocks * p.kv_heads * ((group + p.unit_heads - 1) / p.unit_heads);
-  t.tiles = (t.cached + t.nodes - t.begin + p.tile_keys - 1) / p.tile_keys;
+  t.node_blocks = divide(t.nodes + p.unit_nodes - 1, p.unit_nodes);
+  t.units = t.node_blocks * p.kv_heads * p.head_blocks;
+  t.tiles = (t.cached + t.nodes - t.begin + (1 << p.tile_shift) - 1) >> p.tile_shift;
   return t;
 }
 
@@ -108,93 +150,127 @@ struct TreeUnit {
 
 __device__ __forceinline__ TreeUnit tree_unit(const TreeParams& p, const TreeRequest& t, int unit) {
   TreeUnit u;
-  const int group = p.heads / p.kv_heads;
-  const int head_blocks = (group + p.unit_heads - 1) / p.unit_heads;
-  const int pair = unit / t.node_blocks, block = unit - pair * t.node_blocks;
-  u.kv_head = pair / head_blocks;
-  const int head_block = pair - u.kv_head * head_blocks;
-  u.first_head = u.kv_head * group + head_block * p.unit_heads;
-  u.heads = min(p.unit_heads, group - head_block * p.unit_heads);
-  const int each = (t.nodes + t.node_blocks - 1) / t.node_blocks;     // blocks of one size
+  const int pair = divide(unit, t.node_blocks), block = unit - pair * t.node_blocks;
+  u.kv_head = p.head_blocks == 1 ? pair : divide(pair, p.head_blocks);
+  const int head_block = pair - u.kv_head * p.head_blocks;
+  u.first_head = u.kv_head * p.group + head_block * p.unit_heads;
+  u.heads = min(p.unit_heads, p.group - head_block * p.unit_heads);
+  const int each = divide(t.nodes + t.node_blocks - 1, t.node_blocks);     // blocks of one size
   u.first_node = min(t.nodes, block * each);
   u.nodes = min(each, t.nodes - u.first_node);
   return u;
 }
 
-// Every warp works out the cut by itself: all (unit, tile) pairs of the launch, and a CTA's share of them.
-__device__ __forceinline__ long long tree_pairs(const TreeParams& p) {
-  long long sum = 0;
-  for (int r0 = 0; r0 < p.requests; r0 += 32) {
-    const int r = r0 + (threadIdx.x & 31);
-    long long mine = 0;
-    if (r < p.requests) {
-      const TreeRequest t = tree_request(p, r);
-      mine = (long long)t.units * t.tiles;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    sum += mine;
-  }
-  return sum;
-}
-
-// The pieces of a CTA's share, one unit after the other.
+// The pieces of a worker, one unit after the other.
 struct TreeWalk {
   int request, unit;         // where the walk stands
-  int tile_begin, tile_end;  // tiles of that unit that are this CTA's
-  bool whole;                // no other CTA has tiles of this unit
+  int tile_begin, tile_end;  // key tiles of that unit that are this worker's
+  bool whole;                // no other worker has tiles of this unit
   int share;                 // where its results go otherwise
   TreeRequest t;
-  long long left;            // pairs of the share that come after this piece
+  int left;                  // what comes after this piece: pairs of the list, or units
   int pieces, chunk;
+  bool list;
 };
 
-__device__ __forceinline__ void tree_piece(const TreeParams& p, TreeWalk* w, int tile_begin, long long available) {
+__device__ __forceinline__ int warp_add(int v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ void tree_piece(const TreeParams& p, int worker, TreeWalk* w, int tile_begin, int available) {
   w->tile_begin = tile_begin;
-  w->tile_end = (int)min((long long)w->t.tiles, tile_begin + available);
+  w->tile_end = min(w->t.tiles, tile_begin + available);
   w->left = available - (w->tile_end - tile_begin);
   w->whole = tile_begin == 0 && w->tile_end == w->t.tiles;
-  w->share = 2 * blockIdx.x + (w->pieces > 0 ? 1 : 0);
+  w->share = 2 * worker + (w->pieces > 0 ? 1 : 0);
   ++w->pieces;
 }
-// False where the CTA has nothing to do.
-__device__ __forceinline__ bool tree_first(const TreeParams& p, TreeWalk* w) {
-  const long long pairs = tree_pairs(p);
-  const long long chunk = max((long long)p.min_chunk, (pairs + p.ctas - 1) / p.ctas);
-  const long long begin = chunk * blockIdx.x;
-  if (begin >= pairs) return false;
+// The first piece of a worker; every warp works it out by itself.  False where there is nothing to do.  (Sums are 32-bit: a
+// launch of 2^31 key tiles would read more than there is memory.)
+__device__ __forceinline__ bool tree_first(const TreeParams& p, int worker, TreeWalk* w) {
   const int lane = threadIdx.x & 31;
-  long long before = 0;
-  w->pieces = 0;
-  w->chunk = (int)chunk;
-  for (int r0 = 0; r0 < p.requests; r0 += 32) {
-    const int r = r0 + lane;
-    long long mine = 0;
-    if (r < p.requests) {
-      const TreeRequest t = tree_request(p, r);
-      mine = (long long)t.units * t.tiles;
+  TreeRequest mine = {};
+  if (lane < p.requests) mine = tree_request(p, lane);
+  const bool few = p.requests <= 32;
+  auto request = [&](int r) {                    // lane's request of the 32 from r - lane on
+    if (few) return mine;
+    TreeRequest none = {};
+    return r < p.requests ? tree_request(p, r) : none;
+  };
+  auto total = [&](auto weight) {
+    if (few) return warp_add(weight(mine));
+    int sum = 0;
+    for (int r0 = 0; r0 < p.requests; r0 += 32) sum += warp_add(weight(request(r0 + lane)));
+    return sum;
+  };
+  const int units = total([](const TreeRequest& t) { return t.units; });
+  int chunk = 1, begin, end;
+  w->list = false;
+  if (p.whole) {
+    chunk = 0x7fffffff;
+    const int each = divide(units + p.workers - 1, p.workers);
+    begin = worker * each;
+    end = min(units, begin + each);
+  } else {
+    const int pairs = total([](const TreeRequest& t) { return t.units * t.tiles; });
+    chunk = max(p.min_chunk, (pairs + p.workers - 1) / p.workers);
+    if (units > p.workers) {
+      w->list = true;
+      begin = worker * chunk;
+      end = min(pairs, begin + chunk);
+    } else {
+      int pieces;
+#pragma unroll 1
+      while ((pieces = total([&](const TreeRequest& t) { return t.units * divide(t.tiles + chunk - 1, chunk); })) > p.workers)
+        chunk = max(chunk + 1, (int)__fdividef((float)chunk * pieces, (float)p.workers));
+      begin = worker;
+      end = min(pieces, begin + 1);
     }
-    long long upto = mine;
+  }
+  w->pieces = 0;
+  w->chunk = chunk;
+  if (begin >= end) return false;
+  int before = 0;
+  for (int r0 = 0; r0 < p.requests; r0 += 32) {
+    const TreeRequest t = request(r0 + lane);
+    const int each = w->list ? t.tiles : p.whole ? 1 : divide(t.tiles + chunk - 1, chunk);      // of a unit
+    const int here = t.units * each;
+    int upto = here;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += v;
     }
     const uint32_t after = __ballot_sync(0xffffffffu, before + upto > begin);
     if (after) {
       const int at = __ffs(after) - 1;
-      const long long start = before + __shfl_sync(0xffffffffu, upto - mine, at);
+      const int skip = begin - before - __shfl_sync(0xffffffffu, upto - here, at), unit_each = __shfl_sync(0xffffffffu, each, at);
       w->request = r0 + at;
-      w->t = tree_request(p, w->request);
-      w->unit = (int)((begin - start) / w->t.tiles);
-      tree_piece(p, w, (int)((begin - start) - (long long)w->unit * w->t.tiles), min(chunk, pairs - begin));
+      w->t.first = __shfl_sync(0xffffffffu, t.first, at);
+      w->t.nodes = __shfl_sync(0xffffffffu, t.nodes, at);
+      w->t.cached = __shfl_sync(0xffffffffu, t.cached, at);
+      w->t.begin = __shfl_sync(0xffffffffu, t.begin, at);
+      w->t.units = __shfl_sync(0xffffffffu, t.units, at);
+      w->t.tiles = __shfl_sync(0xffffffffu, t.tiles, at);
+      w->t.node_blocks = __shfl_sync(0xffffffffu, t.node_blocks, at);
+      w->unit = divide(skip, unit_each);
+      const int part = skip - w->unit * unit_each;
+      if (w->list) {
+        tree_piece(p, worker, w, part, end - begin);
+      } else if (p.whole) {
+        tree_piece(p, worker, w, 0, w->t.tiles);
+        w->left = end - begin - 1;
+      } else {
+        tree_piece(p, worker, w, part * chunk, min(chunk, w->t.tiles - part * chunk));
+      }
       return true;
     }
     before += __shfl_sync(0xffffffffu, upto, 31);
   }
   return false;
 }
-__device__ __forceinline__ bool tree_next(const TreeParams& p, TreeWalk* w) {
+__device__ __forceinline__ bool tree_next(const TreeParams& p, int worker, TreeWalk* w) {
   if (w->left <= 0) return false;
   if (++w->unit >= w->t.units) {
     w->unit = 0;
@@ -203,7 +279,13 @@ __device__ __forceinline__ bool tree_next(const TreeParams& p, TreeWalk* w) {
       w->t = tree_request(p, w->request);
     } while (w->t.units == 0);
   }
-  tree_piece(p, w, 0, w->left);
+  if (w->list) {
+    tree_piece(p, worker, w, 0, w->left);
+  } else {
+    const int left = w->left;
+    tree_piece(p, worker, w, 0, w->t.tiles);
+    w->left = left - 1;
+  }
   return true;
 }
 
@@ -248,72 +330,109 @@ __device__ __forceinline__ int tree_lowest(const TreeParams& p, int position) {
   return p.window > 0 ? max(0, position - p.window + 1) : 0;
 }
 
-constexpr int kTreeMergeWarps = 8;
-constexpr int kTreeMergeBlocks = 16;       // CTAs that take one unit's rows in turn
-
-// What the second launch has to know of a CTA's share: the unit of its first piece, where that piece begins, the length of
-// a share.  (x = -1: nothing to put together here.)
-__device__ __forceinline__ void tree_note(const TreeParams& p, const TreeWalk& w, bool any) {
-  if (threadIdx.x == 0)
-    p.notes[blockIdx.x] = any && w.tile_begin > 0 ? make_int4(w.request, w.unit, w.tile_begin, w.chunk) : make_int4(-1, 0, 0, 0);
+// Where four elements of a row of a share lie.
+__device__ __forceinline__ float* tree_share(const TreeParams& p, int share, int row, int d) {
+  return p.part_o + ((((size_t)share * (p.unit_rows >> 5) + (row >> 5)) * (p.padded >> 2) + (d >> 2)) * 32 + (row & 31)) * 4;
 }
 
-// Rows whose keys several CTAs had: o = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c over the shares in the order of
-// their keys.  The CTAs (blockIdx.x) stand for the places where a share ends and the next begins; the first of
-// those inside a unit puts that unit together.  A warp per row.
+__device__ __forceinline__ void tree_note(const TreeParams& p, int worker, const TreeWalk& w, bool any) {
+  if (!p.notes) return;
+  TreeNote n = {};
+  if (any && w.tile_begin > 0) {
+    const TreeUnit u = tree_unit(p, w.t, w.unit);
+    n.place = divide(w.tile_begin - 1, w.chunk);
+    n.places = n.place + divide(w.t.tiles - w.tile_begin + w.chunk - 1, w.chunk);
+    n.second = w.tile_begin - n.place * w.chunk < w.chunk ? 1 : 0;
+    n.token = w.t.first + u.first_node;
+    n.nodes = u.nodes;
+    n.heads = u.heads;
+    n.first_head = u.first_head;
+  }
+  p.notes[worker] = n;
+}
+
+constexpr int kTreeMergeWarps = 4;
+constexpr int kTreeMergeShares = 4;        // shares that a warp has in flight
+
+// Rows whose keys several workers had: o = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c over the shares in the order of
+// their keys.  blockIdx.x stands for the place where a worker's list ends and the next one's begins; the places inside one
+// unit share its work out: an item is 32 rows, one a lane, and eight elements of each, which lie as 2 x 512 bytes in a
+// share.  Loops stay rolled: the kernel runs for a few microseconds, and its instructions come at the pace of their first fetch.
 template <typename T>
 __global__ void __launch_bounds__(32 * kTreeMergeWarps) tree_merge_kernel(TreeParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int4 note = p.notes[blockIdx.x + 1];
-  const int chunk = note.w;
-  if (note.x < 0 || note.z > chunk) return;              // no unit is cut here, or it was cut before
+  const TreeNote n = p.notes[blockIdx.x + 1];
+  if (n.places == 0) return;                             // no unit is cut here
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const TreeRequest t = tree_request(p, note.x);
-  const TreeUnit u = tree_unit(p, t, note.y);
-  const int first = blockIdx.x, last = first + (t.tiles - note.z + chunk - 1) / chunk;
-  const int second = note.z < chunk ? 1 : 0;             // the unit was not the first piece of its first CTA
-  for (int row = blockIdx.y * kTreeMergeWarps + warp; row < u.nodes * u.heads; row += gridDim.y * kTreeMergeWarps) {
-    auto share = [&](int c) { return (size_t)(2 * c + (c == first ? second : 0)) * p.unit_rows + row; };
+  const int first = blockIdx.x - n.place, rows = n.nodes * n.heads, groups = p.padded >> 2;
+  for (int item = (blockIdx.y * kTreeMergeWarps + warp) * n.places + n.place;; item += n.places * gridDim.y * kTreeMergeWarps) {
+    const int row_block = divide(2 * item, groups), row = row_block * 32 + lane, group = 2 * item - row_block * groups;
+    if (row_block * 32 >= rows) break;
+    if (row >= rows) continue;
+    const float2* ml = p.part_ml + row;
+    const float4* sums = reinterpret_cast<const float4*>(p.part_o) + ((size_t)row_block * groups + group) * 32 + lane;
+    const size_t share_rows = (size_t)p.unit_rows, share_sums = (size_t)(p.unit_rows >> 5) * groups * 32;
+    const bool two = group + 1 < groups;
     float m = -INFINITY, l = 0.f;
-    for (int c0 = first; c0 <= last; c0 += 32) {
-      const float2 ml = c0 + lane <= last ? __ldcg(p.part_ml + share(c0 + lane)) : make_float2(-INFINITY, 0.f);
-      const float top = fmaxf(m, warp_max(ml.x));
-      // a sum that is not a number stays one, whatever the reference beside it
-      const float here = ml.y == 0.f ? 0.f : ml.y * (ml.x == -INFINITY ? 0.f : exp2f(ml.x - top));
-      l = (l == 0.f ? 0.f : l * (m == -INFINITY ? 0.f : exp2f(m - top))) + warp_sum(here);
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+#pragma unroll 1
+    for (int c0 = 0; c0 <= n.places; c0 += kTreeMergeShares) {
+      float2 v[kTreeMergeShares];
+      float4 x[kTreeMergeShares], y[kTreeMergeShares];
+      // all of these in flight at once; what lies beyond the last share is the last one again
+#pragma unroll
+      for (int i = 0; i < kTreeMergeShares; ++i) {
+        const int c = min(c0 + i, n.places);
+        const size_t share = 2 * (first + c) + (c == 0 ? n.second : 0);
+        v[i] = __ldcg(ml + share * share_rows);
+        x[i] = __ldcg(sums + share * share_sums);
+        y[i] = __ldcg(sums + share * share_sums + (two ? 32 : 0));
+      }
+      float top = m;
+#pragma unroll
+      for (int i = 0; i < kTreeMergeShares; ++i) top = fmaxf(top, v[i].x);
+      const float keep = m == -INFINITY ? 0.f : fast_exp2(m - top);
       m = top;
+      // a sum of weights that is not a number stays one, whatever the reference beside it
+      l = l == 0.f ? 0.f : l * keep;
+      a.x *= keep, a.y *= keep, a.z *= keep, a.w *= keep;
+      b.x *= keep, b.y *= keep, b.z *= keep, b.w *= keep;
+#pragma unroll
+      for (int i = 0; i < kTreeMergeShares; ++i) {
+        const float f = v[i].x == -INFINITY || c0 + i > n.places ? 0.f : fast_exp2(v[i].x - top);
+        l += v[i].y == 0.f || c0 + i > n.places ? 0.f : v[i].y * f;
+        if (f == 0.f) continue;                          // a share without a reference has nothing in its sums
+        a.x = fmaf(x[i].x, f, a.x), a.y = fmaf(x[i].y, f, a.y), a.z = fmaf(x[i].z, f, a.z), a.w = fmaf(x[i].w, f, a.w);
+        b.x = fmaf(y[i].x, f, b.x), b.y = fmaf(y[i].y, f, b.y), b.z = fmaf(y[i].z, f, b.z), b.w = fmaf(y[i].w, f, b.w);
+      }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    const size_t at = ((size_t)(t.first + u.first_node + row / u.heads) * p.heads + u.first_head + row % u.heads) * p.size;
-    T* out = static_cast<T*>(p.out) + at;
-    for (int d0 = 0; d0 < p.size; d0 += 128) {
-      const int d = d0 + 4 * lane;
-      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (d < p.padded)
-#pragma unroll 4
-        for (int c = first; c <= last; ++c) {
-          const float mc = __ldcg(&p.part_ml[share(c)].x);
-          if (mc == -INFINITY) continue;
-          const float f = exp2f(mc - m);
-          const float4 o = __ldcg(reinterpret_cast<const float4*>(p.part_o + share(c) * p.padded + d));
-          sum.x += o.x * f;
-          sum.y += o.y * f;
-          sum.z += o.z * f;
-          sum.w += o.w * f;
-        }
-      const float v[4] = {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv};
+    const int node = divide(row, n.heads), d = 4 * group;
+    T* out = static_cast<T*>(p.out) + ((size_t)(n.token + node) * p.heads + n.first_head + row - node * n.heads) * p.size + d;
+    const float v[8] = {a.x * inv, a.y * inv, a.z * inv, a.w * inv, b.x * inv, b.y * inv, b.z * inv, b.w * inv};
+    if (p.size % 8 == 0 && ((uintptr_t)out & 15) == 0) {
+      // sixteen bytes at a time (element by element, rows apart, these stores took most of the kernel's time)
+      __align__(16) T narrow[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (d + e < p.size) out[d + e] = from_float<T>(v[e]);
+      for (int e = 0; e < 8; ++e) narrow[e] = from_float<T>(v[e]);
+#pragma unroll
+      for (int e = 0; e < (int)(8 * sizeof(T) / 16); ++e) reinterpret_cast<uint4*>(out)[e] = reinterpret_cast<const uint4*>(narrow)[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (d + e < p.size) out[e] = from_float<T>(v[e]);
     }
   }
 }
 
 template <typename T>
 inline int tree_merge(const TreeParams& p, cudaStream_t stream) {
-  if (p.ctas < 2) return 0;
-  return (int)launch_pdl(tree_merge_kernel<T>, dim3((unsigned)p.ctas - 1, kTreeMergeBlocks), dim3(32 * kTreeMergeWarps), 0, stream, p);
+  if (p.workers < 2 || p.whole) return 0;
+  // two items a warp where a unit is cut once
+  const int items = p.unit_rows / 32 * ((p.padded + 7) / 8);
+  return (int)launch_pdl(tree_merge_kernel<T>, dim3((unsigned)p.workers - 1, (unsigned)(items + 2 * kTreeMergeWarps - 1) / (2 * kTreeMergeWarps)),
+                         dim3(32 * kTreeMergeWarps), 0, stream, p);
 }
 
 }  // namespace einf

@@ -9,19 +9,15 @@
 // together at the end.
 //
 //   warps 0, 1    K and V producers: TMA-load the pages that the block table names into rings of tiles
-//   warps 2, 3    one lane each issues a slot's products: S = Q K^T into tensor memory, O += P V with P from there
-//   warps 4-11    softmax, a warpgroup a slot: thread r has row r of the slot's tile
+//   warps 2, 3    issue a slot's products: S = Q K^T into tensor memory, O += P V with P from there
+//   warps 4-19    softmax, two warpgroups a slot: thread r of either has row r of the slot's tile, and half of its keys
 //
-// Sums stay in tensor memory, scaled by a reference that is the maximum of the row's first tile and moves only when a
-// later tile has a score 2^8 above it.  Thread r looks for its row's maximum first and then goes over the scores again: the
-// probabilities take the place of scores that were read (head size 128, where tensor memory has no other) or a
-// place of their own (64, where the next scores need not wait for the second product).
+// Sums stay in tensor memory, scaled by a reference that is the maximum of the row's first tile and moves only when a later
+// tile has a score 2^8 above it.
 //
 // Tiles with keys that some row does not see (the drafted ones, a window) run with masks of 128 bits a row.  There a
 // value that is not finite must not meet a weight of zero, so the V producer looks over such a tile, clears the
 // elements it finds and names their keys; the rows that do see such a key add them to their sums themselves.
-#include <type_traits>
-
 #include "attention_tree.cuh"
 #include "mma_sync.cuh"
 #include "tcgen05.cuh"
@@ -30,25 +26,31 @@ namespace einf {
 
 constexpr int kTile = 128;                     // rows of a slot, keys of a tile
 constexpr int kSlice = kTile * 128;            // a [128 rows x 64] bfloat16 slice: 16 KB
-constexpr int kTreeThreads = 384;
+constexpr int kTreeThreads = 640;
 constexpr float kMove = 8.f;                   // exponents above its reference at which a row moves it
-constexpr int kTmemColumns = 512;
+constexpr int kHalf = kTile / 2;               // keys of a softmax thread
+constexpr int kTmemColumns = 512;              // S: 2 x 128 columns, O: 2 x D
 
 template <int D>
 struct Layout {
   static constexpr int kBlocks = D / 64;                       // 64-wide slices of the head
   static constexpr int kTileBytes = kBlocks * kSlice;
-  static constexpr bool kOwnP = D == 64;                       // P has tensor memory of its own
   static constexpr int kKStages = D == 64 ? 5 : 3;
   static constexpr int kVStages = D == 64 ? 5 : 2;
   static constexpr int kQ = 0;                                 // a tile of rows per slot
   static constexpr int kK = kQ + 2 * kTileBytes;
   static constexpr int kV = kK + kKStages * kTileBytes;
   static constexpr int kBars = kV + kVStages * kTileBytes;
-  static constexpr int kNumBars = 10 + 3 * kKStages + 4 * kVStages;
+  static constexpr int kNumBars = 8 + 3 * kKStages + 4 * kVStages;
   static constexpr int kBad = kBars + 8 * kNumBars + 16;       // per V stage: 128 bits, rows of the tile that were cleared
-  static constexpr int kXchg = kBad + 16 * kVStages;           // reference and sum of every row, per slot
-  static constexpr int kBytes = kXchg + 2 * 128 * 8;
+  static constexpr int kXchg = kBad + 16 * kVStages;           // a float for every thread of the softmax warps
+  // what the CTAs of a cluster exchange, in the place of the K and V tiles: the sums of 256 rows (padded so that neither
+  // threads with a row each nor warps with a row each meet a bank twice), then reference and sum of every row
+  static constexpr int kPitch = D + 4;
+  static constexpr int kSums = kK;
+  static constexpr int kSumsMl = kSums + 256 * kPitch * 4;
+  static_assert(kSumsMl + 256 * 8 <= kBars, "the exchange needs the K and V tiles");
+  static constexpr int kBytes = kXchg + 4 * 128 * 4;
   static_assert(kBytes <= 227 * 1024, "shared memory of the tree attention kernel exceeds an SM");
   static_assert(2 * kBytes > 228 * 1024, "two CTAs on an SM would wait for each other's tensor memory");
   static_assert(kXchg % 8 == 0 && kBad % 4 == 0, "alignment");
@@ -60,23 +62,118 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int
       ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
 }
-__device__ __forceinline__ void both_slots_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+// True in one lane of the warp, always the same.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t elected;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(elected));
+  return elected != 0;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float4 ld_peer4(uint32_t local, uint32_t rank) {
+  uint32_t peer;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(local), "r"(rank));
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(peer) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_peer2(uint32_t local, uint32_t rank) {
+  uint32_t peer;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(local), "r"(rank));
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(peer) : "memory");
+  return v;
+}
+__device__ __forceinline__ void both_slots_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
+// The two warps with the same rows meet; true if `value` is, in any thread of them.
+__device__ __forceinline__ bool pair_any(int pair, bool value) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %2, 0;\n\t"
+      "barrier.cta.red.or.pred q, %1, 64, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(2 + pair), "r"((uint32_t)value)
+      : "memory");
+  return any != 0;
+}
+__device__ __forceinline__ void pair_sync(int pair) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(2 + pair) : "memory"); }
+
+// A cluster shares the key tiles of its piece out among its CTAs.
+__device__ __forceinline__ void share_out(TreeWalk* w, int rank, int cluster) {
+  const int each = divide(w->tile_end - w->tile_begin + cluster - 1, cluster);
+  w->tile_begin = min(w->tile_end, w->tile_begin + rank * each);
+  w->tile_end = min(w->tile_end, w->tile_begin + each);
+}
+
+// The shares of a unit's rows that the CTAs of a cluster left in their shared memory, put together: rank takes a run of rows.
+template <int D>
+__device__ __forceinline__ void merge_cluster(const TreeParams& p, const TreeWalk& w, const TreeUnit& u, uint32_t base, int rank) {
+  using L = Layout<D>;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = u.nodes * u.heads;
+  const int each = divide(rows + p.cluster - 1, p.cluster), first = rank * each, last = min(rows, first + each);
+#pragma unroll 1
+  for (int row = first + warp; row < last; row += kTreeThreads / 32) {
+    const float2 ml = lane < p.cluster ? ld_peer2(base + L::kSumsMl + row * 8, lane) : make_float2(-INFINITY, 0.f);
+    const float m = warp_max(ml.x);
+    const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - m);
+    const float l = warp_sum(ml.y == 0.f ? 0.f : ml.y * f);
+    const uint32_t at = base + L::kSums + (row * L::kPitch + (4 * lane) % D) * 4;      // (D = 64: the upper lanes repeat the lower)
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int c = 0; c < p.cluster; ++c) {
+      const float fc = __shfl_sync(0xffffffffu, f, c);
+      const float4 o = ld_peer4(at, c);
+      if (fc == 0.f) continue;
+      sum.x += o.x * fc;
+      sum.y += o.y * fc;
+      sum.z += o.z * fc;
+      sum.w += o.w * fc;
+    }
+    if (4 * lane < D && w.whole) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int node = divide(row, u.heads);
+      __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) +
+          ((size_t)(w.t.first + u.first_node + node) * p.heads + u.first_head + row - node * u.heads) * D + 4 * lane;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_pair(sum.x * inv, sum.y * inv), pack_pair(sum.z * inv, sum.w * inv));
+    } else if (4 * lane < D) {
+      *reinterpret_cast<float4*>(tree_share(p, w.share, row, 4 * lane)) = sum;
+      if (lane == 0) p.part_ml[(size_t)w.share * p.unit_rows + row] = make_float2(m, l);
+    }
+    __syncwarp();
+  }
+}
+
+// A softmax thread's row.
+struct Row {
+  bool live;
+  int token, position, lowest;
+  float m, l;               // the reference and the sum of weights
+};
 
 // What a slot has of a unit.
 struct Slot {
   int first_node, rows, first_tile, step, tiles;   // tiles of the piece: first_tile, first_tile + step, ...
   bool pair;                                       // the unit has two tiles of rows, one a slot
 };
-__device__ __forceinline__ Slot slot_of(const TreeParams& p, const TreeWalk& w, const TreeUnit& u, int g) {
+__device__ __forceinline__ Slot slot_of(const TreeWalk& w, const TreeUnit& u, int g) {
   Slot s;
-  const int most = kTile / u.heads;
+  const int most = divide(kTile, u.heads);
   s.pair = u.nodes > most;
   const int half = (u.nodes + 1) >> 1;
   s.first_node = s.pair && g ? half : 0;
   s.rows = (s.pair ? (g ? u.nodes - half : half) : u.nodes) * u.heads;
   s.step = s.pair ? 1 : 2;
   s.first_tile = w.tile_begin + (s.pair ? 0 : g);
-  s.tiles = max(0, (w.tile_end - s.first_tile + s.step - 1) / s.step);
+  s.tiles = max(0, (w.tile_end - s.first_tile + s.step - 1) >> (s.pair ? 0 : 1));
   return s;
 }
 
@@ -97,24 +194,22 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
   auto s_full = [&](int g) { return bars + 8u * (2 + g); };
   auto p_full = [&](int g) { return bars + 8u * (4 + g); };
   auto o_done = [&](int g) { return bars + 8u * (6 + g); };
-  auto s_free = [&](int g) { return bars + 8u * (8 + g); };
-  auto k_full = [&](int s) { return bars + 8u * (10 + s); };
-  auto k_empty = [&](int g, int s) { return bars + 8u * (10 + (1 + g) * L::kKStages + s); };
-  auto v_full = [&](int s) { return bars + 8u * (10 + 3 * L::kKStages + s); };
-  auto v_checked = [&](int s) { return bars + 8u * (10 + 3 * L::kKStages + L::kVStages + s); };
-  auto v_empty = [&](int g, int s) { return bars + 8u * (10 + 3 * L::kKStages + (2 + g) * L::kVStages + s); };
+  auto k_full = [&](int s) { return bars + 8u * (8 + s); };
+  auto k_empty = [&](int g, int s) { return bars + 8u * (8 + (1 + g) * L::kKStages + s); };
+  auto v_full = [&](int s) { return bars + 8u * (8 + 3 * L::kKStages + s); };
+  auto v_checked = [&](int s) { return bars + 8u * (8 + 3 * L::kKStages + L::kVStages + s); };
+  auto v_empty = [&](int g, int s) { return bars + 8u * (8 + 3 * L::kKStages + (2 + g) * L::kVStages + s); };
   const uint32_t tmem_holder = bars + 8 * L::kNumBars;
   uint32_t* cleared = reinterpret_cast<uint32_t*>(smem_raw + L::kBad);      // [V stage][4]
-  float2* xchg = reinterpret_cast<float2*>(smem_raw + L::kXchg);            // [slot][row]
+  float* xchg = reinterpret_cast<float*>(smem_raw + L::kXchg);              // [slot][half of the keys][row]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int g = 0; g < 2; ++g) {
       bar_init(q_full(g), 1);
       bar_init(s_full(g), 1);
-      bar_init(p_full(g), 128);
+      bar_init(p_full(g), 256);
       bar_init(o_done(g), 1);
-      bar_init(s_free(g), 128);
       for (int s = 0; s < L::kKStages; ++s) bar_init(k_empty(g, s), 1);
       for (int s = 0; s < L::kVStages; ++s) bar_init(v_empty(g, s), 1);
     }
@@ -134,15 +229,31 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(smem_raw + L::kBars + 8 * L::kNumBars);
+  // the scores and, in the first 32 of the 64 columns of either half of the keys, the probabilities
   auto tmem_s = [&](int g) { return tmem_base + 128u * g; };
   auto tmem_o = [&](int g) { return tmem_base + 256u + (uint32_t)D * g; };
-  auto tmem_p = [&](int g) { return L::kOwnP ? tmem_base + 384u + 64u * g : tmem_base + 128u * g; };
   pdl_launch_dependents();   // after the tensor-memory allocation, see common.cuh
   pdl_wait();
 
+  const int cluster = p.cluster, worker = divide(blockIdx.x, cluster), rank = blockIdx.x - worker * cluster;
   TreeWalk w;
-  bool any = tree_first(p, &w);
-  tree_note(p, w, any);
+  bool any = tree_first(p, worker, &w);
+  if (threadIdx.x == 0 && rank == 0) tree_note(p, worker, w, any);
+  if (any && cluster > 1) share_out(&w, rank, cluster);
+  // Every warp ends a piece here.  The CTAs of a cluster put their shares of it together: once they have all left them in shared
+  // memory, and before any of them takes that for the next piece (or leaves).
+  auto next_piece = [&]() {
+    if (cluster > 1) {
+      __syncwarp();
+      cluster_barrier();
+      merge_cluster<D>(p, w, tree_unit(p, w.t, w.unit), base, rank);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // TMA and the tensor core have the place next
+      __syncwarp();
+      cluster_barrier();
+    }
+    any = tree_next(p, worker, &w);
+    if (any && cluster > 1) share_out(&w, rank, cluster);
+  };
 
   if (warp < 2) {
     // ---- producers: warp 0 the K tiles, warp 1 the V tiles; lane j fetches page j of a tile ----
@@ -157,9 +268,9 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
     uint32_t held[2] = {0u, 0u}, parity[2] = {0u, 0u};
     bool ok = true, bad = false;
     int stage = 0, round = 0;
-    for (; any; any = tree_next(p, &w)) {
+    for (; any; next_piece()) {
       const TreeUnit u = tree_unit(p, w.t, w.unit);
-      const bool pair = slot_of(p, w, u, 0).pair;
+      const bool pair = slot_of(w, u, 0).pair;
       const int* table = p.block_table + (size_t)w.request * p.table_width;
       const int keys_end = w.t.cached + w.t.nodes;
       auto pages_of = [&](int i) {
@@ -248,38 +359,43 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
           ++round;
         }
       }
-      if (!ok) break;
     }
     if (__any_sync(0xffffffffu, bad) && lane == 0) atomicOr(p.status, kStatusBadPage);
   } else if (warp < 4) {
-    // ---- a slot's products ----
+    // ---- a slot's products: the whole warp goes the way of the lane that issues, so that addresses stay in uniform registers ----
     const int g = warp - 2;
-    if (lane == 0) {
-      // S: M = 128 rows, N = 128 keys, both K-major.  O: M = 128, N = D, P from tensor memory, V MN-major.
-      const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kTile >> 3) << 17) | ((128u >> 4) << 24);
-      const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
-      const uint64_t desc_q = desc_k_major(base + L::kQ + g * L::kTileBytes);
-      bool ok = true;
-      int queries = 0;               // loads of Q so far
-      int done = 0;                  // this slot's tiles so far
-      int before = 0;                // the CTA's tiles before this piece
-      for (; any && ok; any = tree_next(p, &w)) {
-        const TreeUnit u = tree_unit(p, w.t, w.unit);
-        const Slot s = slot_of(p, w, u, g);
-        const int first = before + s.first_tile - w.tile_begin;
-        before += w.tile_end - w.tile_begin;
-        if (s.tiles == 0) continue;
-        bar_expect_tx(q_full(g), (uint32_t)(kTile / u.heads * u.heads) * 128u * L::kBlocks);
+    // S: M = 128 rows, N = 128 keys, both K-major.  O: M = 128, N = D, P from tensor memory, V MN-major.
+    constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kTile >> 3) << 17) | ((128u >> 4) << 24);
+    constexpr uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
+    const uint64_t desc_q = desc_k_major(base + L::kQ + g * L::kTileBytes);
+    auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, bar_wait_likely_done(bar, parity, p.status)) != 0; };
+    bool ok = true;
+    int queries = 0;               // loads of Q so far
+    int done = 0;                  // this slot's tiles so far
+    int before = 0;                // the CTA's tiles before this piece
+    for (; any; next_piece()) {
+      const TreeUnit u = tree_unit(p, w.t, w.unit);
+      const Slot s = slot_of(w, u, g);
+      const int first = before + s.first_tile - w.tile_begin;
+      before += w.tile_end - w.tile_begin;
+      if (s.tiles == 0 || !ok) continue;
+      if (elect_one()) {
+        bar_expect_tx(q_full(g), (uint32_t)(p.unit_nodes / 2 * u.heads) * 128u * L::kBlocks);
         for (int db = 0; db < L::kBlocks; ++db)
           tma_3d(base + L::kQ + g * L::kTileBytes + db * kSlice, &map_q, db * 64, u.first_head, w.t.first + u.first_node + s.first_node,
                  q_full(g));
-        ok = bar_wait(q_full(g), queries & 1, p.status);
-        ++queries;
-        auto scores = [&](int j) {
-          const int c = first + j * s.step, stage = c % L::kKStages;
-          if (!bar_wait_likely_done(k_full(stage), (c / L::kKStages) & 1, p.status)) return false;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint64_t desc_k = desc_k_major(base + L::kK + stage * L::kTileBytes);
+      }
+      __syncwarp();
+      ok = wait(q_full(g), queries & 1);
+      ++queries;
+#pragma unroll 1
+      for (int j = 0; j < s.tiles && ok; ++j, ++done) {
+        const int c = first + j * s.step, k_stage = c % L::kKStages, v_stage = c % L::kVStages;
+        ok = wait(k_full(k_stage), (c / L::kKStages) & 1);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (elect_one()) {
+          const uint64_t desc_k = desc_k_major(base + L::kK + k_stage * L::kTileBytes);
 #pragma unroll
           for (int db = 0; db < L::kBlocks; ++db)
 #pragma unroll
@@ -287,207 +403,187 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
               mma_ss(tmem_s(g), desc_advance(desc_q, db * kSlice + kk * 32), desc_advance(desc_k, db * kSlice + kk * 32), idesc_s,
                      (db > 0 || kk > 0) ? 1u : 0u);
           mma_commit(s_full(g));
-          mma_commit(k_empty(g, stage));
-          return true;
-        };
-        auto sums = [&](int j) {
-          const int c = first + j * s.step, stage = c % L::kVStages;
-          const uint32_t parity = (c / L::kVStages) & 1;
-          if (!bar_wait_likely_done(v_full(stage), parity, p.status) || !bar_wait_likely_done(v_checked(stage), parity, p.status) ||
-              !bar_wait(p_full(g), (done + j) & 1, p.status))
-            return false;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint64_t desc_v = desc_mn_major(base + L::kV + stage * L::kTileBytes, kSlice);
+          mma_commit(k_empty(g, k_stage));
+        }
+        __syncwarp();
+        const uint32_t parity = (c / L::kVStages) & 1;
+        ok = wait(v_full(v_stage), parity) && wait(v_checked(v_stage), parity) && wait(p_full(g), done & 1);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (elect_one()) {
+          const uint64_t desc_v = desc_mn_major(base + L::kV + v_stage * L::kTileBytes, kSlice);
 #pragma unroll
           for (int ks = 0; ks < kTile / 16; ++ks)      // onto the zeros or sums that the softmax warps left
-            mma_ts(tmem_o(g), tmem_p(g) + ks * 8, desc_advance(desc_v, ks * 16 * 128), idesc_o, 1u);
+            mma_ts(tmem_o(g), tmem_s(g) + (ks >> 2) * kHalf + (ks & 3) * 8, desc_advance(desc_v, ks * 16 * 128), idesc_o, 1u);
           mma_commit(o_done(g));
-          mma_commit(v_empty(g, stage));
-          return true;
-        };
-        if (L::kOwnP) {
-          ok = ok && scores(0);
-          for (int j = 0; j < s.tiles && ok; ++j) {
-            if (j + 1 < s.tiles) ok = bar_wait(s_free(g), (done + j) & 1, p.status) && scores(j + 1);
-            ok = ok && sums(j);
-          }
-          done += s.tiles;
-          ok = ok && bar_wait(o_done(g), (done - 1) & 1, p.status);      // the queries' place is free again
-        } else {
-          for (int j = 0; j < s.tiles && ok; ++j)      // the scores' place holds the probabilities until the product has them
-            ok = scores(j) && sums(j) && bar_wait(o_done(g), (done + j) & 1, p.status);
-          done += s.tiles;
+          mma_commit(v_empty(g, v_stage));
         }
+        __syncwarp();
+        // the scores' place holds the probabilities until the product has them; after the last, Q's place is free too
+        ok = wait(o_done(g), done & 1);
       }
     }
   } else {
-    // ---- softmax: thread r has row r of its slot ----
-    const int g = warp >= 8 ? 1 : 0, r = (warp & 3) * 32 + lane;
+    // ---- softmax: thread r has row r of its slot, and 64 of the 128 keys of a tile ----
+    const int g = (warp - 4) >> 3, part = (warp - 4) >> 2 & 1, r = (warp & 3) * 32 + lane, pair = g * 4 + (warp & 3);
     const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_row = tmem_s(g) + lane_addr, o_row = tmem_o(g) + lane_addr, p_row = tmem_p(g) + lane_addr;
+    const uint32_t s_row = tmem_s(g) + lane_addr + part * kHalf, o_row = tmem_o(g) + lane_addr;
+    float* my_xchg = xchg + (g * 2 + part) * 128 + r;
+    const float* pair_xchg = xchg + (g * 2 + (part ^ 1)) * 128 + r;
     const ScoreScale sc = make_score_scale(p.scale, p.softcap);
-    const bool has_cap = p.softcap > 0.f;
     bool ok = true;
     int done = 0, before = 0;
-    for (; any; any = tree_next(p, &w)) {
+    for (; any; next_piece()) {
       const TreeUnit u = tree_unit(p, w.t, w.unit);
-      const Slot s = slot_of(p, w, u, g);
-      const bool live = r < s.rows, warp_live = (warp & 3) * 32 < s.rows;
-      const int row = s.first_node * u.heads + r;                  // of the unit
-      const int token = w.t.first + u.first_node + (live ? s.first_node + r / u.heads : 0);
-      const int position = live ? tree_position(p, w.t, token) : 0;
-      const int lowest = live ? tree_lowest(p, position) : 0;
+      const Slot s = slot_of(w, u, g);
+      const bool warp_live = (warp & 3) * 32 < s.rows;
+      const int unit_row = s.first_node * u.heads + r;
+      Row row;
+      row.live = r < s.rows;
+      const int node = divide(r, u.heads);
+      row.token = w.t.first + u.first_node + (row.live ? s.first_node + node : 0);
+      row.position = row.live ? tree_position(p, w.t, row.token) : 0;
+      row.lowest = row.live ? tree_lowest(p, row.position) : 0;
+      row.m = -INFINITY;
+      row.l = 0.f;
+      // keys that every row of the warp sees, but for those from the drafted ones on
+      const int all_from = p.window > 0 ? __reduce_max_sync(0xffffffffu, row.lowest) : 0;
       const int first = before + s.first_tile - w.tile_begin;
       before += w.tile_end - w.tile_begin;
-      float m_ref = -INFINITY, l_run = 0.f;
       if (s.tiles > 0 && warp_live) {
-        float zero[32];
+        uint32_t zero[16];
 #pragma unroll
-        for (int c = 0; c < 32; ++c) zero[c] = 0.f;
-#pragma unroll
-        for (int c0 = 0; c0 < D; c0 += 32) tmem_st32(o_row + c0, zero);
+        for (int c = 0; c < 16; ++c) zero[c] = 0u;
+#pragma unroll 1
+        for (int c0 = part * (D / 2); c0 < (part + 1) * (D / 2); c0 += 16) tmem_st16(o_row + c0, zero);
       }
-      for (int j = 0; j < s.tiles; ++j, ++done) {
-        if (ok) ok = __all_sync(0xffffffffu, bar_wait(s_full(g), done & 1, p.status));
+#pragma unroll 1
+      for (int j = 0; j < s.tiles; ++j, ++done) {      // `done` counts this slot's tiles
+        if (ok) ok = __all_sync(0xffffffffu, bar_wait_likely_done(s_full(g), done & 1, p.status));
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (!warp_live || !ok) {
-          if (L::kOwnP) bar_arrive(s_free(g));
-          bar_arrive(p_full(g));
-          continue;
-        }
-        const int tile = s.first_tile + j * s.step, key0 = w.t.begin + tile * kTile;
-        const bool all_visible = __all_sync(0xffffffffu, !live || (key0 + kTile <= w.t.cached && key0 >= lowest));
-        uint32_t seen[4];
-        if (!all_visible) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) seen[c] = live ? tree_visible(p, w.t, token, lowest, position, key0 + 32 * c) : 0u;
-          __syncwarp();
-        }
-        // The second product of this slot's previous tile is complete: with scores and probabilities in one place the scores
-        // could not be there otherwise.
-        auto wait_product = [&]() {
-          if (L::kOwnP && j > 0) {
-            ok = __all_sync(0xffffffffu, bar_wait_likely_done(o_done(g), (done - 1) & 1, p.status)) && ok;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (warp_live) {
+          const int tile0 = w.t.begin + (s.first_tile + j * s.step) * kTile, key0 = tile0 + part * kHalf;
+          const bool all_visible = key0 >= all_from && key0 + kHalf <= w.t.cached;
+          uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
+          if (!all_visible) {
+#pragma unroll 1
+            for (int c = 0; c < 2; ++c) {
+              const uint32_t bits = row.live ? tree_visible(p, w.t, row.token, row.lowest, row.position, key0 + 32 * c) : 0u;
+              if (c) seen[1] = bits;
+              else seen[0] = bits;
+            }
+            __syncwarp();
           }
-        };
-        auto walk = [&](auto masked_tag) {
-          constexpr bool kMasked = decltype(masked_tag)::value;
           auto mask = [&](float* v, uint32_t bits) {
 #pragma unroll
             for (int c = 0; c < 32; ++c) v[c] = bits >> c & 1u ? v[c] : -INFINITY;
           };
           float top = -INFINITY;
 #pragma unroll 1
-          for (int c0 = 0; c0 < kTile; c0 += 64) {
-            float a[32], b[32];
-            tmem_ld32(s_row + c0, a);
-            tmem_ld32(s_row + c0 + 32, b);
-            tmem_ld_wait();
-            if (kMasked) {
-              mask(a, c0 ? seen[2] : seen[0]);
-              mask(b, c0 ? seen[3] : seen[1]);
-            }
-            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          for (int c0 = 0; c0 < kHalf; c0 += 32) {
+            float v[32];
+            tmem_ld32(s_row + c0, v);
+            tmem_ld_wait32(v);
+            if (!all_visible) mask(v, c0 ? seen[1] : seen[0]);
+            float top4[4];
 #pragma unroll
-            for (int c = 0; c < 32; ++c) m4[c & 3] = fmaxf(m4[c & 3], fmaxf(a[c], b[c]));
-            top = fmaxf(top, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+            for (int c = 0; c < 4; ++c) top4[c] = max3(v[c], v[c + 4], v[c + 8]);
+#pragma unroll
+            for (int c = 12; c < 28; c += 8)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) top4[e] = max3(top4[e], v[c + e], v[c + 4 + e]);
+            top = max3(top, max3(top4[0], top4[1], v[28]), max3(max3(top4[2], top4[3], v[29]), v[30], v[31]));
           }
+          // the scale is positive and the cap grows with the score: the maximum and either commute
           top = top == -INFINITY ? -INFINITY : score_log2(top, sc);
-          const bool move = live && top > (m_ref == -INFINITY ? -INFINITY : m_ref + kMove);
-          wait_product();
-          if (__any_sync(0xffffffffu, move)) {
-            const float factor = !move ? 1.f : m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - top);
-            if (j > 0) {
+          // where a row has no reference yet, or a score far above it, the two warps with it settle on one
+          if (pair_any(pair, row.live && top > (row.m == -INFINITY ? -INFINITY : row.m + kMove))) {
+            *my_xchg = top;
+            pair_sync(pair);
+            top = fmaxf(fmaxf(top, *pair_xchg), row.m);
+            const float factor = top == -INFINITY ? 1.f : row.m == -INFINITY ? 0.f : fast_exp2(row.m - top);
+            if (j > 0) {      // (the product of the tile before is complete: these scores lie in its probabilities' place)
 #pragma unroll 1
-              for (int c0 = 0; c0 < D; c0 += 32) {
-                float v[32];
-                tmem_ld32(o_row + c0, v);
+              for (int c0 = part * (D / 2); c0 < (part + 1) * (D / 2); c0 += 16) {
+                float o[16];
+                tmem_ld16(o_row + c0, o);
                 tmem_ld_wait();
+                uint32_t bits[16];
 #pragma unroll
-                for (int c = 0; c < 32; ++c) v[c] *= factor;
-                tmem_st32(o_row + c0, v);
+                for (int c = 0; c < 16; ++c) bits[c] = __float_as_uint(o[c] * factor);
+                tmem_st16(o_row + c0, bits);
               }
             }
-            l_run = l_run == 0.f ? 0.f : l_run * factor;
-            if (move) m_ref = top;
+            row.l = row.l == 0.f ? 0.f : row.l * factor;
+            row.m = top;
+            pair_sync(pair);      // before either writes its place again
           }
-          const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+          const float m_use = row.m == -INFINITY ? 0.f : row.m;
           const float2 scale2 = make_float2(sc.scale_log2, sc.scale_log2), shift2 = make_float2(-m_use, -m_use);
-          float2 sum2 = make_float2(0.f, 0.f);
-          auto exps = [&](float* v, uint32_t bits, int c0) {
-            if (kMasked) mask(v, bits);
-            if (has_cap) {
+          float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll 1
+          for (int c0 = 0; c0 < kHalf; c0 += 32) {
+            float v[32];
+            tmem_ld32(s_row + c0, v);
+            tmem_ld_wait32(v);
+            if (!all_visible) mask(v, c0 ? seen[1] : seen[0]);
+            if (sc.tanh_in != 0.f) {
 #pragma unroll
-              for (int c = 0; c < 32; ++c) {
-                const float x = kMasked && v[c] == -INFINITY ? -INFINITY : capped(v[c], sc) - m_use;
-                v[c] = fast_exp2(x);
-              }
-            } else {
-#pragma unroll
-              for (int c = 0; c < 32; c += 2) {
-                const float2 x = __ffma2_rn(make_float2(v[c], v[c + 1]), scale2, shift2);
-                v[c] = fast_exp2(x.x);
-                v[c + 1] = fast_exp2(x.y);
-              }
+              for (int c = 0; c < 32; ++c) v[c] = v[c] == -INFINITY ? -INFINITY : __fdividef(capped(v[c], sc), sc.scale_log2);
             }
             uint32_t packed[16];
 #pragma unroll
             for (int c = 0; c < 32; c += 2) {
-              sum2 = __fadd2_rn(sum2, make_float2(v[c], v[c + 1]));
-              packed[c >> 1] = pack_pair(v[c], v[c + 1]);
+              const float2 x = __ffma2_rn(make_float2(v[c], v[c + 1]), scale2, shift2);
+              const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+              sum2[c >> 1 & 1] = __fadd2_rn(sum2[c >> 1 & 1], e);
+              packed[c >> 1] = pack_pair(e.x, e.y);
             }
-            tmem_st16(p_row + (c0 >> 1), packed);      // two keys to a column
-          };
-#pragma unroll 1
-          for (int c0 = 0; c0 < kTile; c0 += 64) {
-            float a[32], b[32];
-            tmem_ld32(s_row + c0, a);
-            tmem_ld_wait32(a);
-            tmem_ld32(s_row + c0 + 32, b);
-            exps(a, kMasked ? (c0 ? seen[2] : seen[0]) : 0u, c0);
-            tmem_ld_wait32(b);
-            if (L::kOwnP && c0 > 0) {
-              asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-              bar_arrive(s_free(g));
-            }
-            exps(b, kMasked ? (c0 ? seen[3] : seen[1]) : 0u, c0 + 32);
+            tmem_st16(s_row + (c0 >> 1), packed);      // two keys to a column, over scores that were read
           }
-          l_run += sum2.x + sum2.y;
-        };
-        if (all_visible) {
-          walk(std::false_type{});
-        } else {
-          walk(std::true_type{});
-          // values that are not finite, for the rows that see their keys
-          const int c = first + j * s.step, stage = c % L::kVStages;
-          ok = __all_sync(0xffffffffu, bar_wait_likely_done(v_checked(stage), (c / L::kVStages) & 1, p.status)) && ok;
+          row.l += (sum2[0].x + sum2[1].x) + (sum2[0].y + sum2[1].y);
+          if (tile0 < all_from || tile0 + kTile > w.t.cached) {
+            // Values that are not finite, for the rows that see their keys: the two warps one after the other.
+            const int c = first + j * s.step, stage = c % L::kVStages;
+            const uint32_t* named = cleared + stage * 4;
+            ok = __all_sync(0xffffffffu, bar_wait_likely_done(v_checked(stage), (c / L::kVStages) & 1, p.status)) && ok;
+            tmem_st_wait();
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            if (pair_any(pair, ok && (named[0] | named[1] | named[2] | named[3]) != 0u)) {
 #pragma unroll 1
-          for (int word = 0; word < 4; ++word) {
-            const uint32_t mine = cleared[stage * 4 + word] & seen[word];
-            for (uint32_t rest = __reduce_or_sync(0xffffffffu, mine); rest; rest &= rest - 1) {
-              const int bit = __ffs(rest) - 1, key = key0 + 32 * word + bit;
-              const int page = p.block_table[(size_t)w.request * p.table_width + key / p.page_size];
-              const bool add = (mine >> bit & 1u) && page >= 0 && page < p.num_pages;
-              const __nv_bfloat16* value = static_cast<const __nv_bfloat16*>(p.v_cache) +
-                  (((size_t)(add ? page : 0) * p.kv_heads + u.kv_head) * p.page_size + key % p.page_size) * D;
+              for (int word = 0; word < 4; ++word) {
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t mine = word >> 1 == part && ok ? named[word] & (word & 1 ? seen[1] : seen[0]) : 0u;
 #pragma unroll 1
-              for (int c0 = 0; c0 < D; c0 += 32) {
-                float v[32];
-                tmem_st_wait();
-                tmem_ld32(o_row + c0, v);
-                tmem_ld_wait();
+                for (uint32_t rest = __reduce_or_sync(0xffffffffu, mine); rest; rest &= rest - 1) {
+                  const int bit = __ffs(rest) - 1, key = tile0 + 32 * word + bit;
+                  const int page = p.block_table[(size_t)w.request * p.table_width + key / p.page_size];
+                  const bool add = (mine >> bit & 1u) && page >= 0 && page < p.num_pages;
+                  const __nv_bfloat16* value = static_cast<const __nv_bfloat16*>(p.v_cache) +
+                      (((size_t)(add ? page : 0) * p.kv_heads + u.kv_head) * p.page_size + key % p.page_size) * D;
+#pragma unroll 1
+                  for (int c0 = 0; c0 < D; c0 += 16) {
+                    float o[16];
+                    tmem_st_wait();
+                    tmem_ld16(o_row + c0, o);
+                    tmem_ld_wait();
+                    uint32_t bits[16];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                  const float x = add ? __bfloat162float(value[c0 + e]) : 0.f;
-                  if (!isfinite(x)) v[e] += x;       // times a weight above zero
+                    for (int e = 0; e < 16; ++e) {
+                      const float x = add ? __bfloat162float(value[c0 + e]) : 0.f;
+                      bits[e] = __float_as_uint(isfinite(x) ? o[e] : o[e] + x);       // times a weight above zero
+                    }
+                    tmem_st16(o_row + c0, bits);
+                  }
                 }
-                tmem_st32(o_row + c0, v);
+                tmem_st_wait();
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                pair_sync(pair);
               }
             }
           }
+          tmem_st_wait();
         }
-        tmem_st_wait();
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         bar_arrive(p_full(g));
       }
@@ -495,58 +591,66 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
         ok = __all_sync(0xffffffffu, bar_wait(o_done(g), (done - 1) & 1, p.status));
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       }
-      // The row's sums: this slot's alone, or, where both slots had the same rows, both slots', half of the head each.
-      float m = m_ref, l = l_run, mine = 1.f, other = 0.f;
-      int d0 = 0, d1 = D;
+      // The row's sums: this slot's alone, half of the head to a warp, or, where both slots had the same rows, both slots',
+      // a quarter of the head to a warp.
+      *my_xchg = row.l;
+      pair_sync(pair);
+      float m = row.m, l = row.l + *pair_xchg, mine = 1.f, other = 0.f;
+      int d0 = part * (D / 2), d1 = d0 + D / 2;
       if (!s.pair) {
-        xchg[g * 128 + r] = make_float2(m_ref, l_run);
+        pair_sync(pair);
+        *my_xchg = part ? l : m;
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         both_slots_sync();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const float2 theirs = xchg[(g ^ 1) * 128 + r];
-        m = fmaxf(m_ref, theirs.x);
-        mine = m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - m);
-        other = theirs.x == -INFINITY ? 0.f : fast_exp2(theirs.x - m);
-        l = (l_run == 0.f ? 0.f : l_run * mine) + (theirs.y == 0.f ? 0.f : theirs.y * other);
-        d0 = g * (D / 2);
-        d1 = d0 + D / 2;
+        const float m_other = xchg[(g ^ 1) * 256 + r], l_other = xchg[(g ^ 1) * 256 + 128 + r];
+        m = fmaxf(row.m, m_other);
+        mine = row.m == -INFINITY ? 0.f : fast_exp2(row.m - m);
+        other = m_other == -INFINITY ? 0.f : fast_exp2(m_other - m);
+        l = (l == 0.f ? 0.f : l * mine) + (l_other == 0.f ? 0.f : l_other * other);
+        d0 = (g * 2 + part) * (D / 4);
+        d1 = d0 + D / 4;
+      } else if (cluster > 1) {
+        both_slots_sync();      // the tiles' place, which the sums take, is the other slot's too
       }
-      const bool write = live && ok;
+      const bool write = row.live && ok;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const uint32_t o_other = tmem_o(g ^ 1) + lane_addr;
-      const size_t share = (size_t)w.share * p.unit_rows + row;
-      __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + ((size_t)token * p.heads + u.first_head + (live ? r % u.heads : 0)) * D;
+      float* left = reinterpret_cast<float*>(smem_raw + L::kSums) + unit_row * L::kPitch;
+      __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + ((size_t)row.token * p.heads + u.first_head + (row.live ? r - node * u.heads : 0)) * D;
       if (warp_live) {
 #pragma unroll 1
-        for (int c0 = d0; c0 < d1; c0 += 32) {
-          float v[32], x[32];
-          tmem_ld32(o_row + c0, v);
-          if (!s.pair) tmem_ld32(o_other + c0, x);
+        for (int c0 = d0; c0 < d1; c0 += 16) {
+          float v[16], x[16];
+          tmem_ld16(o_row + c0, v);
+          if (!s.pair) tmem_ld16(o_other + c0, x);
           tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
+          for (int c = 0; c < 16; ++c) {
             v[c] = mine == 0.f ? 0.f : v[c] * mine;
             if (!s.pair && other != 0.f) v[c] += x[c] * other;
           }
-          if (write && w.whole) {
+          if (write && cluster == 1 && w.whole) {
 #pragma unroll
-            for (int d = 0; d < 32; d += 8) {
-              uint4 raw;
-              raw.x = pack_pair(v[d] * inv, v[d + 1] * inv);
-              raw.y = pack_pair(v[d + 2] * inv, v[d + 3] * inv);
-              raw.z = pack_pair(v[d + 4] * inv, v[d + 5] * inv);
-              raw.w = pack_pair(v[d + 6] * inv, v[d + 7] * inv);
-              *reinterpret_cast<uint4*>(dst + c0 + d) = raw;
-            }
+            for (int d = 0; d < 16; d += 8)
+              *reinterpret_cast<uint4*>(dst + c0 + d) =
+                  make_uint4(pack_pair(v[d] * inv, v[d + 1] * inv), pack_pair(v[d + 2] * inv, v[d + 3] * inv),
+                             pack_pair(v[d + 4] * inv, v[d + 5] * inv), pack_pair(v[d + 6] * inv, v[d + 7] * inv));
           } else if (write) {
+            // a share: a cluster's, in shared memory, or a worker's
+            float* to = cluster > 1 ? left + c0 : tree_share(p, w.share, unit_row, c0);
+            const int step4 = cluster > 1 ? 4 : 128;
 #pragma unroll
-            for (int d = 0; d < 32; d += 4)
-              *reinterpret_cast<float4*>(p.part_o + share * D + c0 + d) = make_float4(v[d], v[d + 1], v[d + 2], v[d + 3]);
+            for (int d = 0; d < 4; ++d)
+              *reinterpret_cast<float4*>(to + d * step4) = make_float4(v[4 * d], v[4 * d + 1], v[4 * d + 2], v[4 * d + 3]);
           }
           __syncwarp();
         }
       }
-      if (write && !w.whole && d0 == 0) p.part_ml[share] = make_float2(m, l);
+      if (write && part == 0 && (s.pair || g == 0)) {
+        if (cluster > 1) reinterpret_cast<float2*>(smem_raw + L::kSumsMl)[unit_row] = make_float2(m, l);
+        else if (!w.whole) p.part_ml[(size_t)w.share * p.unit_rows + unit_row] = make_float2(m, l);
+      }
       if (!s.pair) {
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         both_slots_sync();
@@ -589,7 +693,7 @@ int launch_tree(const TreeParams& p, cudaStream_t stream) {
   const auto kernel = tree_attention_tcgen05_kernel<D>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kBytes);
   if (e != cudaSuccess) return (int)e;
-  e = launch_pdl(kernel, dim3(p.ctas), dim3(kTreeThreads), Layout<D>::kBytes, stream, map_q, map_k, map_v, run_k, run_v, p);
+  e = launch_pdl_cluster(kernel, dim3(p.workers * p.cluster), dim3(kTreeThreads), Layout<D>::kBytes, p.cluster, stream, map_q, map_k, map_v, run_k, run_v, p);
   if (e != cudaSuccess) return (int)e;
   return tree_merge<__nv_bfloat16>(p, stream);
 }
@@ -598,26 +702,47 @@ int launch_tree(const TreeParams& p, cudaStream_t stream) {
 
 using namespace einf;
 
-// The arguments of einf_tree_attention without a dtype.  part_o: [2 * ctas][rows][size] floats with
-// rows = 2 * (128 / (heads / kv_heads)) * (heads / kv_heads), part_ml: [2 * ctas][rows][2], notes: [ctas][4].
-extern "C" int einf_tree_attention_tcgen05(const void* q, const void* k_cache, const void* v_cache, const int* block_table,
-                                           const int* q_start, const int* cached_lens, const void* mask, const int* positions,
-                                           void* out, float* part_o, float* part_ml, int* notes, int requests, int tokens, int heads,
-                                           int kv_heads, int size, int page_size, int num_pages, int table_width, int words,
-                                           int window, float scale, float softcap, int ctas, int min_chunk, int* status,
-                                           cudaStream_t stream) {
-  if (requests == 0 || tokens == 0) return 0;
-  if ((size != 64 && size != 128) || ctas < 1 || min_chunk < 1 || kv_heads < 1 || heads % kv_heads || heads / kv_heads > kTile ||
-      page_size < 8 || page_size > 128 || (page_size & (page_size - 1)) || words < 1 || (window > 0 && !positions) ||
-      ((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) % 16)
+// How many clusters of `cluster` CTAs the device holds at once; 0 on error.
+extern "C" int einf_tree_attention_tcgen05_max_clusters(int cluster) {
+  if (cluster < 1 || cluster > 8) return 0;
+  const auto kernel = tree_attention_tcgen05_kernel<128>;      // the other takes as much of an SM: one CTA
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(cluster);
+  config.blockDim = dim3(kTreeThreads);
+  config.dynamicSmemBytes = Layout<128>::kBytes;
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = cluster;
+  attribute.val.clusterDim.y = 1;
+  attribute.val.clusterDim.z = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  int clusters = 0;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<128>::kBytes) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&clusters, kernel, &config) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return clusters;
+}
+
+// call: a TreeCall, on the host; a worker is a cluster of 1 to 8 CTAs.  part_o: [2 * workers][256][size] floats, part_ml:
+// [2 * workers][256][2], notes: [workers][8]; none of them where every unit has one worker (whole).
+extern "C" int einf_tree_attention_tcgen05(const char* call, cudaStream_t stream) {
+  const TreeCall& c = *reinterpret_cast<const TreeCall*>(call);
+  if (c.requests == 0 || c.tokens == 0) return 0;
+  if (!tree_call_fits(c) || c.cluster > 8 || c.dtype != kBFloat16 || (c.size != 64 && c.size != 128) || c.heads / c.kv_heads > kTile ||
+      c.page_size < 8 || c.page_size > 128 || (c.page_size & (c.page_size - 1)) ||
+      ((uintptr_t)c.q | (uintptr_t)c.k_cache | (uintptr_t)c.v_cache | (uintptr_t)c.out) % 16)
     return (int)cudaErrorInvalidValue;
-  TreeParams p = tree_params(q, k_cache, v_cache, block_table, q_start, cached_lens, mask, positions, out, part_o, part_ml, notes,
-                             requests, tokens, heads, kv_heads, size, page_size, num_pages, table_width, words, window, scale, softcap,
-                             ctas, min_chunk, status);
-  p.unit_heads = heads / kv_heads;
+  TreeParams p = tree_params(c);
+  p.unit_heads = c.heads / c.kv_heads;
   p.unit_nodes = 2 * (kTile / p.unit_heads);
-  p.unit_rows = p.unit_nodes * p.unit_heads;
-  p.padded = size;
-  p.tile_keys = kTile;
-  return size == 64 ? launch_tree<64>(p, stream) : launch_tree<128>(p, stream);
+  p.group = p.unit_heads;
+  p.head_blocks = 1;
+  p.unit_rows = 2 * kTile;
+  p.padded = c.size;
+  p.tile_shift = 7;
+  static_assert(kTile == 128, "a tile of keys");
+  return c.size == 64 ? launch_tree<64>(p, stream) : launch_tree<128>(p, stream);
 }

@@ -7,6 +7,7 @@ namespace einf {
 
 constexpr int kWalkNodes = 1024;      // nodes whose children lie in shared memory
 
+// A call's arguments, as the caller packs them.
 struct WalkParams {
   const int* tokens;       // [rows]: a node's token
   const int* targets;      // [rows]: the model's token behind that node
@@ -15,8 +16,9 @@ struct WalkParams {
   int* path;               // [requests, depth]: the kept nodes, -1 behind the last
   int* answer;             // [requests, depth]: the tokens that the step answers, -1 behind the last
   int* counts;             // [requests]
-  int rows, depth;
+  int rows, requests, depth, more;
 };
+static_assert(sizeof(WalkParams) == 7 * 8 + 4 * 4, "as packed");
 
 // A warp per request.  Every node that agrees with its parent's target reports to that parent, which keeps the lowest
 // (an integer minimum: no order of arrival shows); the walk from the root then is a chain of reads of shared memory.
@@ -79,14 +81,20 @@ struct MoveTensor {
   int first_column;        // of the launch's columns
   int row_units;
 };
-struct MoveParams {
-  MoveTensor tensors[kMoveTensors];
+// A call's arguments, as the caller packs them.
+struct MoveCall {
   const int* block_table;  // [requests, table_width]
   const int* cached_lens;
   const int* path;         // [requests, depth]
   const int* counts;
   int* status;
-  int count, columns, depth, page_size, num_pages, table_width;
+  int requests, depth, table_width, more;
+};
+static_assert(sizeof(MoveCall) == 5 * 8 + 4 * 4, "as packed");
+struct MoveParams {
+  MoveTensor tensors[kMoveTensors];
+  MoveCall call;
+  int count, columns, page_size, num_pages;
 };
 
 // A column is one unit (16 bytes where all rows allow it) of one head's row in one tensor; a thread takes a column and
@@ -98,9 +106,9 @@ __global__ void __launch_bounds__(kMoveThreads) move_accepted_kernel(const __gri
   pdl_launch_dependents();
   pdl_wait();
   const int request = blockIdx.x;
-  const int count = max(0, min(p.counts[request], p.depth)), cached = p.cached_lens[request];
-  const int* path = p.path + (size_t)request * p.depth;
-  const int* table = p.block_table + (size_t)request * p.table_width;
+  const int count = max(0, min(p.call.counts[request], p.call.depth)), cached = p.call.cached_lens[request];
+  const int* path = p.call.path + (size_t)request * p.call.depth;
+  const int* table = p.call.block_table + (size_t)request * p.call.table_width;
   const int column = blockIdx.y * kMoveThreads + threadIdx.x;
   Unit* base = nullptr;
   int head = 0, unit = 0, row_units = 0, heads = 1;
@@ -119,13 +127,13 @@ __global__ void __launch_bounds__(kMoveThreads) move_accepted_kernel(const __gri
     unit = (column - p.tensors[low].first_column) % row_units;
   }
   auto place = [&](int at) -> long long {     // page and row of a place, or -1
-    if (at < 0 || at / p.page_size >= p.table_width) {
-      atomicOr(p.status, kStatusBadPage);
+    if (at < 0 || at / p.page_size >= p.call.table_width) {
+      atomicOr(p.call.status, kStatusBadPage);
       return -1;
     }
     const int page = table[at / p.page_size];
     if (page < 0 || page >= p.num_pages) {
-      atomicOr(p.status, kStatusBadPage);
+      atomicOr(p.call.status, kStatusBadPage);
       return -1;
     }
     return (long long)page << 32 | (unsigned)(at % p.page_size);
@@ -135,7 +143,7 @@ __global__ void __launch_bounds__(kMoveThreads) move_accepted_kernel(const __gri
     for (int i = i0 + threadIdx.x; i < min(count, i0 + kMoveSteps); i += kMoveThreads) {
       const int step = path[i];
       long long a = -1, b = -1;
-      if (step < i || step <= path[i - 1]) atomicOr(p.status, kStatusBadIndex);
+      if (step < i || step <= path[i - 1]) atomicOr(p.call.status, kStatusBadIndex);
       else if (step != i) a = place(cached + step), b = place(cached + i);
       from[i - i0] = b < 0 ? -1 : a;
       to[i - i0] = b;
@@ -162,38 +170,33 @@ __global__ void __launch_bounds__(kMoveThreads) move_accepted_kernel(const __gri
 
 using namespace einf;
 
-extern "C" int einf_accept_drafts(const int* tokens, const int* targets, const int* parents, const int* q_start, int* path,
-                                  int* answer, int* counts, int rows, int requests, int depth, cudaStream_t stream) {
-  if (requests == 0) return 0;
-  if (depth < 1) return (int)cudaErrorInvalidValue;
-  const WalkParams p = {tokens, targets, parents, q_start, path, answer, counts, rows, depth};
-  return (int)launch_pdl(accept_drafts_kernel, dim3(requests), dim3(32), 0, stream, p);
+// call: a WalkParams, on the host.
+extern "C" int einf_accept_drafts(const char* call, cudaStream_t stream) {
+  const WalkParams& p = *reinterpret_cast<const WalkParams*>(call);
+  if (p.requests == 0) return 0;
+  if (p.depth < 1) return (int)cudaErrorInvalidValue;
+  return (int)launch_pdl(accept_drafts_kernel, dim3(p.requests), dim3(32), 0, stream, p);
 }
 
-extern "C" int einf_move_accepted_tensors() { return kMoveTensors; }
-
-// bases, heads, row_units: per tensor, on the host; unit: bytes of a unit (2, 4, 8 or 16).
-extern "C" int einf_move_accepted(void* const* bases, const int* heads, const int* row_units, int count, int unit,
-                                  const int* block_table, const int* cached_lens, const int* path, const int* counts, int requests,
-                                  int depth, int page_size, int num_pages, int table_width, int* status, cudaStream_t stream) {
-  if (requests == 0 || count == 0 || depth < 2) return 0;
-  if (count > kMoveTensors || page_size < 1) return (int)cudaErrorInvalidValue;
-  MoveParams p = {};
+// tensors: how many, bytes of a unit (2, 4, 8 or 16), page size, pages, then each tensor's address, heads and units of a
+// row; call: a MoveCall.  Both on the host.
+extern "C" int einf_move_accepted(const long long* tensors, const char* call, cudaStream_t stream) {
+  const MoveCall& c = *reinterpret_cast<const MoveCall*>(call);
+  const long long count = tensors[0], unit = tensors[1];
+  if (c.requests == 0 || count == 0 || c.depth < 2) return 0;
+  if (count < 0 || count > kMoveTensors || tensors[2] < 1) return (int)cudaErrorInvalidValue;
+  MoveParams p;
+  p.call = c;
+  p.count = (int)count;
+  p.columns = 0;
+  p.page_size = (int)tensors[2];
+  p.num_pages = (int)tensors[3];
   for (int t = 0; t < count; ++t) {
-    p.tensors[t] = {bases[t], p.columns, row_units[t]};
-    p.columns += heads[t] * row_units[t];
+    const long long* tensor = tensors + 4 + 3 * t;
+    p.tensors[t] = {reinterpret_cast<void*>(tensor[0]), p.columns, (int)tensor[2]};
+    p.columns += (int)(tensor[1] * tensor[2]);
   }
-  p.block_table = block_table;
-  p.cached_lens = cached_lens;
-  p.path = path;
-  p.counts = counts;
-  p.status = status;
-  p.count = count;
-  p.depth = depth;
-  p.page_size = page_size;
-  p.num_pages = num_pages;
-  p.table_width = table_width;
-  const dim3 grid(requests, (p.columns + kMoveThreads - 1) / kMoveThreads);
+  const dim3 grid(c.requests, (p.columns + kMoveThreads - 1) / kMoveThreads);
   if (grid.y > 65535) return (int)cudaErrorInvalidValue;
   switch (unit) {
     case 16: return (int)launch_pdl(move_accepted_kernel<uint4>, grid, dim3(kMoveThreads), 0, stream, p);

@@ -14,29 +14,34 @@
 namespace einf {
 
 constexpr int kShapeThreads = 256;
+constexpr int kMostPlaces = 16384;            // of a CTA's piece of the vocabulary
 constexpr uint32_t kInPrompt = 1u << 31;      // a place's word: in the prompt, some node's token, how often answered
 constexpr uint32_t kDrafted = 1u << 30;
 constexpr uint32_t kCount = kDrafted - 1;
 
+// A call's arguments, as the caller packs them.
 struct ShapeParams {
   const float* logits;         // [rows, vocab]
   float* out;
-  const int* row_start;        // [requests + 1], or null: a row each
-  const int* history;          // [requests, capacity] or null
+  int* status;
   const int* history_lens;     // [requests]
-  const int* prompt_lens;      // [requests]: so many of the history's tokens are the prompt's
+  const int* prompt_lens;      // [requests] or null: so many of the history's tokens are the prompt's
   const float* repetition;     // [requests] or null: 1
   const float* presence;       // [requests] or null: 0
   const float* frequency;
+  const int* row_start;        // [requests + 1], or null: a row each
+  const int* history;          // [requests, capacity] or null
   const int* node_tokens;      // [rows] or null
   const uint32_t* tree_mask;   // [rows, 2 * words]
   const int* bias_ids;         // [requests, biases], negative: none
   const float* bias;
   const uint32_t* allowed;     // [masks, mask_words] or null
   const int* allowed_rows;     // [rows] or null: row r has mask r
-  int* status;
-  int rows, vocab, requests, capacity, words, biases, masks, mask_words, piece;
+  int rows, vocab, requests, capacity, words, biases, masks, mask_words;
+  int piece;                   // places of the vocabulary that a CTA has, a multiple of 32
+  int row_ways;                // CTAs that take a request's rows in turn
 };
+static_assert(sizeof(ShapeParams) == 16 * 8 + 10 * 4, "as packed");
 
 struct ShapeRequest {
   float repetition, presence, frequency;
@@ -205,25 +210,18 @@ __global__ void __launch_bounds__(kShapeThreads) shape_logits_kernel(ShapeParams
 
 using namespace einf;
 
-// piece: places of the vocabulary that a CTA has, a multiple of 32; row_ways: CTAs that take a request's rows in turn.
-extern "C" int einf_shape_logits(const float* logits, float* out, const int* row_start, const int* history, const int* history_lens,
-                                 const int* prompt_lens, const float* repetition, const float* presence, const float* frequency,
-                                 const int* node_tokens, const void* tree_mask, const int* bias_ids, const float* bias,
-                                 const void* allowed, const int* allowed_rows, int rows, int vocab, int requests, int capacity,
-                                 int words, int biases, int masks, int mask_words, int piece, int row_ways, int* status,
-                                 cudaStream_t stream) {
-  if (rows == 0 || requests == 0) return 0;
-  if (vocab < 1 || piece < 32 || piece % 32 || piece > 16384 || row_ways < 1 || row_ways > 65535 || requests > 65535 || (node_tokens && !tree_mask) ||
-      (history && !history_lens))
+// call: a ShapeParams, on the host.
+extern "C" int einf_shape_logits(const char* call, cudaStream_t stream) {
+  const ShapeParams& p = *reinterpret_cast<const ShapeParams*>(call);
+  if (p.rows == 0 || p.requests == 0) return 0;
+  if (p.vocab < 1 || p.piece < 32 || p.piece % 32 || p.piece > kMostPlaces || p.row_ways < 1 || p.row_ways > 65535 || p.requests > 65535 ||
+      (p.node_tokens && !p.tree_mask) || (p.history && !p.history_lens))
     return (int)cudaErrorInvalidValue;
-  ShapeParams p = {logits, out, row_start, history, history_lens, prompt_lens, repetition, presence, frequency, node_tokens,
-                   static_cast<const uint32_t*>(tree_mask), bias_ids, bias, static_cast<const uint32_t*>(allowed), allowed_rows,
-                   status, rows, vocab, requests, capacity, words, biases, masks, mask_words, piece};
-  const bool has_bias = biases > 0, vec = vocab % 4 == 0 && (((uintptr_t)logits | (uintptr_t)out) & 15) == 0;
+  const bool has_bias = p.biases > 0, vec = p.vocab % 4 == 0 && (((uintptr_t)p.logits | (uintptr_t)p.out) & 15) == 0;
   const auto kernel = vec ? (has_bias ? shape_logits_kernel<4, true> : shape_logits_kernel<4, false>)
                           : (has_bias ? shape_logits_kernel<1, true> : shape_logits_kernel<1, false>);
-  const size_t smem = (size_t)piece * 4 * (has_bias ? 2 : 1);
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * 16384 * 4);
+  const size_t smem = (size_t)p.piece * 4 * (has_bias ? 2 : 1);
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kMostPlaces * 4);
   if (e != cudaSuccess) return (int)e;
-  return (int)launch_pdl(kernel, dim3((vocab + piece - 1) / piece, requests, row_ways), dim3(kShapeThreads), smem, stream, p);
+  return (int)launch_pdl(kernel, dim3((p.vocab + p.piece - 1) / p.piece, p.requests, p.row_ways), dim3(kShapeThreads), smem, stream, p);
 }

@@ -12,7 +12,8 @@ from __future__ import annotations
 
 import ctypes
 import functools
-from ctypes import c_float, c_int, c_longlong, c_void_p
+import struct
+from ctypes import c_char_p, c_float, c_int, c_longlong, c_void_p
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -3501,22 +3502,38 @@ def sample(
 # ``accept_drafts`` walks the tree by the tokens that the model gave, and ``move_accepted`` closes the gaps in the cache.
 
 
-def _here(device: torch.device, *tensors: Optional[torch.Tensor]) -> None:
-    """Every tensor lies on ``device``, and a launch goes there."""
-    if device.type != "cuda":
-        raise KernelError(f"a tensor is on {device}: the kernels run on a CUDA device only and have no CPU path")
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"tensors on {t.device} and on {device} in one call")
-    if device.index != _get_device():
-        raise ValueError(f"the tensors are on {device}, which is not the current device")
+# A step makes these calls many times, and a small tree's kernels take a few microseconds: what the host does for a call
+# counts as much.  So a tensor is looked at once (:func:`_at`), what follows from sizes alone is remembered by the sizes, and
+# arguments travel as one packed block (28 arguments one by one take ctypes 3.8 us, packed 0.8).
 
 
-def _check_mask(tree_mask: torch.Tensor, rows: int) -> int:
+def _at(t: torch.Tensor, name: str, dtype: torch.dtype, device: int) -> int:
+    """The address of a contiguous tensor of ``dtype`` on the current device, which ``device`` is."""
+    if t.dtype is dtype and t.get_device() == device and t.is_contiguous():
+        return t.data_ptr()
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.is_cuda and t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, and the current device is cuda:{device}")
+    return _dev(t, name)
+
+
+def _current() -> tuple[int, int]:
+    """The current device and its current stream."""
+    if _raw_stream is not None and torch.cuda.is_initialized():
+        device = _get_device()
+        return device, _raw_stream(device)
+    if not torch.cuda.is_available():
+        raise KernelError("there is no CUDA device: the kernels run on one only and have no CPU path")
+    return torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream
+
+
+def _mask_words(tree_mask: torch.Tensor, rows: int) -> int:
     """Words of a node's mask."""
-    if tree_mask.dtype != torch.int64 or tree_mask.dim() != 2 or tree_mask.shape[0] != rows or tree_mask.shape[1] < 1:
-        raise ValueError(f"tree_mask must be int64 [{rows}, words], got {tree_mask.dtype} {tuple(tree_mask.shape)}")
-    return tree_mask.shape[1]
+    shape = tree_mask.shape
+    if len(shape) != 2 or shape[0] != rows or shape[1] < 1:
+        raise ValueError(f"tree_mask must be int64 [{rows}, words], got {tuple(shape)}")
+    return shape[1]
 
 
 #: keys and rows that a CTA of the tree attention kernel with 32-bit products works on at a time
@@ -3535,10 +3552,59 @@ def tree_takes_tcgen05(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     )
 
 
-def _tree_ctas(requests: int, units: int, tiles: int, device_ctas: int, min_chunk: int) -> int:
-    """CTAs of a tree attention launch: what the device holds at once, or fewer where the requests' most key tiles, at
-    least ``min_chunk`` to a CTA, do not need as many."""
-    return max(1, min(device_ctas, -(-requests * units * tiles // min_chunk)))
+#: key tiles that a worker of a tree attention launch takes at least
+TREE_MIN_TILES = 2
+
+_tree_room: dict[tuple[int, int], int] = {}
+
+
+def tree_cluster_room(cluster: int) -> int:
+    """How many clusters of ``cluster`` CTAs of the tensor-core tree attention kernel the device holds at once."""
+    key = (torch.cuda.current_device(), cluster)
+    if key not in _tree_room:
+        _tree_room[key] = int(_fn("einf_tree_attention_tcgen05_max_clusters", [c_int])(cluster))
+    return _tree_room[key]
+
+
+def _tree_workers(units: int, tiles: int, sms: int, room) -> tuple[int, int, bool]:
+    """Workers, CTAs of a worker, and whether every unit has a worker of its own, for that many units of up to so many key tiles
+    each: what takes the least time, by a tile's and a launch's (see the table in attention_tree_tcgen05.cu)."""
+    best = None
+    for cluster in (1, 2, 4, 8):
+        workers = min(room(cluster), sms // cluster)
+        if workers < 1:
+            continue
+        if units <= workers:
+            cost = TREE_TILE_US * -(-tiles // cluster) + (TREE_CLUSTER_US if cluster > 1 else 0.0)
+            if best is None or cost < best[0]:
+                best = (cost, units, cluster, True)
+        if cluster in (1, 8) and (units > workers or tiles > TREE_MIN_TILES):
+            each = -(-units * tiles // workers) if units > workers else -(-tiles // (workers // units))
+            cost = TREE_TILE_US * -(-each // cluster) + (TREE_CLUSTER_US if cluster > 1 else 0.0) + TREE_MERGE_US
+            if best is None or cost < best[0]:
+                best = (cost, min(workers, max(1, units * -(-tiles // TREE_MIN_TILES))), cluster, False)
+    return best[1:]
+
+
+#: microseconds of a key tile, of putting a cluster's shares together, of the second launch
+TREE_TILE_US, TREE_CLUSTER_US, TREE_MERGE_US = 2.2, 2.0, 6.0
+
+
+@functools.lru_cache(maxsize=4096)
+def _tree_plan(tensor_cores: bool, device: int, requests: int, nodes: int, context: int, group: int, kv_heads: int,
+               size: int) -> tuple[str, int, int, bool, int, int]:
+    """The launcher; its workers, the CTAs of each, whether each has whole units; rows of all shares in scratch memory, elements of a row."""
+    if tensor_cores:
+        units = requests * kv_heads * -(-nodes // (2 * (TREE_TILE // group)))
+        workers, cluster, whole = _tree_workers(units, -(-context // TREE_TILE), _sm_count(), tree_cluster_room)
+        return "einf_tree_attention_tcgen05", workers, cluster, whole, 0 if whole else 2 * workers * 2 * TREE_TILE, size
+    unit_heads = min(group, TREE_ROWS)
+    units = requests * kv_heads * -(-group // unit_heads) * -(-nodes // (TREE_ROWS // unit_heads))
+    workers = max(1, min(3 * _sm_count(), units * -(-context // (TREE_KEYS * TREE_MIN_TILES))))
+    return "einf_tree_attention", workers, 1, False, 2 * workers * TREE_ROWS, -(-size // 4) * 4
+
+
+_TREE_CALL = struct.Struct("<13Q15i2f4x")
 
 
 def tree_attention(
@@ -3571,62 +3637,73 @@ def tree_attention(
     far as the caller knows them, only size the launch: any request's nodes are computed whole."""
     tokens, heads, size = q.shape
     num_pages, kv_heads, page_size, cache_size = k_cache.shape
-    requests = cached_lens.shape[0]
+    requests, (table_rows, width) = cached_lens.shape[0], block_table.shape
+    dtype = q.dtype
     if out.shape != q.shape or v_cache.shape != k_cache.shape or cache_size != size:
         raise ValueError(f"q {tuple(q.shape)}, out {tuple(out.shape)} and caches {tuple(k_cache.shape)}, {tuple(v_cache.shape)} do not "
                          "fit together")
-    if not q.dtype == k_cache.dtype == v_cache.dtype == out.dtype:
-        raise TypeError("q, caches and out must have one dtype")
+    code = _code(q)
     if kv_heads < 1 or heads % kv_heads:
         raise UnsupportedSize(f"{heads} query heads are not a multiple of {kv_heads} key/value heads")
     if not 1 <= size <= MAX_HEAD_SIZE:
         raise UnsupportedSize(f"tree attention takes heads of up to {MAX_HEAD_SIZE}, not {size}")
-    if q_start.shape != (requests + 1,) or block_table.dim() != 2 or block_table.shape[0] < requests:
+    if q_start.shape[0] != requests + 1 or table_rows < requests:
         raise ValueError(f"q_start must hold {requests + 1} entries and block_table a row for each of {requests} requests")
-    words = _check_mask(tree_mask, tokens)
-    if window is not None and window < 1:
-        raise ValueError(f"a window holds at least one token, not {window}")
-    if softcap is not None and not softcap > 0:
-        raise ValueError(f"a soft cap is positive, not {softcap}")
+    words = _mask_words(tree_mask, tokens)
     if not scale > 0:
         raise ValueError(f"the scale is positive, not {scale}")
-    if window:
+    if softcap is not None and not softcap > 0:
+        raise ValueError(f"a soft cap is positive, not {softcap}")
+    if window is not None:
+        if window < 1:
+            raise ValueError(f"a window holds at least one token, not {window}")
         if positions is None or positions.shape != (tokens,):
             raise ValueError("a window needs the position of every node")
-    else:
-        positions = None
-    _here(q.device, k_cache, v_cache, block_table, q_start, cached_lens, tree_mask, out, status, positions)
+    device, stream = _current()
+    places = (
+        _at(q, "q", dtype, device), _at(k_cache, "k_cache", dtype, device), _at(v_cache, "v_cache", dtype, device),
+        _at(block_table, "block_table", torch.int32, device), _at(q_start, "q_start", torch.int32, device),
+        _at(cached_lens, "cached_lens", torch.int32, device), _at(tree_mask, "tree_mask", torch.int64, device),
+        _at(positions, "positions", torch.int32, device) if window else 0, _at(out, "out", dtype, device),
+        _at(status, "status", torch.int32, device),
+    )
     if tokens == 0 or requests == 0:
         return
-    group, width = heads // kv_heads, block_table.shape[1]
-    nodes = min(tokens, max(1, int(max_nodes))) if max_nodes is not None else min(tokens, 64 * words)
+    nodes = min(tokens, 64 * words if max_nodes is None else max(1, int(max_nodes)))
     context = width * page_size
     if max_cached is not None:
         context = min(context, max(0, int(max_cached)) + nodes)
     if window:
         context = min(context, window + nodes + page_size)
-    if tree_takes_tcgen05(q, k_cache, v_cache, out):
-        symbol, code, keys, min_chunk, device_ctas = "einf_tree_attention_tcgen05", (), TREE_TILE, 2, _sm_count()
-        unit_nodes = 2 * (TREE_TILE // group)
-        rows, units, padded = unit_nodes * group, kv_heads * -(-nodes // unit_nodes), size
-    else:
-        symbol, code, keys, min_chunk, device_ctas = "einf_tree_attention", (_code(q),), TREE_KEYS, 2, 3 * _sm_count()
-        unit_heads = min(group, TREE_ROWS)
-        rows, units, padded = TREE_ROWS, kv_heads * -(-group // unit_heads) * -(-nodes // (TREE_ROWS // unit_heads)), -(-size // 4) * 4
-    ctas = _tree_ctas(requests, units, -(-context // keys), device_ctas, min_chunk)
-    shares = 2 * ctas * rows
-    scratch = torch.empty(4 * ctas + shares * (padded + 2), dtype=torch.float32, device=q.device)
-    notes = scratch.data_ptr()
-    sums = notes + 16 * ctas
-    fn = _fn(symbol, [c_void_p] * 3 + [c_int] * len(code) + [c_void_p] * 9 + [c_int] * 10 + [c_float] * 2 + [c_int] * 2 + [c_void_p] * 2)
+    symbol, workers, cluster, whole, shares, padded = _tree_plan(
+        tree_takes_tcgen05(q, k_cache, v_cache, out), device, requests, nodes, context, heads // kv_heads, kv_heads, size)
+    notes = sums = 0
+    if shares:
+        scratch = torch.empty(8 * workers + shares * (padded + 2), dtype=torch.float32, device=q.device)
+        notes = scratch.data_ptr()
+        sums = notes + 32 * workers
+    fn = _fn(symbol, [c_char_p, c_void_p])
     _check(
-        fn(_dev(q, "q"), _dev(k_cache, "k_cache"), _dev(v_cache, "v_cache"), *code, _opt(block_table, "block_table", torch.int32),
-           _opt(q_start, "q_start", torch.int32), _opt(cached_lens, "cached_lens", torch.int32), _dev(tree_mask, "tree_mask"),
-           _opt(positions, "positions", torch.int32), _dev(out, "out"), sums, sums + 4 * shares * padded, notes, requests, tokens,
-           heads, kv_heads, size, page_size, num_pages, width, words, int(window or 0), float(scale), float(softcap or 0.0), ctas,
-           min_chunk, _opt(status, "status", torch.int32), _stream()),
+        fn(_TREE_CALL.pack(*places, sums, sums + 4 * shares * padded, notes, requests, tokens, heads, kv_heads, size, page_size,
+                           num_pages, width, words, int(window or 0), code, workers, cluster, whole, TREE_MIN_TILES, scale,
+                           softcap or 0.0), stream),
         "tree_attention",
     )
+
+
+@functools.lru_cache(maxsize=4096)
+def _shape_pieces(rows: int, requests: int, vocab: int) -> tuple[int, int]:
+    """Places of the vocabulary that a CTA of :func:`shape_logits` has, and how many CTAs take a request's rows in turn."""
+    piece = 4096
+    while piece > 1024 and requests * -(-vocab // piece) < 4 * _sm_count():
+        piece //= 2
+    ways = 1
+    while ways < -(-rows // requests) and ways * requests * -(-vocab // piece) < 4 * _sm_count():
+        ways *= 2
+    return piece, ways
+
+
+_SHAPE_CALL = struct.Struct("<16Q10i")
 
 
 def shape_logits(
@@ -3662,8 +3739,8 @@ def shape_logits(
     ``v // 32`` set for tokens that may come; row ``i`` has mask ``i``, or mask ``allowed_rows[i]`` (int32, negative: none).
     A token outside the vocabulary and a mask that is not there set the status word and count for nothing."""
     rows, vocab = logits.shape
-    if logits.dtype != torch.float32 or out.dtype != torch.float32 or out.shape != logits.shape:
-        raise TypeError("shape_logits takes float32 logits and a result like them")
+    if out.shape != logits.shape:
+        raise ValueError(f"logits {tuple(logits.shape)}, out {tuple(out.shape)}")
     requests = rows if row_start is None else row_start.shape[0] - 1
     if requests < 0:
         raise ValueError("row_start must hold one more entry than there are requests")
@@ -3673,10 +3750,6 @@ def shape_logits(
         raise ValueError("the nodes' tokens come with their mask")
     if (bias_ids is None) != (bias is None):
         raise ValueError("bias_ids come with bias")
-    for t, name in ((history_lens, "history_lens"), (prompt_lens, "prompt_lens"), (repetition, "repetition"), (presence, "presence"),
-                    (frequency, "frequency")):
-        if t is not None and t.shape != (requests,):
-            raise ValueError(f"{name} is {tuple(t.shape)}, expected ({requests},)")
     capacity = words = biases = masks = mask_words = 0
     if history is not None:
         if history.dim() != 2 or history.shape[0] != requests:
@@ -3685,7 +3758,7 @@ def shape_logits(
     if node_tokens is not None:
         if node_tokens.shape != (rows,):
             raise ValueError(f"node_tokens is {tuple(node_tokens.shape)}, expected ({rows},)")
-        words = _check_mask(tree_mask, rows)
+        words = _mask_words(tree_mask, rows)
     if bias is not None:
         if bias.dim() != 2 or bias.shape[0] != requests or bias_ids.shape != bias.shape:
             raise ValueError(f"bias_ids {tuple(bias_ids.shape)} and bias {tuple(bias.shape)} must be [{requests}, n]")
@@ -3698,35 +3771,40 @@ def shape_logits(
             raise ValueError("allowed has a mask per row, or allowed_rows says which mask a row has")
     elif allowed_rows is not None:
         raise ValueError("allowed_rows needs allowed")
-    _here(logits.device, out, row_start, status, history, history_lens, prompt_lens, repetition, presence, frequency, node_tokens,
-          tree_mask, bias_ids, bias, allowed, allowed_rows)
+    device, stream = _current()
+    for t, name in ((history_lens, "history_lens"), (prompt_lens, "prompt_lens"), (repetition, "repetition"), (presence, "presence"),
+                    (frequency, "frequency")):
+        if t is not None and t.shape[0] != requests:
+            raise ValueError(f"{name} is {tuple(t.shape)}, expected ({requests},)")
+    i32, f32 = torch.int32, torch.float32
+    places = (
+        _at(logits, "logits", f32, device), _at(out, "out", f32, device), _at(status, "status", i32, device),
+        0 if history_lens is None else _at(history_lens, "history_lens", i32, device),
+        0 if prompt_lens is None else _at(prompt_lens, "prompt_lens", i32, device),
+        0 if repetition is None else _at(repetition, "repetition", f32, device),
+        0 if presence is None else _at(presence, "presence", f32, device),
+        0 if frequency is None else _at(frequency, "frequency", f32, device),
+        0 if row_start is None else _at(row_start, "row_start", i32, device),
+        0 if history is None else _at(history, "history", i32, device),
+        0 if node_tokens is None else _at(node_tokens, "node_tokens", i32, device),
+        0 if tree_mask is None else _at(tree_mask, "tree_mask", torch.int64, device),
+        0 if bias_ids is None else _at(bias_ids, "bias_ids", i32, device), 0 if bias is None else _at(bias, "bias", f32, device),
+        0 if allowed is None else _at(allowed, "allowed", i32, device),
+        0 if allowed_rows is None else _at(allowed_rows, "allowed_rows", i32, device),
+    )
     if rows == 0 or requests == 0 or vocab == 0:
         return
     if requests > 65535:
         raise UnsupportedSize(f"shape_logits takes up to 65535 requests, not {requests}")
-    piece, row_ways = _shape_pieces(rows, requests, vocab)
-    fn = _fn("einf_shape_logits", [c_void_p] * 15 + [c_int] * 10 + [c_void_p] * 2)
+    fn = _fn("einf_shape_logits", [c_char_p, c_void_p])
     _check(
-        fn(_dev(logits, "logits"), _dev(out, "out"), _opt(row_start, "row_start", torch.int32), _opt(history, "history", torch.int32),
-           _opt(history_lens, "history_lens", torch.int32), _opt(prompt_lens, "prompt_lens", torch.int32),
-           _opt(repetition, "repetition", torch.float32), _opt(presence, "presence", torch.float32),
-           _opt(frequency, "frequency", torch.float32), _opt(node_tokens, "node_tokens", torch.int32),
-           _opt(tree_mask, "tree_mask", torch.int64), _opt(bias_ids, "bias_ids", torch.int32), _opt(bias, "bias", torch.float32),
-           _opt(allowed, "allowed", torch.int32), _opt(allowed_rows, "allowed_rows", torch.int32), rows, vocab, requests, capacity,
-           words, biases, masks, mask_words, piece, row_ways, _opt(status, "status", torch.int32), _stream()),
+        fn(_SHAPE_CALL.pack(*places, rows, vocab, requests, capacity, words, biases, masks, mask_words, *_shape_pieces(rows, requests, vocab)),
+           stream),
         "shape_logits",
     )
 
 
-def _shape_pieces(rows: int, requests: int, vocab: int) -> tuple[int, int]:
-    """Places of the vocabulary that a CTA of :func:`shape_logits` has, and how many CTAs take a request's rows in turn."""
-    piece = 4096
-    while piece > 1024 and requests * -(-vocab // piece) < 4 * _sm_count():
-        piece //= 2
-    ways = 1
-    while ways < -(-rows // requests) and ways * requests * -(-vocab // piece) < 4 * _sm_count():
-        ways *= 2
-    return piece, ways
+_ACCEPT_CALL = struct.Struct("<7Q3i4x")
 
 
 def accept_drafts(node_tokens: torch.Tensor, targets: torch.Tensor, parents: torch.Tensor, q_start: torch.Tensor,
@@ -3738,23 +3816,22 @@ def accept_drafts(node_tokens: torch.Tensor, targets: torch.Tensor, parents: tor
     taken.  ``path[r, i]`` becomes the path's nodes and ``answer[r, i]`` the targets behind them (the tokens of this step: the
     last is the next root), -1 behind the last, ``counts[r]`` how many there are; a path ends where its row
     (``[requests, depth]``) is full."""
-    rows, requests = node_tokens.shape[0], counts.shape[0]
-    if targets.shape != node_tokens.shape or parents.shape != node_tokens.shape or node_tokens.dim() != 1:
+    (rows,), (requests,), (path_rows, depth) = node_tokens.shape, counts.shape, path.shape
+    if targets.shape != node_tokens.shape or parents.shape != node_tokens.shape:
         raise ValueError("node_tokens, targets and parents must be [rows]")
-    if q_start.shape != (requests + 1,):
+    if q_start.shape[0] != requests + 1:
         raise ValueError(f"q_start must hold {requests + 1} entries")
-    if path.dim() != 2 or path.shape[0] != requests or path.shape[1] < 1 or answer.shape != path.shape:
+    if path_rows != requests or depth < 1 or answer.shape != path.shape:
         raise ValueError(f"path {tuple(path.shape)} and answer {tuple(answer.shape)} must be [{requests}, depth]")
-    _here(node_tokens.device, targets, parents, q_start, path, answer, counts)
+    device, stream = _current()
+    call = _ACCEPT_CALL.pack(
+        _at(node_tokens, "node_tokens", torch.int32, device), _at(targets, "targets", torch.int32, device),
+        _at(parents, "parents", torch.int32, device), _at(q_start, "q_start", torch.int32, device),
+        _at(path, "path", torch.int32, device), _at(answer, "answer", torch.int32, device), _at(counts, "counts", torch.int32, device),
+        rows, requests, depth)
     if requests == 0:
         return
-    fn = _fn("einf_accept_drafts", [c_void_p] * 7 + [c_int] * 3 + [c_void_p])
-    _check(
-        fn(_opt(node_tokens, "node_tokens", torch.int32), _opt(targets, "targets", torch.int32), _opt(parents, "parents", torch.int32),
-           _opt(q_start, "q_start", torch.int32), _opt(path, "path", torch.int32), _opt(answer, "answer", torch.int32),
-           _opt(counts, "counts", torch.int32), rows, requests, path.shape[1], _stream()),
-        "accept_drafts",
-    )
+    _check(_fn("einf_accept_drafts", [c_char_p, c_void_p])(call, stream), "accept_drafts")
 
 
 class CacheRows:
@@ -3768,27 +3845,30 @@ class CacheRows:
         if not self.caches:
             raise ValueError("CacheRows needs at least one cache tensor")
         first = self.caches[0]
-        self.device, self.num_pages, self.page_size = first.device, first.shape[0], first.shape[2]
+        self.device, self.num_pages, self.page_size = first.get_device(), first.shape[0], first.shape[2]
         unit = 16
         for t in self.caches:
             if t.dim() != 4 or (t.shape[0], t.shape[2]) != (self.num_pages, self.page_size):
                 raise ValueError(f"caches must be [{self.num_pages}, kv_heads, {self.page_size}, size], got {tuple(t.shape)}")
-            if t.device != self.device:
-                raise ValueError(f"cache tensors on {t.device} and on {self.device}")
+            if t.get_device() != self.device:
+                raise ValueError(f"cache tensors on {first.device} and on {t.device}")
             if t.numel() == 0:
                 raise ValueError("a cache tensor is empty")
             _code(t)
             while _dev(t, "cache") % unit or t.shape[3] * t.element_size() % unit:
                 unit //= 2
         self.unit = unit
-        self._parts = []
+        #: per launch: how many tensors, the unit, what the pages are, and each tensor's address, heads and units of a row
+        self.parts = []
         for start in range(0, len(self.caches), self.MAX_TENSORS):
             part = self.caches[start:start + self.MAX_TENSORS]
-            n = len(part)
-            self._parts.append((
-                (c_void_p * n)(*(t.data_ptr() for t in part)), (c_int * n)(*(t.shape[1] for t in part)),
-                (c_int * n)(*(t.shape[3] * t.element_size() // unit for t in part)), n,
-            ))
+            words = [len(part), unit, self.page_size, self.num_pages]
+            for t in part:
+                words += [t.data_ptr(), t.shape[1], t.shape[3] * t.element_size() // unit]
+            self.parts.append((c_longlong * len(words))(*words))
+
+
+_MOVE_CALL = struct.Struct("<5Q4i")
 
 
 def move_accepted(caches: CacheRows, block_table: torch.Tensor, cached_lens: torch.Tensor, path: torch.Tensor, counts: torch.Tensor,
@@ -3797,23 +3877,23 @@ def move_accepted(caches: CacheRows, block_table: torch.Tensor, cached_lens: tor
     ``cached_lens[r] + path[r, i]`` of request ``r`` goes to place ``cached_lens[r] + i``, for ``i = 1 .. counts[r] - 1`` (all
     int32, as :func:`accept_drafts` writes them), as if every row were read before any is written.  A path's nodes rise; one
     that does not, or a place without a page, sets the status word and is not moved."""
-    requests = cached_lens.shape[0]
-    if path.dim() != 2 or path.shape[0] != requests or counts.shape != (requests,):
+    (requests,), (path_rows, depth), (table_rows, width) = cached_lens.shape, path.shape, block_table.shape
+    if path_rows != requests or counts.shape != cached_lens.shape:
         raise ValueError(f"path must be [{requests}, depth] and counts ({requests},)")
-    if block_table.dim() != 2 or block_table.shape[0] < requests:
+    if table_rows < requests:
         raise ValueError(f"block_table needs a row for each of {requests} requests")
-    _here(caches.device, block_table, cached_lens, path, counts, status)
-    if requests == 0 or path.shape[1] < 2:
+    device, stream = _current()
+    if caches.device != device:
+        raise ValueError(f"the caches are on cuda:{caches.device}, and the current device is cuda:{device}")
+    call = _MOVE_CALL.pack(
+        _at(block_table, "block_table", torch.int32, device), _at(cached_lens, "cached_lens", torch.int32, device),
+        _at(path, "path", torch.int32, device), _at(counts, "counts", torch.int32, device), _at(status, "status", torch.int32, device),
+        requests, depth, width, 0)
+    if requests == 0 or depth < 2:
         return
-    fn = _fn("einf_move_accepted", [c_void_p] * 3 + [c_int] * 2 + [c_void_p] * 4 + [c_int] * 5 + [c_void_p] * 2)
-    table, lens = _opt(block_table, "block_table", torch.int32), _opt(cached_lens, "cached_lens", torch.int32)
-    steps, kept, word = _opt(path, "path", torch.int32), _opt(counts, "counts", torch.int32), _opt(status, "status", torch.int32)
-    for bases, heads, units, count in caches._parts:
-        _check(
-            fn(bases, heads, units, count, caches.unit, table, lens, steps, kept, requests, path.shape[1], caches.page_size,
-               caches.num_pages, block_table.shape[1], word, _stream()),
-            "move_accepted",
-        )
+    fn = _fn("einf_move_accepted", [c_void_p, c_char_p, c_void_p])
+    for part in caches.parts:
+        _check(fn(part, call, stream), "move_accepted")
 
 
 __all__ = [

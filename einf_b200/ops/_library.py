@@ -80,6 +80,7 @@ LAUNCHERS = {
     "einf_report": "sampling",
     "einf_tree_attention": "attention_tree",
     "einf_tree_attention_tcgen05": "attention_tree_tcgen05",
+    "einf_tree_attention_tcgen05_max_clusters": "attention_tree_tcgen05",
     "einf_shape_logits": "logits",
     "einf_accept_drafts": "drafts",
     "einf_move_accepted": "drafts",

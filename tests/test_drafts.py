@@ -17,20 +17,14 @@ def on_this_machine(monkeypatch):
             return 0
         return launch
 
-    def pointer(t, name="", dtype=None):
-        if t is None:
-            return 0
-        if dtype is not None and t.dtype != dtype:
-            raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    def pointer(t, name):
         if not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous")
         return t.data_ptr()
 
     monkeypatch.setattr(ops, "_fn", fn)
     monkeypatch.setattr(ops, "_dev", pointer)
-    monkeypatch.setattr(ops, "_opt", pointer)
-    monkeypatch.setattr(ops, "_here", lambda device, *tensors: None)
-    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(ops, "_current", lambda: (-1, 0))
     monkeypatch.setattr(ops, "_sm_count", lambda: 148)
     return calls
 
@@ -59,7 +53,7 @@ def attention_arguments(**change):
      ops.UnsupportedSize),
     (dict(q_start=ints(2)), ValueError),
     (dict(block_table=ints(1, 3)), ValueError),
-    (dict(tree_mask=ints(5, 1)), ValueError),
+    (dict(tree_mask=ints(5, 1)), TypeError),
     (dict(tree_mask=torch.zeros(4, 1, dtype=torch.int64)), ValueError),
     (dict(tree_mask=torch.zeros(5, 0, dtype=torch.int64)), ValueError),
     (dict(window=0), ValueError),
@@ -98,7 +92,7 @@ def logits_arguments(**change):
 
 @pytest.mark.parametrize("change, error", [
     (dict(logits=torch.zeros(6, 50, dtype=torch.bfloat16)), TypeError),
-    (dict(out=torch.zeros(6, 51)), TypeError),
+    (dict(out=torch.zeros(6, 51)), ValueError),
     (dict(row_start=ints(0)), ValueError),
     (dict(history=None), ValueError),
     (dict(history=None, history_lens=None), ValueError),
