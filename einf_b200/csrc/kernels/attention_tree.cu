@@ -19,6 +19,19 @@ constexpr int kWarps = 4;
 constexpr int kRowsPerWarp = 8;
 constexpr int kRows = kWarps * kRowsPerWarp;
 
+__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
+  const uint2 v = *reinterpret_cast<const uint2*>(p);
+  return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+}
+// Four elements of a row from d on; zeros behind its end.
+template <typename T>
+__device__ __forceinline__ float4 elements(const T* row, int d, int size, bool aligned) {
+  if (aligned) return load4(row + d);
+  return make_float4(d < size ? to_float(row[d]) : 0.f, d + 1 < size ? to_float(row[d + 1]) : 0.f, d + 2 < size ? to_float(row[d + 2]) : 0.f,
+                     d + 3 < size ? to_float(row[d + 3]) : 0.f);
+}
+
 // VEC: elements of the head that a lane has (2, 4 or 8: heads of up to 64, 128, 256)
 template <typename T, int VEC>
 __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams p) {
@@ -28,12 +41,14 @@ __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams 
   float* vs = ks + kKeys * pitch;                   // [keys][32 * VEC]
   float* qs = vs + kKeys * 32 * VEC;                // [rows][size4]
   float* ps = qs + kRows * size4;                   // [rows][keys]
+  __shared__ long long places[kKeys];               // where a key's row starts in the caches, or -1
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_launch_dependents();
   pdl_wait();
   const T* q = static_cast<const T*>(p.q);
   const T* k_cache = static_cast<const T*>(p.k_cache);
   const T* v_cache = static_cast<const T*>(p.v_cache);
+  const bool aligned = p.size % 4 == 0 && (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) == 0;
   TreeWalk w;
   bool any = tree_first(p, blockIdx.x, &w);
   if (threadIdx.x == 0) tree_note(p, blockIdx.x, w, any);
@@ -42,13 +57,17 @@ __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams 
     const TreeUnit u = tree_unit(p, w.t, w.unit);
     const int rows = u.nodes * u.heads;
     __syncthreads();
-    for (int e = threadIdx.x; e < kRows * size4; e += 32 * kWarps) {
-      const int row = e / size4, d = e - row * size4;
-      float v = 0.f;
-      if (row < rows && d < p.size)
-        v = to_float(q[((size_t)(w.t.first + u.first_node + row / u.heads) * p.heads + u.first_head + row % u.heads) * p.size + d]);
-      qs[e] = v;
+    const int pieces = size4 >> 2;                  // of a row, four elements each
+    for (int e = threadIdx.x; e < kRows * pieces; e += 32 * kWarps) {
+      const int row = divide(e, pieces), d = 4 * (e - row * pieces), node = divide(row, u.heads);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row < rows)
+        v = elements(q + ((size_t)(w.t.first + u.first_node + node) * p.heads + u.first_head + row - node * u.heads) * p.size, d, p.size, aligned);
+      *reinterpret_cast<float4*>(qs + row * size4 + d) = v;
     }
+    // elements beyond the head are zeros, once
+    for (int e = threadIdx.x; e < kKeys * 32 * VEC; e += 32 * kWarps)
+      if (e % (32 * VEC) >= size4) vs[e] = 0.f;
     float m[kRowsPerWarp], l[kRowsPerWarp], acc[kRowsPerWarp][VEC];
 #pragma unroll
     for (int i = 0; i < kRowsPerWarp; ++i) {
@@ -62,24 +81,41 @@ __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams 
     for (int tile = w.tile_begin; tile < w.tile_end; ++tile) {
       const int key0 = w.t.begin + tile * kKeys;
       __syncthreads();
-      // four threads a key; a key beyond the end is zeros
-      {
-        const int key = key0 + (threadIdx.x >> 2), part = threadIdx.x & 3;
-        size_t at = 0;
-        bool live = key < keys_end;
-        if (live) {
+      if (threadIdx.x < kKeys) {
+        const int key = key0 + threadIdx.x;
+        long long at = -1;
+        if (key < keys_end) {
           const int page = table[key / p.page_size];
-          if (page < 0 || page >= p.num_pages) {
-            atomicOr(p.status, kStatusBadPage);
-            live = false;
-          } else {
-            at = (((size_t)page * p.kv_heads + u.kv_head) * p.page_size + key % p.page_size) * p.size;
+          if (page < 0 || page >= p.num_pages) atomicOr(p.status, kStatusBadPage);
+          else at = (((long long)page * p.kv_heads + u.kv_head) * p.page_size + key % p.page_size) * p.size;
+        }
+        places[threadIdx.x] = at;
+      }
+      __syncthreads();
+      // a key beyond the end, or without a page, is zeros
+      constexpr int kAhead = 4;
+#pragma unroll 1
+      for (int e0 = threadIdx.x; e0 < kKeys * pieces; e0 += kAhead * 32 * kWarps) {
+        float4 k4[kAhead], v4[kAhead];
+        int key[kAhead], d[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+          const int e = e0 + a * 32 * kWarps;
+          key[a] = divide(e, pieces);
+          d[a] = 4 * (e - key[a] * pieces);
+          const long long at = key[a] < kKeys ? places[key[a]] : -1;
+          k4[a] = v4[a] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (at >= 0) {
+            k4[a] = elements(k_cache + at, d[a], p.size, aligned);
+            v4[a] = elements(v_cache + at, d[a], p.size, aligned);
           }
         }
-        float* kr = ks + (threadIdx.x >> 2) * pitch;
-        float* vr = vs + (threadIdx.x >> 2) * 32 * VEC;
-        for (int d = part; d < size4; d += 4) kr[d] = live && d < p.size ? to_float(k_cache[at + d]) : 0.f;
-        for (int d = part; d < 32 * VEC; d += 4) vr[d] = live && d < p.size ? to_float(v_cache[at + d]) : 0.f;
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a)
+          if (key[a] < kKeys) {
+            *reinterpret_cast<float4*>(ks + key[a] * pitch + d[a]) = k4[a];
+            *reinterpret_cast<float4*>(vs + key[a] * 32 * VEC + d[a]) = v4[a];
+          }
       }
       __syncthreads();
       const int my_rows = min(kRowsPerWarp, rows - warp * kRowsPerWarp);
@@ -98,19 +134,20 @@ __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams 
           s[i] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[i]))));
         }
       }
+      // lane i finds out what row i sees
+      uint32_t mine = 0xffffffffu;
+      if (lane < my_rows && (key0 + kKeys > w.t.cached || p.window > 0)) {
+        const int token = w.t.first + u.first_node + divide(warp * kRowsPerWarp + lane, u.heads), position = tree_position(p, w.t, token);
+        mine = tree_visible(p, w.t, token, tree_lowest(p, position), position, key0);
+      }
+      __syncwarp();
+      const bool all = __all_sync(0xffffffffu, mine == 0xffffffffu);
       uint32_t seen[kRowsPerWarp];
-      uint32_t all = 0xffffffffu;
 #pragma unroll
       for (int i = 0; i < kRowsPerWarp; ++i) {
         const int row = warp * kRowsPerWarp + i;
-        uint32_t bits = 0u;
-        if (row < rows) {
-          const int token = w.t.first + u.first_node + row / u.heads;
-          const int position = tree_position(p, w.t, token);
-          bits = tree_visible(p, w.t, token, tree_lowest(p, position), position, key0);
-        }
+        const uint32_t bits = row < rows ? __shfl_sync(0xffffffffu, mine, i) : 0u;
         seen[i] = bits;
-        all &= row < rows ? bits : 0xffffffffu;
         float x = p.softcap > 0.f ? cap_log2 * tanhf(s[i] * p.scale / p.softcap) : s[i] * scale_log2;
         if (!(bits >> lane & 1u)) x = -INFINITY;
         const float top = fmaxf(m[i], warp_max(x));
@@ -137,7 +174,7 @@ __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams 
           }
         }
       };
-      if (all == 0xffffffffu) {
+      if (all) {
 #pragma unroll 1
         for (int j = 0; j < kKeys; j += 4) {
           float4 e4[kRowsPerWarp];

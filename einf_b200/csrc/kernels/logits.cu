@@ -6,18 +6,25 @@
 //
 // A pass has to read and write the rows and to read their masks: it is bound by memory.  No table of counts over the
 // vocabulary is kept between calls; a CTA has a piece of the vocabulary, counts the request's tokens that fall into it in
-// shared memory (the history is read once per piece, from the L2) and then walks the request's rows.  The nodes of a
-// request share these counts.  A row's path is a few tokens: their places are left out of the walk and done one by
-// one at the end, so that a row may be shaped in place.
-#include "common.cuh"
+// shared memory (the history is read once per piece, from the L2) and then walks the request's rows, a part of 2,048 places at
+// a time.  Where rows start on 16 bytes the parts come to shared memory by bulk copies, four ahead, so that what is in flight
+// depends neither on registers nor on how long a thread is at a part; other rows are read a float at a time, a part ahead.
+// The nodes of a request share the counts.  A row's path is a few tokens: their places are left out of the walk and done
+// one by one at the end, so that a row may be shaped in place.
+#include "tcgen05.cuh"
 
 namespace einf {
 
 constexpr int kShapeThreads = 256;
-constexpr int kMostPlaces = 16384;            // of a CTA's piece of the vocabulary
-constexpr uint32_t kInPrompt = 1u << 31;      // a place's word: in the prompt, some node's token, how often answered
+constexpr int kPart = 8 * kShapeThreads;      // places that a CTA has at a time
+constexpr int kMostParts = 4;                 // of its piece of the vocabulary
+constexpr int kStages = 4;                    // parts on their way or in work
+constexpr uint32_t kInPrompt = 1u << 31;      // a place's word: in the prompt, some node's token, a token with a bias, how often answered
 constexpr uint32_t kDrafted = 1u << 30;
-constexpr uint32_t kCount = kDrafted - 1;
+constexpr uint32_t kBiased = 1u << 29;
+constexpr uint32_t kCount = kBiased - 1;
+constexpr int kMostWords = 64;                // of a node's mask: 4,096 nodes
+static_assert(64 * kMostWords * 8 <= kStages * kPart * 4, "the hits take the place of the parts");
 
 // A call's arguments, as the caller packs them.
 struct ShapeParams {
@@ -38,20 +45,21 @@ struct ShapeParams {
   const uint32_t* allowed;     // [masks, mask_words] or null
   const int* allowed_rows;     // [rows] or null: row r has mask r
   int rows, vocab, requests, capacity, words, biases, masks, mask_words;
-  int piece;                   // places of the vocabulary that a CTA has, a multiple of 32
+  int parts;                   // parts of the vocabulary that a CTA has: 1, 2 or 4
   int row_ways;                // CTAs that take a request's rows in turn
 };
 static_assert(sizeof(ShapeParams) == 16 * 8 + 10 * 4, "as packed");
 
 struct ShapeRequest {
-  float repetition, presence, frequency;
+  float repetition, inverse, presence, frequency;
 };
 
+// Without branches: where one place in a warp's 128 has been seen, they all come here.
 __device__ __forceinline__ float shaped(float x, uint32_t word, int on_path, const ShapeRequest& s) {
   const int count = (int)(word & kCount) + on_path;
-  if ((word & kInPrompt) || count > 0) x = x > 0.f ? x / s.repetition : x * s.repetition;
-  if (count > 0) x -= fmaf(s.frequency, (float)count, s.presence);
-  return x;
+  const float factor = x > 0.f ? s.inverse : s.repetition;
+  const float off = count > 0 ? fmaf(s.frequency, (float)count, s.presence) : 0.f;
+  return ((word & kInPrompt) || count > 0 ? x * factor : x) - off;
 }
 
 // Which mask a row has: its words, or null.
@@ -65,145 +73,290 @@ __device__ __forceinline__ const uint32_t* row_mask(const ShapeParams& p, int ro
   return mask < 0 ? nullptr : p.allowed + (size_t)mask * p.mask_words;
 }
 
-// VEC: elements of a row read together (4 where every row starts on 16 bytes); HAS_BIAS: the places' biases lie in
-// shared memory behind their words.
-template <int VEC, bool HAS_BIAS>
-__global__ void __launch_bounds__(kShapeThreads) shape_logits_kernel(ShapeParams p) {
-  extern __shared__ __align__(16) uint32_t words[];
-  pdl_launch_dependents();
-  pdl_wait();
-  const int request = blockIdx.y, v0 = blockIdx.x * p.piece, length = min(p.piece, p.vocab - v0);
-  const int first = p.row_start ? max(0, min(p.row_start[request], p.rows)) : request;
-  const int nodes = p.row_start ? max(0, min(p.row_start[request + 1], p.rows) - first) : 1;
-  if (nodes <= (int)blockIdx.z) return;
-  uint32_t* which = words + p.piece;          // 1 + the place's entry in the list of biases, or 0
-  for (int i = 4 * threadIdx.x; i < (HAS_BIAS ? 2 : 1) * p.piece; i += 4 * kShapeThreads)
+// What a CTA works on: rows first_row, first_row + ways, ... of a request and places v0 .. v0 + length of them.
+struct Walk {
+  int request, first, nodes, first_row, rows, v0, length, piece;
+};
+__device__ __forceinline__ Walk walk_of(const ShapeParams& p) {
+  Walk w;
+  w.piece = p.parts * kPart;
+  w.request = blockIdx.y;
+  w.v0 = blockIdx.x * w.piece;
+  w.length = min(w.piece, p.vocab - w.v0);
+  w.first = p.row_start ? max(0, min(p.row_start[w.request], p.rows)) : w.request;
+  w.nodes = p.row_start ? max(0, min(p.row_start[w.request + 1], p.rows) - w.first) : 1;
+  w.first_row = w.first + (int)blockIdx.z;
+  w.rows = max(0, (w.nodes - (int)blockIdx.z + (int)gridDim.z - 1) / (int)gridDim.z);
+  return w;
+}
+
+constexpr int kTokensAhead = 4;               // times four tokens of the history that a thread asks for at once
+
+// The first tokens of the history: asked for before anything is known of how many there are.
+__device__ __forceinline__ void ask_tokens(const ShapeParams& p, const Walk& w, int i0, int4 (&t)[kTokensAhead]) {
+  const int* history = p.history + (size_t)w.request * p.capacity;
+#pragma unroll
+  for (int a = 0; a < kTokensAhead; ++a) {
+    const int i = i0 + a * 4 * kShapeThreads;
+    if (i + 4 <= p.capacity) t[a] = *reinterpret_cast<const int4*>(history + i);
+  }
+}
+
+// The words of the CTA's places, and behind them (HAS_BIAS) 1 + a place's entry in the list of biases, or 0.
+template <bool HAS_BIAS>
+__device__ __forceinline__ ShapeRequest count_tokens(const ShapeParams& p, const Walk& w, uint32_t* words) {
+  uint32_t* which = words + w.piece;
+  const bool four = p.history && p.capacity % 4 == 0 && ((uintptr_t)p.history & 15) == 0;
+  int4 t[kTokensAhead];
+  if (four) ask_tokens(p, w, 4 * threadIdx.x, t);
+  const int filled = p.history ? max(0, min(p.history_lens[w.request], p.capacity)) : 0, prompt = p.prompt_lens ? p.prompt_lens[w.request] : 0;
+  ShapeRequest s;
+  s.repetition = p.repetition ? p.repetition[w.request] : 1.f;
+  s.presence = p.presence ? p.presence[w.request] : 0.f;
+  s.frequency = p.frequency ? p.frequency[w.request] : 0.f;
+  for (int i = 4 * threadIdx.x; i < (HAS_BIAS ? 2 : 1) * w.piece; i += 4 * kShapeThreads)
     *reinterpret_cast<uint4*>(words + i) = make_uint4(0u, 0u, 0u, 0u);
   __syncthreads();
   bool bad = false;
-  if (p.history) {
-    const int* history = p.history + (size_t)request * p.capacity;
-    const int filled = max(0, min(p.history_lens[request], p.capacity)), prompt = p.prompt_lens ? p.prompt_lens[request] : 0;
-    auto count = [&](int i, int token) {
-      if ((unsigned)token >= (unsigned)p.vocab) {
-        bad = true;
-      } else if ((unsigned)(token - v0) < (unsigned)length) {
-        if (i < prompt) atomicOr(words + token - v0, kInPrompt);
-        else atomicAdd(words + token - v0, 1u);
-      }
-    };
-    int done = 0;
-    if (((uintptr_t)history & 15) == 0) {
-      done = filled & ~3;
-      for (int i = 4 * threadIdx.x; i < done; i += 4 * kShapeThreads) {
-        const int4 t = *reinterpret_cast<const int4*>(history + i);
-        count(i, t.x);
-        count(i + 1, t.y);
-        count(i + 2, t.z);
-        count(i + 3, t.w);
-      }
+  auto count = [&](int i, int token) {
+    if (i >= filled) return;
+    if ((unsigned)(token - w.v0) < (unsigned)w.length) {
+      if (i < prompt) atomicOr(words + token - w.v0, kInPrompt);
+      else atomicAdd(words + token - w.v0, 1u);
+    } else if ((unsigned)token >= (unsigned)p.vocab) {
+      bad = true;
     }
-    for (int i = done + threadIdx.x; i < filled; i += kShapeThreads) count(i, history[i]);
+  };
+  if (four) {
+#pragma unroll 1
+    for (int i0 = 4 * threadIdx.x; i0 < filled;) {
+#pragma unroll
+      for (int a = 0; a < kTokensAhead; ++a) {
+        const int i = i0 + a * 4 * kShapeThreads;
+        if (i >= filled) break;
+        count(i, t[a].x);
+        count(i + 1, t[a].y);
+        count(i + 2, t[a].z);
+        count(i + 3, t[a].w);
+      }
+      i0 += kTokensAhead * 4 * kShapeThreads;
+      if (i0 < filled) ask_tokens(p, w, i0, t);
+    }
+  } else {
+    for (int i = threadIdx.x; i < filled; i += kShapeThreads) count(i, p.history[(size_t)w.request * p.capacity + i]);
   }
   if (p.node_tokens)
-    for (int k = threadIdx.x; k < nodes; k += kShapeThreads) {
-      const int token = p.node_tokens[first + k];
+    for (int k = threadIdx.x; k < min(w.nodes, 64 * p.words); k += kShapeThreads) {
+      const int token = p.node_tokens[w.first + k];
       if ((unsigned)token >= (unsigned)p.vocab) bad = true;
-      else if ((unsigned)(token - v0) < (unsigned)length) atomicOr(words + token - v0, kDrafted);
+      else if ((unsigned)(token - w.v0) < (unsigned)w.length) atomicOr(words + token - w.v0, kDrafted);
     }
   if (HAS_BIAS)
     for (int j = threadIdx.x; j < p.biases; j += kShapeThreads) {
-      const int token = p.bias_ids[(size_t)request * p.biases + j];
+      const int token = p.bias_ids[(size_t)w.request * p.biases + j];
       if (token >= p.vocab) bad = true;
-      else if (token >= 0 && (unsigned)(token - v0) < (unsigned)length) atomicMax(which + token - v0, j + 1u);
+      else if (token >= 0 && (unsigned)(token - w.v0) < (unsigned)w.length) {
+        atomicMax(which + token - w.v0, j + 1u);
+        atomicOr(words + token - w.v0, kBiased);
+      }
     }
   if (bad && blockIdx.x == 0) atomicOr(p.status, kStatusBadToken);
-  ShapeRequest s;
-  s.repetition = p.repetition ? p.repetition[request] : 1.f;
-  s.presence = p.presence ? p.presence[request] : 0.f;
-  s.frequency = p.frequency ? p.frequency[request] : 0.f;
-  const float* biases = p.bias + (size_t)request * p.biases;
+  s.inverse = 1.f / s.repetition;
   __syncthreads();
+  return s;
+}
 
-  constexpr int kAhead = 4;
-  for (int node = blockIdx.z; node < nodes; node += gridDim.z) {
-    const int row = first + node;
-    const float* in = p.logits + (size_t)row * p.vocab + v0;
-    float* out = p.out + (size_t)row * p.vocab + v0;
-    const uint32_t* mask = row_mask(p, row);
-    for (int i0 = VEC * threadIdx.x; i0 < length; i0 += kAhead * VEC * kShapeThreads) {
-      float x[kAhead][VEC];
-      uint32_t bits[kAhead];
-#pragma unroll
-      for (int a = 0; a < kAhead; ++a) {
-        const int i = i0 + a * VEC * kShapeThreads;
-        bits[a] = 0xffffffffu;
-        if (i < length) {
-          if (VEC == 4) {
-            const float4 v = *reinterpret_cast<const float4*>(in + i);
-            x[a][0] = v.x, x[a][1] = v.y, x[a][2] = v.z, x[a][3] = v.w;
-          } else {
-            x[a][0] = in[i];
-          }
-          if (mask) bits[a] = mask[(v0 + i) >> 5] >> ((v0 + i) & 31);
-        }
-      }
-#pragma unroll
-      for (int a = 0; a < kAhead; ++a) {
-        const int i = i0 + a * VEC * kShapeThreads;
-        if (i >= length) break;
-        uint32_t word[VEC], entry[VEC];
-        if (VEC == 4) {
-          *reinterpret_cast<uint4*>(word) = *reinterpret_cast<const uint4*>(words + i);
-          if (HAS_BIAS) *reinterpret_cast<uint4*>(entry) = *reinterpret_cast<const uint4*>(which + i);
-        } else {
-          word[0] = words[i];
-          if (HAS_BIAS) entry[0] = which[i];
-        }
-        uint32_t drafted = 0u;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          drafted |= word[e] & kDrafted;
-          if (word[e]) x[a][e] = shaped(x[a][e], word[e], 0, s);
-          if (HAS_BIAS && entry[e]) x[a][e] += biases[entry[e] - 1];
-          if (!(bits[a] >> e & 1u)) x[a][e] = -INFINITY;
-        }
-        if (VEC == 4 && !drafted) {
-          *reinterpret_cast<float4*>(out + i) = make_float4(x[a][0], x[a][1 % VEC], x[a][2 % VEC], x[a][3 % VEC]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e)
-            if (!(word[e] & kDrafted)) out[i + e] = x[a][e];
-        }
-      }
-    }
-  }
+// The places of the nodes' tokens.  `hits` takes the nodes whose tokens are the CTA's (room for as many as a mask has bits); then
+// (hit, row) pairs, a token that several nodes have at the first of them: the row's count is the request's and that of the hits with
+// this token on the row's path.
+template <bool HAS_BIAS>
+__device__ __forceinline__ void shape_drafted(const ShapeParams& p, const Walk& w, const ShapeRequest& s, const uint32_t* words, int2* hits) {
+  __shared__ int hit_count;
   if (!p.node_tokens) return;
-  // the places of the nodes' tokens: (node whose token it is, row) pairs, a token that several nodes have at its first
-  const int rows_here = (nodes - (int)blockIdx.z + (int)gridDim.z - 1) / (int)gridDim.z;
-  for (int k = threadIdx.x >> 5; k < nodes; k += kShapeThreads / 32) {
-    const int token = p.node_tokens[first + k];
-    if ((unsigned)(token - v0) >= (unsigned)length || (unsigned)token >= (unsigned)p.vocab) continue;
-    const int lane = threadIdx.x & 31;
-    bool before = false;
-    for (int k0 = 0; k0 < k; k0 += 32)
-      before = before || __any_sync(0xffffffffu, k0 + lane < k && p.node_tokens[first + k0 + lane] == token);
-    if (before) continue;
-    const uint32_t word = words[token - v0];
-    const uint32_t entry = HAS_BIAS ? which[token - v0] : 0u;
-    for (int n = lane; n < rows_here; n += 32) {
-      const int row = first + (int)blockIdx.z + n * (int)gridDim.z;
-      const uint32_t* path = p.tree_mask + (size_t)row * 2 * p.words;
-      int on_path = 0;
-      for (int other = k; other < nodes && other < 64 * p.words; ++other)
-        if ((path[other >> 5] >> (other & 31) & 1u) && p.node_tokens[first + other] == token) ++on_path;
-      float x = shaped(p.logits[(size_t)row * p.vocab + token], word, on_path, s);
-      if (entry) x += biases[entry - 1];
-      const uint32_t* mask = row_mask(p, row);
-      if (mask && !(mask[token >> 5] >> (token & 31) & 1u)) x = -INFINITY;
-      p.out[(size_t)row * p.vocab + token] = x;
-    }
+  const uint32_t* which = words + w.piece;
+  if (threadIdx.x == 0) hit_count = 0;
+  __syncthreads();
+  for (int k = threadIdx.x; k < min(w.nodes, 64 * p.words); k += kShapeThreads) {
+    const int token = p.node_tokens[w.first + k];
+    if ((unsigned)(token - w.v0) < (unsigned)w.length) hits[atomicAdd(&hit_count, 1)] = make_int2(k, token);
   }
+  __syncthreads();
+  const int count = hit_count;
+  for (int item = threadIdx.x; item < count * w.rows; item += kShapeThreads) {
+    const int n = item / count, row = w.first_row + n * (int)gridDim.z;
+    const int2 hit = hits[item - n * count];
+    const uint32_t* path = p.tree_mask + (size_t)row * 2 * p.words;
+    int on_path = 0;
+    bool first = true;
+    for (int other = 0; other < count; ++other) {
+      const int2 h = hits[other];
+      if (h.y != hit.y) continue;
+      first = first && h.x >= hit.x;
+      on_path += path[h.x >> 5] >> (h.x & 31) & 1u;
+    }
+    if (!first) continue;
+    const uint32_t entry = HAS_BIAS ? which[hit.y - w.v0] : 0u;
+    float x = shaped(p.logits[(size_t)row * p.vocab + hit.y], words[hit.y - w.v0], on_path, s);
+    if (entry) x += p.bias[(size_t)w.request * p.biases + entry - 1];
+    const uint32_t* mask = row_mask(p, row);
+    if (mask && !(mask[hit.y >> 5] >> (hit.y & 31) & 1u)) x = -INFINITY;
+    p.out[(size_t)row * p.vocab + hit.y] = x;
+  }
+}
+
+// Rows that start on 16 bytes.
+template <bool HAS_BIAS>
+__global__ void __launch_bounds__(kShapeThreads) shape_logits_bulk_kernel(ShapeParams p) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  float* ring = reinterpret_cast<float*>(smem);                                       // [stages][part]
+  uint32_t* words = reinterpret_cast<uint32_t*>(smem + kStages * kPart * 4);
+  __shared__ __align__(8) unsigned long long bars[kStages];
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) bar_init(saddr(bars + i), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  pdl_wait();
+  const Walk w = walk_of(p);
+  if (w.rows == 0) return;
+  const int part_shift = __ffs(p.parts) - 1, steps = w.rows << part_shift;
+  // parts beyond the end of the vocabulary are steps without work
+  auto places = [&](int step) { return min(kPart, w.length - (step & (p.parts - 1)) * kPart); };
+  auto fetch = [&](int step) {
+    const int n = places(step);
+    if (step >= steps || n <= 0) return;
+    const int stage = step % kStages, row = w.first_row + (step >> part_shift) * (int)gridDim.z;
+    const float* from = p.logits + (size_t)row * p.vocab + w.v0 + (step & (p.parts - 1)) * kPart;
+    bar_expect_tx(saddr(bars + stage), n * 4);
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(saddr(ring + stage * kPart)),
+                 "l"(from), "r"(n * 4), "r"(saddr(bars + stage))
+                 : "memory");
+  };
+  // a thread's two runs of four places, 32 words of the mask apart; asked for a step ahead
+  const int i0 = 4 * threadIdx.x;
+  struct Bits {
+    uint32_t run[2];
+  };
+  auto ask_bits = [&](int step) {
+    Bits b = {{0xffffffffu, 0xffffffffu}};
+    if (!p.allowed || step >= steps) return b;
+    const uint32_t* mask = row_mask(p, w.first_row + (step >> part_shift) * (int)gridDim.z);
+    const int n = places(step), at = w.v0 + (step & (p.parts - 1)) * kPart + i0;
+    if (mask && i0 < n) b.run[0] = mask[at >> 5];
+    if (mask && i0 + 4 * kShapeThreads < n) b.run[1] = mask[(at >> 5) + kShapeThreads / 8];
+    return b;
+  };
+  if (threadIdx.x == 0)
+    for (int step = 0; step < kStages; ++step) fetch(step);      // on their way while the history is counted
+  Bits ahead = ask_bits(0);
+  const ShapeRequest s = count_tokens<HAS_BIAS>(p, w, words);
+  const uint32_t* which = words + w.piece;
+  const float* biases = p.bias + (size_t)w.request * p.biases;
+  const int shift = (w.v0 + i0) & 31;                            // parts start on whole words
+  uint32_t parity = 0u;                                          // a bit a stage
+#pragma unroll 1
+  for (int step = 0; step < steps; ++step) {
+    const int stage = step % kStages, n = places(step), part0 = (step & (p.parts - 1)) * kPart;
+    const Bits bits = ahead;
+    ahead = ask_bits(step + 1);
+    if (n > 0) {
+      float* out = p.out + (size_t)(w.first_row + (step >> part_shift) * (int)gridDim.z) * p.vocab + w.v0 + part0;
+      bar_wait_likely_done(saddr(bars + stage), parity >> stage & 1u, p.status);
+      parity ^= 1u << stage;
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const int i = i0 + a * 4 * kShapeThreads;
+        if (i >= n) break;
+        float4 x = *reinterpret_cast<const float4*>(ring + stage * kPart + i);
+        const uint4 word = *reinterpret_cast<const uint4*>(words + part0 + i);
+        const uint32_t any = word.x | word.y | word.z | word.w;
+        if (any) {
+          x.x = shaped(x.x, word.x, 0, s);
+          x.y = shaped(x.y, word.y, 0, s);
+          x.z = shaped(x.z, word.z, 0, s);
+          x.w = shaped(x.w, word.w, 0, s);
+          if (HAS_BIAS && (any & kBiased)) {
+            const uint4 entry = *reinterpret_cast<const uint4*>(which + part0 + i);
+            if (entry.x) x.x += biases[entry.x - 1];
+            if (entry.y) x.y += biases[entry.y - 1];
+            if (entry.z) x.z += biases[entry.z - 1];
+            if (entry.w) x.w += biases[entry.w - 1];
+          }
+        }
+        const uint32_t b = bits.run[a] >> shift;
+        x.x = b & 1u ? x.x : -INFINITY;
+        x.y = b & 2u ? x.y : -INFINITY;
+        x.z = b & 4u ? x.z : -INFINITY;
+        x.w = b & 8u ? x.w : -INFINITY;
+        if (!(any & kDrafted)) {
+          __stcs(reinterpret_cast<float4*>(out + i), x);
+        } else {
+          if (!(word.x & kDrafted)) out[i] = x.x;
+          if (!(word.y & kDrafted)) out[i + 1] = x.y;
+          if (!(word.z & kDrafted)) out[i + 2] = x.z;
+          if (!(word.w & kDrafted)) out[i + 3] = x.w;
+        }
+      }
+    }
+    __syncthreads();                                             // the stage is read
+    if (threadIdx.x == 0) fetch(step + kStages);
+  }
+  shape_drafted<HAS_BIAS>(p, w, s, words, reinterpret_cast<int2*>(ring));
+}
+
+// Any rows.
+template <bool HAS_BIAS>
+__global__ void __launch_bounds__(kShapeThreads) shape_logits_kernel(ShapeParams p) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  uint32_t* words = reinterpret_cast<uint32_t*>(smem);
+  pdl_launch_dependents();
+  pdl_wait();
+  const Walk w = walk_of(p);
+  if (w.rows == 0) return;
+  const int part_shift = __ffs(p.parts) - 1, steps = w.rows << part_shift;
+  struct Places {
+    float x[8];
+    bool allowed[8];
+  };
+  auto load = [&](int step, Places& t) {
+    const int row = w.first_row + (step >> part_shift) * (int)gridDim.z, i0 = (step & (p.parts - 1)) * kPart + threadIdx.x;
+    const float* in = p.logits + (size_t)row * p.vocab + w.v0;
+    const uint32_t* mask = row_mask(p, row);
+#pragma unroll
+    for (int a = 0; a < 8; ++a) {
+      const int i = i0 + a * kShapeThreads;
+      t.x[a] = i < w.length ? __ldcs(in + i) : 0.f;
+      t.allowed[a] = !mask || i >= w.length || (mask[(w.v0 + i) >> 5] >> ((w.v0 + i) & 31) & 1u);
+    }
+  };
+  Places now, next;
+  load(0, now);                               // on their way while the history is counted
+  const ShapeRequest s = count_tokens<HAS_BIAS>(p, w, words);
+  const uint32_t* which = words + w.piece;
+  const float* biases = p.bias + (size_t)w.request * p.biases;
+  auto shape = [&](int step, Places& t) {
+    const int row = w.first_row + (step >> part_shift) * (int)gridDim.z, i0 = (step & (p.parts - 1)) * kPart + threadIdx.x;
+    float* out = p.out + (size_t)row * p.vocab + w.v0;
+#pragma unroll
+    for (int a = 0; a < 8; ++a) {
+      const int i = i0 + a * kShapeThreads;
+      if (i >= w.length) break;
+      const uint32_t word = words[i];
+      float x = t.x[a];
+      if (word) x = shaped(x, word, 0, s);
+      if (HAS_BIAS && (word & kBiased)) x += biases[which[i] - 1];
+      if (!(word & kDrafted)) __stcs(out + i, t.allowed[a] ? x : -INFINITY);
+    }
+  };
+#pragma unroll 1
+  for (int step = 0; step < steps; step += 2) {
+    if (step + 1 < steps) load(step + 1, next);
+    shape(step, now);
+    if (step + 2 < steps) load(step + 2, now);
+    if (step + 1 < steps) shape(step + 1, next);
+  }
+  __syncthreads();
+  shape_drafted<HAS_BIAS>(p, w, s, words, reinterpret_cast<int2*>(words + (HAS_BIAS ? 2 : 1) * w.piece));
 }
 
 }  // namespace einf
@@ -214,14 +367,15 @@ using namespace einf;
 extern "C" int einf_shape_logits(const char* call, cudaStream_t stream) {
   const ShapeParams& p = *reinterpret_cast<const ShapeParams*>(call);
   if (p.rows == 0 || p.requests == 0) return 0;
-  if (p.vocab < 1 || p.piece < 32 || p.piece % 32 || p.piece > kMostPlaces || p.row_ways < 1 || p.row_ways > 65535 || p.requests > 65535 ||
-      (p.node_tokens && !p.tree_mask) || (p.history && !p.history_lens))
+  if (p.vocab < 1 || p.parts < 1 || p.parts > kMostParts || (p.parts & (p.parts - 1)) || p.row_ways < 1 || p.row_ways > 65535 || p.requests > 65535 ||
+      (p.node_tokens && (!p.tree_mask || p.words < 1 || p.words > kMostWords)) || (p.history && !p.history_lens))
     return (int)cudaErrorInvalidValue;
-  const bool has_bias = p.biases > 0, vec = p.vocab % 4 == 0 && (((uintptr_t)p.logits | (uintptr_t)p.out) & 15) == 0;
-  const auto kernel = vec ? (has_bias ? shape_logits_kernel<4, true> : shape_logits_kernel<4, false>)
-                          : (has_bias ? shape_logits_kernel<1, true> : shape_logits_kernel<1, false>);
-  const size_t smem = (size_t)p.piece * 4 * (has_bias ? 2 : 1);
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kMostPlaces * 4);
+  const bool has_bias = p.biases > 0, bulk = p.vocab % 4 == 0 && (((uintptr_t)p.logits | (uintptr_t)p.out) & 15) == 0;
+  const auto kernel = bulk ? (has_bias ? shape_logits_bulk_kernel<true> : shape_logits_bulk_kernel<false>)
+                           : (has_bias ? shape_logits_kernel<true> : shape_logits_kernel<false>);
+  const int piece = p.parts * kPart;
+  const size_t smem = (size_t)piece * 4 * (has_bias ? 2 : 1) + (bulk ? kStages * kPart * 4 : p.node_tokens ? 64 * p.words * 8 : 0);
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 * kMostParts + kStages) * kPart * 4);
   if (e != cudaSuccess) return (int)e;
-  return (int)launch_pdl(kernel, dim3((p.vocab + p.piece - 1) / p.piece, p.requests, p.row_ways), dim3(kShapeThreads), smem, stream, p);
+  return (int)launch_pdl(kernel, dim3((p.vocab + piece - 1) / piece, p.requests, p.row_ways), dim3(kShapeThreads), smem, stream, p);
 }

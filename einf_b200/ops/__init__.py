@@ -3691,16 +3691,20 @@ def tree_attention(
     )
 
 
+SHAPE_PART = 2048      # places of the vocabulary that a CTA of shape_logits has at a time
+
+
 @functools.lru_cache(maxsize=4096)
-def _shape_pieces(rows: int, requests: int, vocab: int) -> tuple[int, int]:
-    """Places of the vocabulary that a CTA of :func:`shape_logits` has, and how many CTAs take a request's rows in turn."""
-    piece = 4096
-    while piece > 1024 and requests * -(-vocab // piece) < 4 * _sm_count():
-        piece //= 2
-    ways = 1
-    while ways < -(-rows // requests) and ways * requests * -(-vocab // piece) < 4 * _sm_count():
+def _shape_pieces(rows: int, requests: int, vocab: int, capacity: int) -> tuple[int, int]:
+    """Parts of the vocabulary to a CTA of :func:`shape_logits`, and how many CTAs take a request's rows in turn.  A CTA reads
+    its request's whole history: more parts to it where the history is longer than they are, as long as the device
+    is filled; the rows are shared out where it is not."""
+    full, parts, ways = 4 * _sm_count(), 1, 1
+    while parts < 4 and SHAPE_PART * parts * rows <= capacity * requests and requests * -(-vocab // (2 * SHAPE_PART * parts)) >= full:
+        parts *= 2
+    while ways < -(-rows // requests) and ways * requests * -(-vocab // (SHAPE_PART * parts)) < full:
         ways *= 2
-    return piece, ways
+    return parts, ways
 
 
 _SHAPE_CALL = struct.Struct("<16Q10i")
@@ -3759,6 +3763,8 @@ def shape_logits(
         if node_tokens.shape != (rows,):
             raise ValueError(f"node_tokens is {tuple(node_tokens.shape)}, expected ({rows},)")
         words = _mask_words(tree_mask, rows)
+        if words > 64:
+            raise UnsupportedSize(f"shape_logits takes masks of up to 64 words (4096 nodes), not {words}")
     if bias is not None:
         if bias.dim() != 2 or bias.shape[0] != requests or bias_ids.shape != bias.shape:
             raise ValueError(f"bias_ids {tuple(bias_ids.shape)} and bias {tuple(bias.shape)} must be [{requests}, n]")
@@ -3798,7 +3804,7 @@ def shape_logits(
         raise UnsupportedSize(f"shape_logits takes up to 65535 requests, not {requests}")
     fn = _fn("einf_shape_logits", [c_char_p, c_void_p])
     _check(
-        fn(_SHAPE_CALL.pack(*places, rows, vocab, requests, capacity, words, biases, masks, mask_words, *_shape_pieces(rows, requests, vocab)),
+        fn(_SHAPE_CALL.pack(*places, rows, vocab, requests, capacity, words, biases, masks, mask_words, *_shape_pieces(rows, requests, vocab, capacity)),
            stream),
         "shape_logits",
     )
