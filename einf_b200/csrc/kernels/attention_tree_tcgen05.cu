@@ -2,22 +2,27 @@
 // and pages of 8 to 128 tokens.  What is computed and how a launch is cut into shares: attention_tree.cuh.
 //
 // A unit is up to two tiles of 128 rows (nodes x the query heads that share a key/value head) over the keys of
-// one request, 128 at a time.  The CTA has two slots, each a tile of rows with its own issuing thread, tensor memory and
-// softmax warpgroup; while one slot's scores are on their way through the exponentials' unit, the other's products
-// have the tensor core.  A unit of two tiles gives each slot one of them, and every tile of keys in shared memory serves
-// both; a unit of one tile gives both slots the same rows and every second tile of keys, and they are put
-// together at the end.
+// one request, 128 at a time.  The CTA has two slots, each a tile of rows with its own issuing warps, tensor memory and
+// two softmax warpgroups, one for either half of a tile's keys.  So four streams of scores, exponentials and sums are on their
+// way at once, and while one waits for the tensor core or for its scores the others have the units.  (With one stream a slot
+// both came to stand in step, exponentials against exponentials: 5,500 cycles for a tile of both slots at head size 128, of
+// which the tensor core had 2,200 and the exponentials' unit 2,048.)  A unit of two tiles gives each slot one of them, and every
+// tile of keys in shared memory serves both; a unit of one tile gives both slots the same rows and every second tile of
+// keys, and they are put together at the end.
 //
 //   warps 0, 1    K and V producers: TMA-load the pages that the block table names into rings of tiles
-//   warps 2, 3    issue a slot's products: S = Q K^T into tensor memory, O += P V with P from there
-//   warps 4-19    softmax, two warpgroups a slot: thread r of either has row r of the slot's tile, and half of its keys
+//   warps 2, 3    issue a slot's products, each stream's as what they need arrives: S = Q K^T into tensor memory, half a
+//                 tile of keys at a time, and O += P V with P from there
+//   warps 4-19    softmax: thread r of a warpgroup has row r of the slot's tile and 64 of a tile's 128 keys
 //
-// Sums stay in tensor memory, scaled by a reference that is the maximum of the row's first tile and moves only when a later
-// tile has a score 2^8 above it.
+// The streams agree on nothing while they run: a row's reference is a whole number at or above the maximum of its
+// first tile, and stays.  What that leaves to be done comes out at the end of a piece: a row with a sum of
+// weights above 2^60 (scores far above the reference; an overflow is such a sum too), or one that saw keys and has less
+// than 2^-60, sends the piece through again, once for the rows' maxima and once against those.
 //
-// Tiles with keys that some row does not see (the drafted ones, a window) run with masks of 128 bits a row.  There a
-// value that is not finite must not meet a weight of zero, so the V producer looks over such a tile, clears the
-// elements it finds and names their keys; the rows that do see such a key add them to their sums themselves.
+// Tiles with keys that some row does not see (the drafted ones, a window) run with masks of 64 bits a thread.  There a
+// value that is not finite must not meet a weight of zero, so the V producer looks over such a tile and clears the
+// elements it finds; if any of them is a key's, the rows that see it add them at the end of the piece, out of the cache.
 #include "attention_tree.cuh"
 #include "mma_sync.cuh"
 #include "tcgen05.cuh"
@@ -27,33 +32,35 @@ namespace einf {
 constexpr int kTile = 128;                     // rows of a slot, keys of a tile
 constexpr int kSlice = kTile * 128;            // a [128 rows x 64] bfloat16 slice: 16 KB
 constexpr int kTreeThreads = 640;
-constexpr float kMove = 8.f;                   // exponents above its reference at which a row moves it
-constexpr int kHalf = kTile / 2;               // keys of a softmax thread
+constexpr float kSumLimit = 1.15292150e18f;    // 2^60
+constexpr int kHalf = kTile / 2;               // keys of a stream
 constexpr int kTmemColumns = 512;              // S: 2 x 128 columns, O: 2 x D
 
 template <int D>
 struct Layout {
   static constexpr int kBlocks = D / 64;                       // 64-wide slices of the head
   static constexpr int kTileBytes = kBlocks * kSlice;
-  static constexpr int kKStages = D == 64 ? 5 : 3;
-  static constexpr int kVStages = D == 64 ? 5 : 2;
+  // even: where the slots take every second tile, a stage is always the same slot's, which has seen each of its phases
+  static constexpr int kKStages = D == 64 ? 6 : 2;
+  static constexpr int kVStages = D == 64 ? 4 : 2;
+  static_assert(kKStages % 2 == 0 && kVStages % 2 == 0, "stages of one slot");
   static constexpr int kQ = 0;                                 // a tile of rows per slot
   static constexpr int kK = kQ + 2 * kTileBytes;
   static constexpr int kV = kK + kKStages * kTileBytes;
   static constexpr int kBars = kV + kVStages * kTileBytes;
-  static constexpr int kNumBars = 8 + 3 * kKStages + 4 * kVStages;
-  static constexpr int kBad = kBars + 8 * kNumBars + 16;       // per V stage: 128 bits, rows of the tile that were cleared
-  static constexpr int kXchg = kBad + 16 * kVStages;           // a float for every thread of the softmax warps
-  // what the CTAs of a cluster exchange, in the place of the K and V tiles: the sums of 256 rows (padded so that neither
+  static constexpr int kNumBars = 14 + 3 * kKStages + 4 * kVStages;
+  static constexpr int kFlags = kBars + 8 * kNumBars + 8;      // to be done again (four, in turn), values that are not finite (four)
+  static constexpr int kXchg = kFlags + 32;                    // a float for every thread of the softmax warps
+  // what the CTAs of a cluster exchange, in the place of the Q, K and V tiles: the sums of 256 rows (padded so that neither
   // threads with a row each nor warps with a row each meet a bank twice), then reference and sum of every row
   static constexpr int kPitch = D + 4;
-  static constexpr int kSums = kK;
+  static constexpr int kSums = kQ;
   static constexpr int kSumsMl = kSums + 256 * kPitch * 4;
-  static_assert(kSumsMl + 256 * 8 <= kBars, "the exchange needs the K and V tiles");
+  static_assert(kSumsMl + 256 * 8 <= kBars, "the exchange needs the tiles");
   static constexpr int kBytes = kXchg + 4 * 128 * 4;
   static_assert(kBytes <= 227 * 1024, "shared memory of the tree attention kernel exceeds an SM");
   static_assert(2 * kBytes > 228 * 1024, "two CTAs on an SM would wait for each other's tensor memory");
-  static_assert(kXchg % 8 == 0 && kBad % 4 == 0, "alignment");
+  static_assert(kXchg % 8 == 0 && kFlags % 4 == 0, "alignment");
 };
 
 __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
@@ -92,20 +99,73 @@ __device__ __forceinline__ float2 ld_peer2(uint32_t local, uint32_t rank) {
   return v;
 }
 __device__ __forceinline__ void both_slots_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
-// The two warps with the same rows meet; true if `value` is, in any thread of them.
-__device__ __forceinline__ bool pair_any(int pair, bool value) {
-  uint32_t any;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %2, 0;\n\t"
-      "barrier.cta.red.or.pred q, %1, 64, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(any)
-      : "r"(2 + pair), "r"((uint32_t)value)
-      : "memory");
-  return any != 0;
-}
+// The two warps of a slot with the same rows meet.
 __device__ __forceinline__ void pair_sync(int pair) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(2 + pair) : "memory"); }
+
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max3_or_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^x by fused multiply-adds, for the scores that the exponentials' unit (16 a cycle) is spared: x = n + f with n the nearest whole
+// number, |f| <= 1/2, and 2^f as a polynomial of the fourth degree whose largest relative error, 2.8e-6, is the least that one
+// with p(0) = 1 has.  n comes out of adding 1.5 x 2^23, which leaves it in the low bits, from where it is shifted onto the
+// exponent.  With a reference that is a whole number the reference and that constant are one exact addend, and a pair of scores
+// takes seven two-way operations.
+constexpr float kRound = 12582912.f;                // 1.5 x 2^23
+constexpr float kLargestReference = 8192.f;         // up to here n and f come out exact enough
+constexpr int kShared = 3;                          // of eight pairs: 1,280 cycles of either kind for a tile of both slots
+
+// 16 scores of a row to 2^(scale s - m): packed, and added to `sum`.  `highest` is the largest kRound + n that was shifted,
+// or NaN if a score is; what lies above the type's exponents has come out wrong.
+__device__ __forceinline__ void shared_exps(const float* v, uint32_t* packed, float scale, float m, float2* sum, float* highest) {
+  const float2 scale2 = make_float2(scale, scale), shift2 = make_float2(-m, -m), base2 = make_float2(kRound - m, kRound - m);
+  const float2 c1 = make_float2(6.9312412e-1f, 6.9312412e-1f), c2 = make_float2(2.4024107e-1f, 2.4024107e-1f);
+  const float2 c3 = make_float2(5.5906828e-2f, 5.5906828e-2f), c4 = make_float2(9.5825763e-3f, 9.5825763e-3f);
+  const float2 one2 = make_float2(1.f, 1.f), minus2 = make_float2(-1.f, -1.f);
+  const float lowest = __fdividef(m - 126.75f, scale);     // weights below 2^-126.75 count as that
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 s = make_float2(v[2 * i], v[2 * i + 1]);
+    float2 e;
+    if (i * kShared % 8 < kShared) {
+      const float2 bound = make_float2(max_or_nan(s.x, lowest), max_or_nan(s.y, lowest));
+      const float2 t = __ffma2_rn(bound, scale2, base2);              // kRound + n
+      *highest = max3_or_nan(*highest, t.x, t.y);
+      const float2 f = __ffma2_rn(bound, scale2, __ffma2_rn(t, minus2, base2));
+      float2 y = __ffma2_rn(f, c4, c3);
+      y = __ffma2_rn(y, f, c2);
+      y = __ffma2_rn(y, f, c1);
+      y = __ffma2_rn(y, f, one2);
+      e.x = __uint_as_float((__float_as_uint(t.x) << 23) + __float_as_uint(y.x));
+      e.y = __uint_as_float((__float_as_uint(t.y) << 23) + __float_as_uint(y.y));
+    } else {
+      const float2 x = __ffma2_rn(s, scale2, shift2);
+      e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+    }
+    *sum = __fadd2_rn(*sum, e);
+    packed[i] = pack_pair(e.x, e.y);
+  }
+}
+// tmem_ld_wait32 of tcgen05.cuh for 16 columns.
+__device__ __forceinline__ void tmem_ld_wait16(float* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]),
+                 "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 
 // A cluster shares the key tiles of its piece out among its CTAs.
 __device__ __forceinline__ void share_out(TreeWalk* w, int rank, int cluster) {
@@ -156,7 +216,7 @@ __device__ __forceinline__ void merge_cluster(const TreeParams& p, const TreeWal
 struct Row {
   bool live;
   int token, position, lowest;
-  float m, l;               // the reference and the sum of weights
+  float m, l;               // the reference, a whole number, and the sum of weights
 };
 
 // What a slot has of a unit.
@@ -191,28 +251,31 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
   }
   const uint32_t bars = base + L::kBars;
   auto q_full = [&](int g) { return bars + 8u * g; };
-  auto s_full = [&](int g) { return bars + 8u * (2 + g); };
-  auto p_full = [&](int g) { return bars + 8u * (4 + g); };
-  auto o_done = [&](int g) { return bars + 8u * (6 + g); };
-  auto k_full = [&](int s) { return bars + 8u * (8 + s); };
-  auto k_empty = [&](int g, int s) { return bars + 8u * (8 + (1 + g) * L::kKStages + s); };
-  auto v_full = [&](int s) { return bars + 8u * (8 + 3 * L::kKStages + s); };
-  auto v_checked = [&](int s) { return bars + 8u * (8 + 3 * L::kKStages + L::kVStages + s); };
-  auto v_empty = [&](int g, int s) { return bars + 8u * (8 + 3 * L::kKStages + (2 + g) * L::kVStages + s); };
+  auto s_full = [&](int g, int h) { return bars + 8u * (2 + 2 * g + h); };
+  auto p_full = [&](int g, int h) { return bars + 8u * (6 + 2 * g + h); };
+  auto o_done = [&](int g, int h) { return bars + 8u * (10 + 2 * g + h); };
+  auto k_full = [&](int s) { return bars + 8u * (14 + s); };
+  auto k_empty = [&](int g, int s) { return bars + 8u * (14 + (1 + g) * L::kKStages + s); };
+  auto v_full = [&](int s) { return bars + 8u * (14 + 3 * L::kKStages + s); };
+  auto v_checked = [&](int s) { return bars + 8u * (14 + 3 * L::kKStages + L::kVStages + s); };
+  auto v_empty = [&](int g, int s) { return bars + 8u * (14 + 3 * L::kKStages + (2 + g) * L::kVStages + s); };
   const uint32_t tmem_holder = bars + 8 * L::kNumBars;
-  uint32_t* cleared = reinterpret_cast<uint32_t*>(smem_raw + L::kBad);      // [V stage][4]
+  volatile int* flags = reinterpret_cast<volatile int*>(smem_raw + L::kFlags);      // [4] to be done again, [4] values that are not finite
   float* xchg = reinterpret_cast<float*>(smem_raw + L::kXchg);              // [slot][half of the keys][row]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int g = 0; g < 2; ++g) {
       bar_init(q_full(g), 1);
-      bar_init(s_full(g), 1);
-      bar_init(p_full(g), 256);
-      bar_init(o_done(g), 1);
+      for (int h = 0; h < 2; ++h) {
+        bar_init(s_full(g, h), 1);
+        bar_init(p_full(g, h), 128);
+        bar_init(o_done(g, h), 1);
+      }
       for (int s = 0; s < L::kKStages; ++s) bar_init(k_empty(g, s), 1);
       for (int s = 0; s < L::kVStages; ++s) bar_init(v_empty(g, s), 1);
     }
+    for (int i = 0; i < 8; ++i) flags[i] = 0;
     for (int s = 0; s < L::kKStages; ++s) bar_init(k_full(s), 1);
     for (int s = 0; s < L::kVStages; ++s) {
       bar_init(v_full(s), 1);
@@ -229,8 +292,8 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(smem_raw + L::kBars + 8 * L::kNumBars);
-  // the scores and, in the first 32 of the 64 columns of either half of the keys, the probabilities
-  auto tmem_s = [&](int g) { return tmem_base + 128u * g; };
+  // the scores of half a tile of keys and, in the first 32 of their 64 columns, the probabilities
+  auto tmem_s = [&](int g, int h) { return tmem_base + 128u * g + 64u * h; };
   auto tmem_o = [&](int g) { return tmem_base + 256u + (uint32_t)D * g; };
   pdl_launch_dependents();   // after the tensor-memory allocation, see common.cuh
   pdl_wait();
@@ -240,7 +303,24 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
   bool any = tree_first(p, worker, &w);
   if (threadIdx.x == 0 && rank == 0) tree_note(p, worker, w, any);
   if (any && cluster > 1) share_out(&w, rank, cluster);
-  // Every warp ends a piece here.  The CTAs of a cluster put their shares of it together: once they have all left them in shared
+  // How a piece is gone through: as it comes, then, if that did not serve, for its rows' maxima and against them.
+  enum { kAsItComes = 0, kForMaxima = 1, kAgainstMaxima = 2 };
+  int way = kAsItComes, turn = 0, pieces = 0;
+  // Every warp ends a passage through a piece here, when its products are complete, and learns whether it is the last.  (A flag is
+  // cleared three turns after it was last looked at.)
+  auto last_passage = [&]() {
+    if (threadIdx.x == 0) {
+      flags[(turn + 1) & 3] = 0;
+      flags[4 + ((pieces + 1) & 3)] = 0;
+    }
+    __syncwarp();
+    __syncthreads();
+    const bool again = way == kForMaxima || (way == kAsItComes && flags[turn & 3] != 0);
+    ++turn;
+    way = again ? way + 1 : kAsItComes;
+    return !again;
+  };
+  // And a piece here.  The CTAs of a cluster put their shares of it together: once they have all left them in shared
   // memory, and before any of them takes that for the next piece (or leaves).
   auto next_piece = [&]() {
     if (cluster > 1) {
@@ -253,6 +333,7 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
     }
     any = tree_next(p, worker, &w);
     if (any && cluster > 1) share_out(&w, rank, cluster);
+    ++pieces;
   };
 
   if (warp < 2) {
@@ -280,159 +361,185 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
         if (i >= w.tile_end || lane >= pages_of(i)) return 0;
         return table[((w.t.begin + i * kTile) >> page_shift) + lane];
       };
-      // read two tiles ahead of their use
-      int page = read_page(w.tile_begin), page_next = read_page(w.tile_begin + 1);
-      for (int i = w.tile_begin; i < w.tile_end && ok; ++i) {
-        const int page_after = read_page(i + 2);
-        const int pages = pages_of(i);
-        if (page < 0 || page >= p.num_pages) {
-          bad = true;
-          page = 0;   // keep the byte count right; the status word fails the step
-        }
-        const int page0 = __shfl_sync(0xffffffffu, page, 0);
-        // pages that follow one another in the pool come as one box
-        const bool run = pages_per_tile > 1 && pages == pages_per_tile && page0 + pages <= p.num_pages &&
-                         __all_sync(0xffffffffu, lane >= pages || page == page0 + lane);
-        const uint32_t bit = 1u << stage;
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-          if (held[g] & bit) {
-            ok = __all_sync(0xffffffffu, bar_wait(empty_bar(g, stage), (parity[g] >> stage) & 1u, p.status)) && ok;
-            parity[g] ^= bit;
-            held[g] &= ~bit;
+      do {
+        // read two tiles ahead of their use
+        int page = read_page(w.tile_begin), page_next = read_page(w.tile_begin + 1);
+        for (int i = w.tile_begin; i < w.tile_end && ok; ++i) {
+          const int page_after = read_page(i + 2);
+          const int pages = pages_of(i);
+          if (page < 0 || page >= p.num_pages) {
+            bad = true;
+            page = 0;   // keep the byte count right; the status word fails the step
           }
-        if (!ok) break;
-        if (pair) {
-          held[0] |= bit;
-          held[1] |= bit;
-        } else {
-          held[(i - w.tile_begin) & 1] |= bit;
-        }
-        const uint32_t full = full_bar(stage);
-        if (lane == 0) bar_expect_tx(full, (uint32_t)pages * page_bytes * L::kBlocks);
-        __syncwarp();
-        const uint32_t offset = (warp ? L::kV : L::kK) + stage * L::kTileBytes;
-        if (run) {
-          if (lane < L::kBlocks) tma_4d(base + offset + lane * kSlice, run_map, lane * 64, 0, u.kv_head, page0, full);
-        } else if (lane < pages) {
-          const int row = (page * p.kv_heads + u.kv_head) * p.page_size;
+          const int page0 = __shfl_sync(0xffffffffu, page, 0);
+          // pages that follow one another in the pool come as one box
+          const bool run = pages_per_tile > 1 && pages == pages_per_tile && page0 + pages <= p.num_pages &&
+                           __all_sync(0xffffffffu, lane >= pages || page == page0 + lane);
+          const uint32_t bit = 1u << stage;
 #pragma unroll
-          for (int db = 0; db < L::kBlocks; ++db)
-            tma_2d(base + offset + db * kSlice + lane * page_bytes, map, db * 64, row, full);
-        }
-        if (warp) {
-          if (p.window > 0 || w.t.begin + (i + 1) * kTile > w.t.cached) {
-            // some row may not see some key of the tile: rows that are not finite are cleared and named
-            ok = __all_sync(0xffffffffu, bar_wait(full, round & 1, p.status));
-#pragma unroll 1
-            for (int r0 = 0; r0 < kTile; r0 += 32) {
-              const int r = r0 + lane;
-              unsigned char* row = smem_raw + offset + (r >> 3) * 1024 + (r & 7) * 128;
-              uint32_t found = 0u;
-#pragma unroll
-              for (int db = 0; db < L::kBlocks; ++db)
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                  const uint4 v = *reinterpret_cast<const uint4*>(row + db * kSlice + ((c ^ (r & 7)) << 4));
-                  found |= not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w);
-                }
-              if (found)
-                for (int c = 0; c < 32 * L::kBlocks; ++c) {
-                  uint32_t* pair = reinterpret_cast<uint32_t*>(row + (c >> 5) * kSlice + ((c & 31) << 2));
-                  *pair &= ~((not_finite(*pair) >> 15) * 0xffffu);
-                }
-              const uint32_t rows = __ballot_sync(0xffffffffu, found != 0u);
-              if (lane == 0) cleared[stage * 4 + (r0 >> 5)] = rows;
+          for (int g = 0; g < 2; ++g)
+            if (held[g] & bit) {
+              ok = __all_sync(0xffffffffu, bar_wait(empty_bar(g, stage), (parity[g] >> stage) & 1u, p.status)) && ok;
+              parity[g] ^= bit;
+              held[g] &= ~bit;
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-          } else if (lane < 4) {
-            cleared[stage * 4 + lane] = 0u;
+          if (!ok) break;
+          if (pair) {
+            held[0] |= bit;
+            held[1] |= bit;
+          } else {
+            held[(i - w.tile_begin) & 1] |= bit;
           }
+          const uint32_t full = full_bar(stage);
+          if (lane == 0) bar_expect_tx(full, (uint32_t)pages * page_bytes * L::kBlocks);
           __syncwarp();
-          if (lane == 0) bar_arrive(v_checked(stage));
+          const uint32_t offset = (warp ? L::kV : L::kK) + stage * L::kTileBytes;
+          if (run) {
+            if (lane < L::kBlocks) tma_4d(base + offset + lane * kSlice, run_map, lane * 64, 0, u.kv_head, page0, full);
+          } else if (lane < pages) {
+            const int row = (page * p.kv_heads + u.kv_head) * p.page_size;
+#pragma unroll
+            for (int db = 0; db < L::kBlocks; ++db)
+              tma_2d(base + offset + db * kSlice + lane * page_bytes, map, db * 64, row, full);
+          }
+          if (warp) {
+            if (p.window > 0 || w.t.begin + (i + 1) * kTile > w.t.cached) {
+              // some row may not see some key of the tile: what is not finite is cleared
+              ok = __all_sync(0xffffffffu, bar_wait(full, round & 1, p.status));
+#pragma unroll 1
+              for (int r0 = 0; r0 < kTile; r0 += 32) {
+                const int r = r0 + lane;
+                unsigned char* row = smem_raw + offset + (r >> 3) * 1024 + (r & 7) * 128;
+                uint32_t found = 0u;
+#pragma unroll
+                for (int db = 0; db < L::kBlocks; ++db)
+#pragma unroll
+                  for (int c = 0; c < 8; ++c) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(row + db * kSlice + ((c ^ (r & 7)) << 4));
+                    found |= not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w);
+                  }
+                if (found)
+                  for (int c = 0; c < 32 * L::kBlocks; ++c) {
+                    uint32_t* pair = reinterpret_cast<uint32_t*>(row + (c >> 5) * kSlice + ((c & 31) << 2));
+                    *pair &= ~((not_finite(*pair) >> 15) * 0xffffu);
+                  }
+                if (found && w.t.begin + i * kTile + r < keys_end) flags[4 + (pieces & 3)] = 1;
+              }
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            }
+            __syncwarp();
+            if (lane == 0) bar_arrive(v_checked(stage));
+          }
+          page = page_next;
+          page_next = page_after;
+          if (++stage == stages) {
+            stage = 0;
+            ++round;
+          }
         }
-        page = page_next;
-        page_next = page_after;
-        if (++stage == stages) {
-          stage = 0;
-          ++round;
-        }
-      }
+      } while (!last_passage());
     }
     if (__any_sync(0xffffffffu, bad) && lane == 0) atomicOr(p.status, kStatusBadPage);
   } else if (warp < 4) {
     // ---- a slot's products: the whole warp goes the way of the lane that issues, so that addresses stay in uniform registers ----
     const int g = warp - 2;
-    // S: M = 128 rows, N = 128 keys, both K-major.  O: M = 128, N = D, P from tensor memory, V MN-major.
-    constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kTile >> 3) << 17) | ((128u >> 4) << 24);
+    // S: M = 128 rows, N = 64 keys, both K-major.  O: M = 128, N = D, P from tensor memory, V MN-major.
+    constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kHalf >> 3) << 17) | ((128u >> 4) << 24);
     constexpr uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
     const uint64_t desc_q = desc_k_major(base + L::kQ + g * L::kTileBytes);
     auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, bar_wait_likely_done(bar, parity, p.status)) != 0; };
+    auto there = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, bar_test(bar, parity)) != 0; };
     bool ok = true;
     int queries = 0;               // loads of Q so far
     int done = 0;                  // this slot's tiles so far
-    int before = 0;                // the CTA's tiles before this piece
+    int before = 0;                // the CTA's tiles before this passage
     for (; any; next_piece()) {
       const TreeUnit u = tree_unit(p, w.t, w.unit);
       const Slot s = slot_of(w, u, g);
-      const int first = before + s.first_tile - w.tile_begin;
-      before += w.tile_end - w.tile_begin;
-      if (s.tiles == 0 || !ok) continue;
-      if (elect_one()) {
-        bar_expect_tx(q_full(g), (uint32_t)(p.unit_nodes / 2 * u.heads) * 128u * L::kBlocks);
-        for (int db = 0; db < L::kBlocks; ++db)
-          tma_3d(base + L::kQ + g * L::kTileBytes + db * kSlice, &map_q, db * 64, u.first_head, w.t.first + u.first_node + s.first_node,
-                 q_full(g));
-      }
-      __syncwarp();
-      ok = wait(q_full(g), queries & 1);
-      ++queries;
-#pragma unroll 1
-      for (int j = 0; j < s.tiles && ok; ++j, ++done) {
-        const int c = first + j * s.step, k_stage = c % L::kKStages, v_stage = c % L::kVStages;
-        ok = wait(k_full(k_stage), (c / L::kKStages) & 1);
-        if (!ok) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (s.tiles > 0 && ok) {
         if (elect_one()) {
-          const uint64_t desc_k = desc_k_major(base + L::kK + k_stage * L::kTileBytes);
-#pragma unroll
+          bar_expect_tx(q_full(g), (uint32_t)(p.unit_nodes / 2 * u.heads) * 128u * L::kBlocks);
           for (int db = 0; db < L::kBlocks; ++db)
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              mma_ss(tmem_s(g), desc_advance(desc_q, db * kSlice + kk * 32), desc_advance(desc_k, db * kSlice + kk * 32), idesc_s,
-                     (db > 0 || kk > 0) ? 1u : 0u);
-          mma_commit(s_full(g));
-          mma_commit(k_empty(g, k_stage));
+            tma_3d(base + L::kQ + g * L::kTileBytes + db * kSlice, &map_q, db * 64, u.first_head, w.t.first + u.first_node + s.first_node,
+                   q_full(g));
         }
         __syncwarp();
-        const uint32_t parity = (c / L::kVStages) & 1;
-        ok = wait(v_full(v_stage), parity) && wait(v_checked(v_stage), parity) && wait(p_full(g), done & 1);
-        if (!ok) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (elect_one()) {
-          const uint64_t desc_v = desc_mn_major(base + L::kV + v_stage * L::kTileBytes, kSlice);
-#pragma unroll
-          for (int ks = 0; ks < kTile / 16; ++ks)      // onto the zeros or sums that the softmax warps left
-            mma_ts(tmem_o(g), tmem_s(g) + (ks >> 2) * kHalf + (ks & 3) * 8, desc_advance(desc_v, ks * 16 * 128), idesc_o, 1u);
-          mma_commit(o_done(g));
-          mma_commit(v_empty(g, v_stage));
-        }
-        __syncwarp();
-        // the scores' place holds the probabilities until the product has them; after the last, Q's place is free too
-        ok = wait(o_done(g), done & 1);
+        ok = wait(q_full(g), queries & 1);
+        ++queries;
       }
+      do {
+        const int first = before + s.first_tile - w.tile_begin;
+        before += w.tile_end - w.tile_begin;
+        // per stream: tiles whose scores, and whose sums, have been issued
+        int scored[2] = {0, 0}, summed[2] = {0, 0}, polls = 0;
+        while (ok && (summed[0] < s.tiles || summed[1] < s.tiles)) {
+          bool progress = false;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            // sums, onto the zeros or sums that are there
+            const int v_tile = first + summed[h] * s.step, v_stage = v_tile % L::kVStages;
+            const uint32_t v_parity = (v_tile / L::kVStages) & 1;
+            if (summed[h] < scored[h] && there(p_full(g, h), (done + summed[h]) & 1) && there(v_full(v_stage), v_parity) &&
+                there(v_checked(v_stage), v_parity)) {
+              const int j = summed[h], stage = v_stage;
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+              if (elect_one()) {
+                const uint64_t desc_v = desc_mn_major(base + L::kV + stage * L::kTileBytes + h * kHalf * 128, kSlice);
+#pragma unroll
+                for (int ks = 0; ks < kHalf / 16; ++ks)
+                  mma_ts(tmem_o(g), tmem_s(g, h) + ks * 8, desc_advance(desc_v, ks * 16 * 128), idesc_o, 1u);
+                mma_commit(o_done(g, h));
+                if (summed[h ^ 1] > j) mma_commit(v_empty(g, stage));      // the other half is through too
+              }
+              __syncwarp();
+              summed[h] = j + 1;
+              progress = true;
+            }
+            // scores; their place holds the probabilities of the tile before until the product has them
+            if (scored[h] < s.tiles && scored[h] == summed[h] &&
+                (scored[h] == 0 || there(o_done(g, h), (done + scored[h] - 1) & 1))) {
+              const int j = scored[h], c = first + j * s.step, stage = c % L::kKStages;
+              if (there(k_full(stage), (c / L::kKStages) & 1)) {
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (elect_one()) {
+                  const uint64_t desc_k = desc_k_major(base + L::kK + stage * L::kTileBytes + h * kHalf * 128);      // rows of 128 bytes
+#pragma unroll
+                  for (int db = 0; db < L::kBlocks; ++db)
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                      mma_ss(tmem_s(g, h), desc_advance(desc_q, db * kSlice + kk * 32), desc_advance(desc_k, db * kSlice + kk * 32), idesc_s,
+                             (db > 0 || kk > 0) ? 1u : 0u);
+                  mma_commit(s_full(g, h));
+                  if (scored[h ^ 1] > j) mma_commit(k_empty(g, stage));
+                }
+                __syncwarp();
+                scored[h] = j + 1;
+                progress = true;
+              }
+            }
+          }
+          if (progress) {
+            polls = 0;
+          } else if (++polls > kPolls) {
+            if (lane == 0) atomicOr(p.status, kStatusWaitExpired);
+            ok = false;
+          }
+        }
+        done += s.tiles;
+        // the products are complete: Q's place, and the sums, are free
+        if (s.tiles > 0) ok = ok && wait(o_done(g, 0), (done - 1) & 1) && wait(o_done(g, 1), (done - 1) & 1);
+      } while (!last_passage());
     }
   } else {
-    // ---- softmax: thread r has row r of its slot, and 64 of the 128 keys of a tile ----
+    // ---- softmax: thread r has row r of its slot, and the first or the second 64 of a tile's 128 keys ----
     const int g = (warp - 4) >> 3, part = (warp - 4) >> 2 & 1, r = (warp & 3) * 32 + lane, pair = g * 4 + (warp & 3);
     const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_row = tmem_s(g) + lane_addr + part * kHalf, o_row = tmem_o(g) + lane_addr;
+    const uint32_t s_row = tmem_s(g, part) + lane_addr, o_row = tmem_o(g) + lane_addr;
     float* my_xchg = xchg + (g * 2 + part) * 128 + r;
     const float* pair_xchg = xchg + (g * 2 + (part ^ 1)) * 128 + r;
     const ScoreScale sc = make_score_scale(p.scale, p.softcap);
     bool ok = true;
-    int done = 0, before = 0;
+    int done = 0;
     for (; any; next_piece()) {
       const TreeUnit u = tree_unit(p, w.t, w.unit);
       const Slot s = slot_of(w, u, g);
@@ -445,160 +552,132 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
       row.position = row.live ? tree_position(p, w.t, row.token) : 0;
       row.lowest = row.live ? tree_lowest(p, row.position) : 0;
       row.m = -INFINITY;
-      row.l = 0.f;
       // keys that every row of the warp sees, but for those from the drafted ones on
       const int all_from = p.window > 0 ? __reduce_max_sync(0xffffffffu, row.lowest) : 0;
-      const int first = before + s.first_tile - w.tile_begin;
-      before += w.tile_end - w.tile_begin;
-      if (s.tiles > 0 && warp_live) {
-        uint32_t zero[16];
+      do {
+        float highest = kRound, best = -INFINITY;
+        bool some = false, cheap = false;      // the row has seen a key; the warp's references allow shared_exps
+        row.l = 0.f;
+        if (s.tiles > 0 && warp_live) {
+          uint32_t zero[16];
 #pragma unroll
-        for (int c = 0; c < 16; ++c) zero[c] = 0u;
+          for (int c = 0; c < 16; ++c) zero[c] = 0u;
 #pragma unroll 1
-        for (int c0 = part * (D / 2); c0 < (part + 1) * (D / 2); c0 += 16) tmem_st16(o_row + c0, zero);
-      }
-#pragma unroll 1
-      for (int j = 0; j < s.tiles; ++j, ++done) {      // `done` counts this slot's tiles
-        if (ok) ok = __all_sync(0xffffffffu, bar_wait_likely_done(s_full(g), done & 1, p.status));
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (warp_live) {
-          const int tile0 = w.t.begin + (s.first_tile + j * s.step) * kTile, key0 = tile0 + part * kHalf;
-          const bool all_visible = key0 >= all_from && key0 + kHalf <= w.t.cached;
-          uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
-          if (!all_visible) {
-#pragma unroll 1
-            for (int c = 0; c < 2; ++c) {
-              const uint32_t bits = row.live ? tree_visible(p, w.t, row.token, row.lowest, row.position, key0 + 32 * c) : 0u;
-              if (c) seen[1] = bits;
-              else seen[0] = bits;
-            }
-            __syncwarp();
-          }
-          auto mask = [&](float* v, uint32_t bits) {
-#pragma unroll
-            for (int c = 0; c < 32; ++c) v[c] = bits >> c & 1u ? v[c] : -INFINITY;
-          };
-          float top = -INFINITY;
-#pragma unroll 1
-          for (int c0 = 0; c0 < kHalf; c0 += 32) {
-            float v[32];
-            tmem_ld32(s_row + c0, v);
-            tmem_ld_wait32(v);
-            if (!all_visible) mask(v, c0 ? seen[1] : seen[0]);
-            float top4[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) top4[c] = max3(v[c], v[c + 4], v[c + 8]);
-#pragma unroll
-            for (int c = 12; c < 28; c += 8)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) top4[e] = max3(top4[e], v[c + e], v[c + 4 + e]);
-            top = max3(top, max3(top4[0], top4[1], v[28]), max3(max3(top4[2], top4[3], v[29]), v[30], v[31]));
-          }
-          // the scale is positive and the cap grows with the score: the maximum and either commute
-          top = top == -INFINITY ? -INFINITY : score_log2(top, sc);
-          // where a row has no reference yet, or a score far above it, the two warps with it settle on one
-          if (pair_any(pair, row.live && top > (row.m == -INFINITY ? -INFINITY : row.m + kMove))) {
-            *my_xchg = top;
-            pair_sync(pair);
-            top = fmaxf(fmaxf(top, *pair_xchg), row.m);
-            const float factor = top == -INFINITY ? 1.f : row.m == -INFINITY ? 0.f : fast_exp2(row.m - top);
-            if (j > 0) {      // (the product of the tile before is complete: these scores lie in its probabilities' place)
-#pragma unroll 1
-              for (int c0 = part * (D / 2); c0 < (part + 1) * (D / 2); c0 += 16) {
-                float o[16];
-                tmem_ld16(o_row + c0, o);
-                tmem_ld_wait();
-                uint32_t bits[16];
-#pragma unroll
-                for (int c = 0; c < 16; ++c) bits[c] = __float_as_uint(o[c] * factor);
-                tmem_st16(o_row + c0, bits);
-              }
-            }
-            row.l = row.l == 0.f ? 0.f : row.l * factor;
-            row.m = top;
-            pair_sync(pair);      // before either writes its place again
-          }
-          const float m_use = row.m == -INFINITY ? 0.f : row.m;
-          const float2 scale2 = make_float2(sc.scale_log2, sc.scale_log2), shift2 = make_float2(-m_use, -m_use);
-          float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll 1
-          for (int c0 = 0; c0 < kHalf; c0 += 32) {
-            float v[32];
-            tmem_ld32(s_row + c0, v);
-            tmem_ld_wait32(v);
-            if (!all_visible) mask(v, c0 ? seen[1] : seen[0]);
-            if (sc.tanh_in != 0.f) {
-#pragma unroll
-              for (int c = 0; c < 32; ++c) v[c] = v[c] == -INFINITY ? -INFINITY : __fdividef(capped(v[c], sc), sc.scale_log2);
-            }
-            uint32_t packed[16];
-#pragma unroll
-            for (int c = 0; c < 32; c += 2) {
-              const float2 x = __ffma2_rn(make_float2(v[c], v[c + 1]), scale2, shift2);
-              const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-              sum2[c >> 1 & 1] = __fadd2_rn(sum2[c >> 1 & 1], e);
-              packed[c >> 1] = pack_pair(e.x, e.y);
-            }
-            tmem_st16(s_row + (c0 >> 1), packed);      // two keys to a column, over scores that were read
-          }
-          row.l += (sum2[0].x + sum2[1].x) + (sum2[0].y + sum2[1].y);
-          if (tile0 < all_from || tile0 + kTile > w.t.cached) {
-            // Values that are not finite, for the rows that see their keys: the two warps one after the other.
-            const int c = first + j * s.step, stage = c % L::kVStages;
-            const uint32_t* named = cleared + stage * 4;
-            ok = __all_sync(0xffffffffu, bar_wait_likely_done(v_checked(stage), (c / L::kVStages) & 1, p.status)) && ok;
-            tmem_st_wait();
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            if (pair_any(pair, ok && (named[0] | named[1] | named[2] | named[3]) != 0u)) {
-#pragma unroll 1
-              for (int word = 0; word < 4; ++word) {
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t mine = word >> 1 == part && ok ? named[word] & (word & 1 ? seen[1] : seen[0]) : 0u;
-#pragma unroll 1
-                for (uint32_t rest = __reduce_or_sync(0xffffffffu, mine); rest; rest &= rest - 1) {
-                  const int bit = __ffs(rest) - 1, key = tile0 + 32 * word + bit;
-                  const int page = p.block_table[(size_t)w.request * p.table_width + key / p.page_size];
-                  const bool add = (mine >> bit & 1u) && page >= 0 && page < p.num_pages;
-                  const __nv_bfloat16* value = static_cast<const __nv_bfloat16*>(p.v_cache) +
-                      (((size_t)(add ? page : 0) * p.kv_heads + u.kv_head) * p.page_size + key % p.page_size) * D;
-#pragma unroll 1
-                  for (int c0 = 0; c0 < D; c0 += 16) {
-                    float o[16];
-                    tmem_st_wait();
-                    tmem_ld16(o_row + c0, o);
-                    tmem_ld_wait();
-                    uint32_t bits[16];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                      const float x = add ? __bfloat162float(value[c0 + e]) : 0.f;
-                      bits[e] = __float_as_uint(isfinite(x) ? o[e] : o[e] + x);       // times a weight above zero
-                    }
-                    tmem_st16(o_row + c0, bits);
-                  }
-                }
-                tmem_st_wait();
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                pair_sync(pair);
-              }
-            }
-          }
+          for (int c0 = part * (D / 2); c0 < (part + 1) * (D / 2); c0 += 16) tmem_st16(o_row + c0, zero);
           tmem_st_wait();
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          pair_sync(pair);      // the first product of either half finds all of the row's zeros
+          cheap = __all_sync(0xffffffffu, !row.live || fabsf(row.m) <= kLargestReference) && sc.tanh_in == 0.f;
         }
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        bar_arrive(p_full(g));
-      }
-      if (ok && s.tiles > 0) {
-        ok = __all_sync(0xffffffffu, bar_wait(o_done(g), (done - 1) & 1, p.status));
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      }
+#pragma unroll 1
+        for (int j = 0; j < s.tiles; ++j, ++done) {      // `done` counts this slot's tiles
+          if (ok) ok = __all_sync(0xffffffffu, bar_wait_likely_done(s_full(g, part), done & 1, p.status));
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          if (warp_live) {
+            const int key0 = w.t.begin + (s.first_tile + j * s.step) * kTile + part * kHalf;
+            const bool all_visible = key0 >= all_from && key0 + kHalf <= w.t.cached;
+            uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
+            if (!all_visible) {
+#pragma unroll 1
+              for (int c = 0; c < 2; ++c) {
+                const uint32_t bits = row.live ? tree_visible(p, w.t, row.token, row.lowest, row.position, key0 + 32 * c) : 0u;
+                if (c) seen[1] = bits;
+                else seen[0] = bits;
+              }
+              __syncwarp();
+            }
+            some = some || (seen[0] | seen[1]) != 0u;
+            // sixteen scores from column c0 on, -inf where the key is not seen
+            auto scores = [&](int c0, float* v, bool masked) {
+              tmem_ld16(s_row + c0, v);
+              tmem_ld_wait16(v);
+              if (masked) {
+                const uint32_t bits = (c0 < 32 ? seen[0] : seen[1]) >> (c0 & 31);
+#pragma unroll
+                for (int c = 0; c < 16; ++c) v[c] = bits >> c & 1u ? v[c] : -INFINITY;
+              }
+            };
+            if (way == kForMaxima || (way == kAsItComes && j == 0)) {
+              float top = -INFINITY;
+#pragma unroll 1
+              for (int c0 = 0; c0 < kHalf; c0 += 16) {
+                float v[16];
+                scores(c0, v, !all_visible);
+#pragma unroll
+                for (int c = 0; c < 16; c += 4) top = max3(top, max3(v[c], v[c + 1], v[c + 2]), v[c + 3]);
+              }
+              best = fmaxf(best, top);
+              if (way == kAsItComes) {
+                // The row's reference: whole, at or above the maximum of the tile (the scale is positive and the cap grows with
+                // the score: the maximum and either commute); nothing where the row sees none of it.
+                *my_xchg = best;
+                pair_sync(pair);
+                best = fmaxf(best, *pair_xchg);
+                row.m = best == -INFINITY ? 0.f : ceilf(score_log2(best, sc));
+                cheap = __all_sync(0xffffffffu, !row.live || fabsf(row.m) <= kLargestReference) && sc.tanh_in == 0.f;
+              }
+            }
+            const float2 scale2 = make_float2(sc.scale_log2, sc.scale_log2), shift2 = make_float2(-row.m, -row.m);
+            float2 sum2 = make_float2(0.f, 0.f);
+            if (all_visible && cheap && way != kForMaxima) {
+#pragma unroll 1
+              for (int c0 = 0; c0 < kHalf; c0 += 16) {
+                float v[16];
+                uint32_t packed[8];
+                scores(c0, v, false);
+                shared_exps(v, packed, sc.scale_log2, row.m, &sum2, &highest);
+                tmem_st8(s_row + (c0 >> 1), packed);      // two keys to a column, over scores that were read
+              }
+            } else {
+              if (way == kForMaxima) seen[0] = seen[1] = 0u;
+#pragma unroll 1
+              for (int c0 = 0; c0 < kHalf; c0 += 16) {
+                float v[16];
+                uint32_t packed[8];
+                scores(c0, v, true);
+                if (sc.tanh_in != 0.f) {
+#pragma unroll
+                  for (int c = 0; c < 16; ++c) v[c] = v[c] == -INFINITY ? -INFINITY : __fdividef(capped(v[c], sc), sc.scale_log2);
+                }
+#pragma unroll
+                for (int c = 0; c < 16; c += 2) {
+                  const float2 x = __ffma2_rn(make_float2(v[c], v[c + 1]), scale2, shift2);
+                  const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+                  sum2 = __fadd2_rn(sum2, e);
+                  packed[c >> 1] = pack_pair(e.x, e.y);
+                }
+                tmem_st8(s_row + (c0 >> 1), packed);
+              }
+            }
+            row.l += sum2.x + sum2.y;
+            tmem_st_wait();
+          }
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          bar_arrive(p_full(g, part));
+        }
+        if (ok && s.tiles > 0) {
+          ok = __all_sync(0xffffffffu, bar_wait(o_done(g, 0), (done - 1) & 1, p.status) && bar_wait(o_done(g, 1), (done - 1) & 1, p.status));
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        }
+        pair_sync(pair);      // both have read what the other left
+        *my_xchg = way == kForMaxima ? best : highest == highest ? row.l : highest;
+        pair_sync(pair);
+        if (way == kForMaxima) {
+          best = fmaxf(best, *pair_xchg);
+          row.m = best == -INFINITY ? 0.f : ceilf(score_log2(best, sc));
+        } else {
+          row.l = *my_xchg + *pair_xchg;
+          if (way == kAsItComes && ok && row.live &&
+              !(row.l <= kSumLimit && (row.l * kSumLimit >= 1.f || !some) && highest <= kRound + 60.f))
+            flags[turn & 3] = 1;
+        }
+      } while (!last_passage());
+      if (row.l == 0.f) row.m = -INFINITY;      // nothing to put together with others
       // The row's sums: this slot's alone, half of the head to a warp, or, where both slots had the same rows, both slots',
       // a quarter of the head to a warp.
-      *my_xchg = row.l;
-      pair_sync(pair);
-      float m = row.m, l = row.l + *pair_xchg, mine = 1.f, other = 0.f;
+      float m = row.m, l = row.l, mine = 1.f, other = 0.f;
       int d0 = part * (D / 2), d1 = d0 + D / 2;
       if (!s.pair) {
-        pair_sync(pair);
         *my_xchg = part ? l : m;
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         both_slots_sync();
@@ -610,10 +689,8 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
         l = (l == 0.f ? 0.f : l * mine) + (l_other == 0.f ? 0.f : l_other * other);
         d0 = (g * 2 + part) * (D / 4);
         d1 = d0 + D / 4;
-      } else if (cluster > 1) {
-        both_slots_sync();      // the tiles' place, which the sums take, is the other slot's too
       }
-      const bool write = row.live && ok;
+      const bool write = row.live && ok, not_all_finite = flags[4 + (pieces & 3)] != 0;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const uint32_t o_other = tmem_o(g ^ 1) + lane_addr;
       float* left = reinterpret_cast<float*>(smem_raw + L::kSums) + unit_row * L::kPitch;
@@ -623,13 +700,37 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
         for (int c0 = d0; c0 < d1; c0 += 16) {
           float v[16], x[16];
           tmem_ld16(o_row + c0, v);
-          if (!s.pair) tmem_ld16(o_other + c0, x);
-          tmem_ld_wait();
+          if (!s.pair) {
+            tmem_ld16(o_other + c0, x);
+            tmem_ld_wait16(x);
+          }
+          tmem_ld_wait16(v);
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
             v[c] = mine == 0.f ? 0.f : v[c] * mine;
             if (!s.pair && other != 0.f) v[c] += x[c] * other;
           }
+          if (not_all_finite && row.live) {
+            // the values that were cleared, for the rows that see their keys, times a weight above zero
+            const __nv_bfloat16* values = static_cast<const __nv_bfloat16*>(p.v_cache) + (size_t)u.kv_head * p.page_size * D + c0;
+            const int keys_end = min(w.t.cached + w.t.nodes, w.t.begin + w.tile_end * kTile);
+#pragma unroll 1
+            for (int key0 = w.t.begin + w.tile_begin * kTile; key0 < keys_end; key0 += 32) {
+              if (p.window == 0 && key0 + kTile <= w.t.cached) continue;      // its tile was not looked over
+#pragma unroll 1
+              for (uint32_t rest = tree_visible(p, w.t, row.token, row.lowest, row.position, key0); rest; rest &= rest - 1) {
+                const int key = key0 + __ffs(rest) - 1, page = p.block_table[(size_t)w.request * p.table_width + key / p.page_size];
+                if (page < 0 || page >= p.num_pages) continue;
+                const __nv_bfloat16* value = values + ((size_t)page * p.kv_heads * p.page_size + key % p.page_size) * D;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                  const float x = __bfloat162float(value[e]);
+                  if (!isfinite(x)) v[e] += x;
+                }
+              }
+            }
+          }
+          __syncwarp();
           if (write && cluster == 1 && w.whole) {
 #pragma unroll
             for (int d = 0; d < 16; d += 8)

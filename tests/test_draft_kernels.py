@@ -215,6 +215,28 @@ def test_scores_far_apart(dev, dtype, heads, kv_heads, size, page):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads, kv_heads, size, page", [(4, 2, 48, 4), (14, 2, 64, 16), (12, 2, 128, 16)])
+@pytest.mark.parametrize("nodes, cached", [([5], [700]), ([30, 3], [390, 1100])])
+def test_scores_that_rise_and_fall_along_the_keys(dev, dtype, heads, kv_heads, size, page, nodes, cached):
+    """One direction for all queries and keys, so that the scores are what is asked for: hundreds above those of the first keys
+    later on; hundreds below zero for all of them; the first tiles outside the window and the rest far below zero; one key at 9,000."""
+    def run(levels, **options):
+        case = Trees(dev, heads, kv_heads, size, page, nodes, cached, dtype, seed=6)
+        case.q[:] = 1.0
+        for r, (c, n) in enumerate(zip(cached, nodes)):
+            for j in range(c + n):
+                where, row = case.slot(r, j)
+                case.k[where, :, row] = torch.tensor(levels(j, c)).to(dtype).float().item() * size ** -0.5
+        case.check(case.run(**options), options.get("window"))
+
+    run(lambda j, c: -100.0 if j < 200 else 150.0 + j % 3)
+    run(lambda j, c: 150.0 if j < 200 else -100.0)
+    run(lambda j, c: -300.0 - j % 5)
+    run(lambda j, c: 40.0 if j < 300 else -250.0, window=200)
+    run(lambda j, c: 9000.0 if j == 350 else 8999.0 if j == 30 else 0.5 * (j % 7))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("size", [48, 128])
 def test_a_result_does_not_depend_on_the_call(dev, dtype, size):
     """The same call twice gives the same bits, on another stream and from a captured graph too."""
