@@ -2,21 +2,19 @@
 // and pages of 8 to 128 tokens.  What is computed and how a launch is cut into shares: attention_tree.cuh.
 //
 // A unit is up to two tiles of 128 rows (nodes x the query heads that share a key/value head) over the keys of
-// one request, 128 at a time.  The CTA has two slots, each a tile of rows with its own issuing warps, tensor memory and
-// two softmax warpgroups, one for either half of a tile's keys.  So four streams of scores, exponentials and sums are on their
-// way at once, and while one waits for the tensor core or for its scores the others have the units.  (With one stream a slot
-// both came to stand in step, exponentials against exponentials: 5,500 cycles for a tile of both slots at head size 128, of
-// which the tensor core had 2,200 and the exponentials' unit 2,048.)  A unit of two tiles gives each slot one of them, and every
-// tile of keys in shared memory serves both; a unit of one tile gives both slots the same rows and every second tile of
-// keys, and they are put together at the end.
+// one request, 128 at a time.  The CTA has two slots, each a tile of rows with its own issuing warp, tensor memory and
+// two softmax warpgroups, one for either half of a tile's keys.  The slots take turns: while one's threads are at their
+// exponentials the other's products have the tensor core.  A unit of two tiles gives each slot one of them, and every tile of keys in shared memory
+// serves both; a unit of one tile gives both slots the same rows and every second tile of keys, and they are put together at the
+// end.  (Scores half a tile at a time, the other half's in the making meanwhile, were no faster: twice the instructions
+// for the scores, which the issuing warps were slower to come by than the tensor core to carry out.)
 //
 //   warps 0, 1    K and V producers: TMA-load the pages that the block table names into rings of tiles
-//   warps 2, 3    issue a slot's products, each stream's as what they need arrives: S = Q K^T into tensor memory, half a
-//                 tile of keys at a time, and O += P V with P from there
+//   warps 2, 3    issue a slot's products: S = Q K^T into tensor memory, then O += P V with P from there, half by half
 //   warps 4-19    softmax: thread r of a warpgroup has row r of the slot's tile and 64 of a tile's 128 keys
 //
-// The streams agree on nothing while they run: a row's reference is a whole number at or above the maximum of its
-// first tile, and stays.  What that leaves to be done comes out at the end of a piece: a row with a sum of
+// The two warpgroups of a slot agree on nothing while they run: a row's reference is the maximum of its first tile,
+// and stays.  What that leaves to be done comes out at the end of a piece: a row with a sum of
 // weights above 2^60 (scores far above the reference; an overflow is such a sum too), or one that saw keys and has less
 // than 2^-60, sends the piece through again, once for the rows' maxima and once against those.
 //
@@ -33,7 +31,7 @@ constexpr int kTile = 128;                     // rows of a slot, keys of a tile
 constexpr int kSlice = kTile * 128;            // a [128 rows x 64] bfloat16 slice: 16 KB
 constexpr int kTreeThreads = 640;
 constexpr float kSumLimit = 1.15292150e18f;    // 2^60
-constexpr int kHalf = kTile / 2;               // keys of a stream
+constexpr int kHalf = kTile / 2;               // keys of a softmax thread
 constexpr int kTmemColumns = 512;              // S: 2 x 128 columns, O: 2 x D
 
 template <int D>
@@ -48,7 +46,7 @@ struct Layout {
   static constexpr int kK = kQ + 2 * kTileBytes;
   static constexpr int kV = kK + kKStages * kTileBytes;
   static constexpr int kBars = kV + kVStages * kTileBytes;
-  static constexpr int kNumBars = 14 + 3 * kKStages + 4 * kVStages;
+  static constexpr int kNumBars = 10 + 3 * kKStages + 4 * kVStages;
   static constexpr int kFlags = kBars + 8 * kNumBars + 8;      // to be done again (four, in turn), values that are not finite (four)
   static constexpr int kXchg = kFlags + 32;                    // a float for every thread of the softmax warps
   // what the CTAs of a cluster exchange, in the place of the Q, K and V tiles: the sums of 256 rows (padded so that neither
@@ -102,53 +100,14 @@ __device__ __forceinline__ void both_slots_sync() { asm volatile("bar.sync 1, 51
 // The two warps of a slot with the same rows meet.
 __device__ __forceinline__ void pair_sync(int pair) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(2 + pair) : "memory"); }
 
-__device__ __forceinline__ float max_or_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ float max3_or_nan(float a, float b, float c) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-
-// 2^x by fused multiply-adds, for the scores that the exponentials' unit (16 a cycle) is spared: x = n + f with n the nearest whole
-// number, |f| <= 1/2, and 2^f as a polynomial of the fourth degree whose largest relative error, 2.8e-6, is the least that one
-// with p(0) = 1 has.  n comes out of adding 1.5 x 2^23, which leaves it in the low bits, from where it is shifted onto the
-// exponent.  With a reference that is a whole number the reference and that constant are one exact addend, and a pair of scores
-// takes seven two-way operations.
-constexpr float kRound = 12582912.f;                // 1.5 x 2^23
-constexpr float kLargestReference = 8192.f;         // up to here n and f come out exact enough
-constexpr int kShared = 3;                          // of eight pairs: 1,280 cycles of either kind for a tile of both slots
-
-// 16 scores of a row to 2^(scale s - m): packed, and added to `sum`.  `highest` is the largest kRound + n that was shifted,
-// or NaN if a score is; what lies above the type's exponents has come out wrong.
-__device__ __forceinline__ void shared_exps(const float* v, uint32_t* packed, float scale, float m, float2* sum, float* highest) {
-  const float2 scale2 = make_float2(scale, scale), shift2 = make_float2(-m, -m), base2 = make_float2(kRound - m, kRound - m);
-  const float2 c1 = make_float2(6.9312412e-1f, 6.9312412e-1f), c2 = make_float2(2.4024107e-1f, 2.4024107e-1f);
-  const float2 c3 = make_float2(5.5906828e-2f, 5.5906828e-2f), c4 = make_float2(9.5825763e-3f, 9.5825763e-3f);
-  const float2 one2 = make_float2(1.f, 1.f), minus2 = make_float2(-1.f, -1.f);
-  const float lowest = __fdividef(m - 126.75f, scale);     // weights below 2^-126.75 count as that
+// 16 scores of a row to 2^(scale s - m): packed, and added to `sum`.  (Taken from the exponentials' unit, 16 a cycle, three of
+// eight by a polynomial of the fourth degree made tree-sized launches 4 per cent slower: while a slot's threads are at this the
+// other slot's products run, and it is the way from scores to weights, not the unit, that a tile waits for.)
+__device__ __forceinline__ void exps(const float* v, uint32_t* packed, float2 scale2, float2 shift2, float2* sum) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float2 s = make_float2(v[2 * i], v[2 * i + 1]);
-    float2 e;
-    if (i * kShared % 8 < kShared) {
-      const float2 bound = make_float2(max_or_nan(s.x, lowest), max_or_nan(s.y, lowest));
-      const float2 t = __ffma2_rn(bound, scale2, base2);              // kRound + n
-      *highest = max3_or_nan(*highest, t.x, t.y);
-      const float2 f = __ffma2_rn(bound, scale2, __ffma2_rn(t, minus2, base2));
-      float2 y = __ffma2_rn(f, c4, c3);
-      y = __ffma2_rn(y, f, c2);
-      y = __ffma2_rn(y, f, c1);
-      y = __ffma2_rn(y, f, one2);
-      e.x = __uint_as_float((__float_as_uint(t.x) << 23) + __float_as_uint(y.x));
-      e.y = __uint_as_float((__float_as_uint(t.y) << 23) + __float_as_uint(y.y));
-    } else {
-      const float2 x = __ffma2_rn(s, scale2, shift2);
-      e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-    }
+    const float2 x = __ffma2_rn(make_float2(v[2 * i], v[2 * i + 1]), scale2, shift2);
+    const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
     *sum = __fadd2_rn(*sum, e);
     packed[i] = pack_pair(e.x, e.y);
   }
@@ -251,14 +210,14 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
   }
   const uint32_t bars = base + L::kBars;
   auto q_full = [&](int g) { return bars + 8u * g; };
-  auto s_full = [&](int g, int h) { return bars + 8u * (2 + 2 * g + h); };
-  auto p_full = [&](int g, int h) { return bars + 8u * (6 + 2 * g + h); };
-  auto o_done = [&](int g, int h) { return bars + 8u * (10 + 2 * g + h); };
-  auto k_full = [&](int s) { return bars + 8u * (14 + s); };
-  auto k_empty = [&](int g, int s) { return bars + 8u * (14 + (1 + g) * L::kKStages + s); };
-  auto v_full = [&](int s) { return bars + 8u * (14 + 3 * L::kKStages + s); };
-  auto v_checked = [&](int s) { return bars + 8u * (14 + 3 * L::kKStages + L::kVStages + s); };
-  auto v_empty = [&](int g, int s) { return bars + 8u * (14 + 3 * L::kKStages + (2 + g) * L::kVStages + s); };
+  auto s_full = [&](int g) { return bars + 8u * (2 + g); };
+  auto p_full = [&](int g, int h) { return bars + 8u * (4 + 2 * g + h); };
+  auto o_done = [&](int g) { return bars + 8u * (8 + g); };
+  auto k_full = [&](int s) { return bars + 8u * (10 + s); };
+  auto k_empty = [&](int g, int s) { return bars + 8u * (10 + (1 + g) * L::kKStages + s); };
+  auto v_full = [&](int s) { return bars + 8u * (10 + 3 * L::kKStages + s); };
+  auto v_checked = [&](int s) { return bars + 8u * (10 + 3 * L::kKStages + L::kVStages + s); };
+  auto v_empty = [&](int g, int s) { return bars + 8u * (10 + 3 * L::kKStages + (2 + g) * L::kVStages + s); };
   const uint32_t tmem_holder = bars + 8 * L::kNumBars;
   volatile int* flags = reinterpret_cast<volatile int*>(smem_raw + L::kFlags);      // [4] to be done again, [4] values that are not finite
   float* xchg = reinterpret_cast<float*>(smem_raw + L::kXchg);              // [slot][half of the keys][row]
@@ -267,11 +226,10 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
   if (threadIdx.x == 0) {
     for (int g = 0; g < 2; ++g) {
       bar_init(q_full(g), 1);
-      for (int h = 0; h < 2; ++h) {
-        bar_init(s_full(g, h), 1);
-        bar_init(p_full(g, h), 128);
-        bar_init(o_done(g, h), 1);
-      }
+      bar_init(s_full(g), 1);
+      bar_init(p_full(g, 0), 128);
+      bar_init(p_full(g, 1), 128);
+      bar_init(o_done(g), 1);
       for (int s = 0; s < L::kKStages; ++s) bar_init(k_empty(g, s), 1);
       for (int s = 0; s < L::kVStages; ++s) bar_init(v_empty(g, s), 1);
     }
@@ -443,19 +401,20 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
   } else if (warp < 4) {
     // ---- a slot's products: the whole warp goes the way of the lane that issues, so that addresses stay in uniform registers ----
     const int g = warp - 2;
-    // S: M = 128 rows, N = 64 keys, both K-major.  O: M = 128, N = D, P from tensor memory, V MN-major.
-    constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kHalf >> 3) << 17) | ((128u >> 4) << 24);
+    // S: M = 128 rows, N = 128 keys, both K-major.  O: M = 128, N = D, P from tensor memory, V MN-major.
+    constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kTile >> 3) << 17) | ((128u >> 4) << 24);
     constexpr uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
     const uint64_t desc_q = desc_k_major(base + L::kQ + g * L::kTileBytes);
     auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, bar_wait_likely_done(bar, parity, p.status)) != 0; };
-    auto there = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, bar_test(bar, parity)) != 0; };
     bool ok = true;
     int queries = 0;               // loads of Q so far
-    int done = 0;                  // this slot's tiles so far
+    int done = 0, other_done = 0;  // this slot's tiles so far, and the other's before this passage
     int before = 0;                // the CTA's tiles before this passage
     for (; any; next_piece()) {
       const TreeUnit u = tree_unit(p, w.t, w.unit);
       const Slot s = slot_of(w, u, g);
+      const int other_tiles = slot_of(w, u, g ^ 1).tiles;
+      const bool turns = s.tiles > 1 || other_tiles > 1;
       if (s.tiles > 0 && ok) {
         if (elect_one()) {
           bar_expect_tx(q_full(g), (uint32_t)(p.unit_nodes / 2 * u.heads) * 128u * L::kBlocks);
@@ -470,64 +429,55 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
       do {
         const int first = before + s.first_tile - w.tile_begin;
         before += w.tile_end - w.tile_begin;
-        // per stream: tiles whose scores, and whose sums, have been issued
-        int scored[2] = {0, 0}, summed[2] = {0, 0}, polls = 0;
-        while (ok && (summed[0] < s.tiles || summed[1] < s.tiles)) {
-          bool progress = false;
+#pragma unroll 1
+        for (int j = 0; j < s.tiles && ok; ++j, ++done) {
+          const int c = first + j * s.step, k_stage = c % L::kKStages, v_stage = c % L::kVStages;
+          // The slots take turns, so that one's exponentials meet the other's products: slot 1's scores wait for slot 0's
+          // probabilities, slot 0's next scores for slot 1's.  (Each lets the other go one tile, so no phase is missed.)  Left to
+          // themselves they fall into step and have their exponentials at the same time: 286 us against 246 for 32 requests
+          // of 8,192 keys and 64 nodes.  Where neither has a second tile there is nothing to gain: 11.0 us without, 12.2 with
+          // turns for one request of 1,024 keys.
+          if (g) ok = !turns || (wait(p_full(0, 0), (other_done + j) & 1) && wait(p_full(0, 1), (other_done + j) & 1));
+          else if (turns && j > 0 && j <= other_tiles) ok = wait(s_full(1), (other_done + j - 1) & 1);
+          ok = ok && wait(k_full(k_stage), (c / L::kKStages) & 1);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          if (elect_one()) {
+            const uint64_t desc_k = desc_k_major(base + L::kK + k_stage * L::kTileBytes);
+#pragma unroll
+            for (int db = 0; db < L::kBlocks; ++db)
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                mma_ss(tmem_s(g, 0), desc_advance(desc_q, db * kSlice + kk * 32), desc_advance(desc_k, db * kSlice + kk * 32), idesc_s,
+                       (db > 0 || kk > 0) ? 1u : 0u);
+            mma_commit(s_full(g));
+            mma_commit(k_empty(g, k_stage));
+          }
+          __syncwarp();
+          const uint32_t parity = (c / L::kVStages) & 1;
+          ok = wait(v_full(v_stage), parity) && wait(v_checked(v_stage), parity);
+          const uint64_t desc_v = desc_mn_major(base + L::kV + v_stage * L::kTileBytes, kSlice);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            // sums, onto the zeros or sums that are there
-            const int v_tile = first + summed[h] * s.step, v_stage = v_tile % L::kVStages;
-            const uint32_t v_parity = (v_tile / L::kVStages) & 1;
-            if (summed[h] < scored[h] && there(p_full(g, h), (done + summed[h]) & 1) && there(v_full(v_stage), v_parity) &&
-                there(v_checked(v_stage), v_parity)) {
-              const int j = summed[h], stage = v_stage;
-              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-              if (elect_one()) {
-                const uint64_t desc_v = desc_mn_major(base + L::kV + stage * L::kTileBytes + h * kHalf * 128, kSlice);
+            ok = ok && wait(p_full(g, h), done & 1);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (elect_one()) {
 #pragma unroll
-                for (int ks = 0; ks < kHalf / 16; ++ks)
-                  mma_ts(tmem_o(g), tmem_s(g, h) + ks * 8, desc_advance(desc_v, ks * 16 * 128), idesc_o, 1u);
-                mma_commit(o_done(g, h));
-                if (summed[h ^ 1] > j) mma_commit(v_empty(g, stage));      // the other half is through too
-              }
-              __syncwarp();
-              summed[h] = j + 1;
-              progress = true;
-            }
-            // scores; their place holds the probabilities of the tile before until the product has them
-            if (scored[h] < s.tiles && scored[h] == summed[h] &&
-                (scored[h] == 0 || there(o_done(g, h), (done + scored[h] - 1) & 1))) {
-              const int j = scored[h], c = first + j * s.step, stage = c % L::kKStages;
-              if (there(k_full(stage), (c / L::kKStages) & 1)) {
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (elect_one()) {
-                  const uint64_t desc_k = desc_k_major(base + L::kK + stage * L::kTileBytes + h * kHalf * 128);      // rows of 128 bytes
-#pragma unroll
-                  for (int db = 0; db < L::kBlocks; ++db)
-#pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                      mma_ss(tmem_s(g, h), desc_advance(desc_q, db * kSlice + kk * 32), desc_advance(desc_k, db * kSlice + kk * 32), idesc_s,
-                             (db > 0 || kk > 0) ? 1u : 0u);
-                  mma_commit(s_full(g, h));
-                  if (scored[h ^ 1] > j) mma_commit(k_empty(g, stage));
-                }
-                __syncwarp();
-                scored[h] = j + 1;
-                progress = true;
+              for (int ks = 0; ks < kHalf / 16; ++ks)      // onto the zeros or sums that are there
+                mma_ts(tmem_o(g), tmem_s(g, h) + ks * 8, desc_advance(desc_v, (h * kHalf + ks * 16) * 128), idesc_o, 1u);
+              if (h) {
+                mma_commit(o_done(g));
+                mma_commit(v_empty(g, v_stage));
               }
             }
+            __syncwarp();
           }
-          if (progress) {
-            polls = 0;
-          } else if (++polls > kPolls) {
-            if (lane == 0) atomicOr(p.status, kStatusWaitExpired);
-            ok = false;
-          }
+          // The scores' place holds the probabilities until the product has them; after the last, Q's place and the sums are
+          // free too.
+          ok = ok && wait(o_done(g), done & 1);
         }
-        done += s.tiles;
-        // the products are complete: Q's place, and the sums, are free
-        if (s.tiles > 0) ok = ok && wait(o_done(g, 0), (done - 1) & 1) && wait(o_done(g, 1), (done - 1) & 1);
+        other_done += other_tiles;
       } while (!last_passage());
     }
   } else {
@@ -555,8 +505,8 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
       // keys that every row of the warp sees, but for those from the drafted ones on
       const int all_from = p.window > 0 ? __reduce_max_sync(0xffffffffu, row.lowest) : 0;
       do {
-        float highest = kRound, best = -INFINITY;
-        bool some = false, cheap = false;      // the row has seen a key; the warp's references allow shared_exps
+        float best = -INFINITY;
+        bool some = false;      // the row has seen a key
         row.l = 0.f;
         if (s.tiles > 0 && warp_live) {
           uint32_t zero[16];
@@ -567,11 +517,10 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
           tmem_st_wait();
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           pair_sync(pair);      // the first product of either half finds all of the row's zeros
-          cheap = __all_sync(0xffffffffu, !row.live || fabsf(row.m) <= kLargestReference) && sc.tanh_in == 0.f;
         }
 #pragma unroll 1
         for (int j = 0; j < s.tiles; ++j, ++done) {      // `done` counts this slot's tiles
-          if (ok) ok = __all_sync(0xffffffffu, bar_wait_likely_done(s_full(g, part), done & 1, p.status));
+          if (ok) ok = __all_sync(0xffffffffu, bar_wait_likely_done(s_full(g), done & 1, p.status));
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           if (warp_live) {
             const int key0 = w.t.begin + (s.first_tile + j * s.step) * kTile + part * kHalf;
@@ -608,24 +557,24 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
               }
               best = fmaxf(best, top);
               if (way == kAsItComes) {
-                // The row's reference: whole, at or above the maximum of the tile (the scale is positive and the cap grows with
-                // the score: the maximum and either commute); nothing where the row sees none of it.
+                // The row's reference: the maximum of the tile (the scale is positive and the cap grows with the score: the
+                // maximum and either commute); nothing where the row sees none of it.
                 *my_xchg = best;
                 pair_sync(pair);
                 best = fmaxf(best, *pair_xchg);
-                row.m = best == -INFINITY ? 0.f : ceilf(score_log2(best, sc));
-                cheap = __all_sync(0xffffffffu, !row.live || fabsf(row.m) <= kLargestReference) && sc.tanh_in == 0.f;
+                row.m = best == -INFINITY ? 0.f : score_log2(best, sc);
               }
             }
             const float2 scale2 = make_float2(sc.scale_log2, sc.scale_log2), shift2 = make_float2(-row.m, -row.m);
             float2 sum2 = make_float2(0.f, 0.f);
-            if (all_visible && cheap && way != kForMaxima) {
+            if (all_visible && sc.tanh_in == 0.f && way != kForMaxima) {
 #pragma unroll 1
               for (int c0 = 0; c0 < kHalf; c0 += 16) {
                 float v[16];
                 uint32_t packed[8];
-                scores(c0, v, false);
-                shared_exps(v, packed, sc.scale_log2, row.m, &sum2, &highest);
+                tmem_ld16(s_row + c0, v);
+                tmem_ld_wait16(v);
+                exps(v, packed, scale2, shift2, &sum2);
                 tmem_st8(s_row + (c0 >> 1), packed);      // two keys to a column, over scores that were read
               }
             } else {
@@ -639,13 +588,7 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
 #pragma unroll
                   for (int c = 0; c < 16; ++c) v[c] = v[c] == -INFINITY ? -INFINITY : __fdividef(capped(v[c], sc), sc.scale_log2);
                 }
-#pragma unroll
-                for (int c = 0; c < 16; c += 2) {
-                  const float2 x = __ffma2_rn(make_float2(v[c], v[c + 1]), scale2, shift2);
-                  const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-                  sum2 = __fadd2_rn(sum2, e);
-                  packed[c >> 1] = pack_pair(e.x, e.y);
-                }
+                exps(v, packed, scale2, shift2, &sum2);
                 tmem_st8(s_row + (c0 >> 1), packed);
               }
             }
@@ -656,19 +599,18 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
           bar_arrive(p_full(g, part));
         }
         if (ok && s.tiles > 0) {
-          ok = __all_sync(0xffffffffu, bar_wait(o_done(g, 0), (done - 1) & 1, p.status) && bar_wait(o_done(g, 1), (done - 1) & 1, p.status));
+          ok = __all_sync(0xffffffffu, bar_wait(o_done(g), (done - 1) & 1, p.status));
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         }
         pair_sync(pair);      // both have read what the other left
-        *my_xchg = way == kForMaxima ? best : highest == highest ? row.l : highest;
+        *my_xchg = way == kForMaxima ? best : row.l;
         pair_sync(pair);
         if (way == kForMaxima) {
           best = fmaxf(best, *pair_xchg);
-          row.m = best == -INFINITY ? 0.f : ceilf(score_log2(best, sc));
+          row.m = best == -INFINITY ? 0.f : score_log2(best, sc);
         } else {
           row.l = *my_xchg + *pair_xchg;
-          if (way == kAsItComes && ok && row.live &&
-              !(row.l <= kSumLimit && (row.l * kSumLimit >= 1.f || !some) && highest <= kRound + 60.f))
+          if (way == kAsItComes && ok && row.live && !(row.l <= kSumLimit && (row.l * kSumLimit >= 1.f || !some)))
             flags[turn & 3] = 1;
         }
       } while (!last_passage());
