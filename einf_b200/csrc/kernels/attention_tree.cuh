@@ -7,7 +7,7 @@
 //
 // The rows of a unit are those of some nodes x the query heads that share one key/value head, so that a tile of keys is
 // read once for all of them; with trees of 8 to 64 nodes that is what makes the work more than a read of the cache.  A
-// worker is a CTA or a thread-block cluster.  A launch's work is cut over its workers in one of three ways:
+// worker is a CTA or, where every unit has a worker, a thread-block cluster.  A launch's work is cut over its workers in one of three ways:
 //   whole    a unit to a worker (a cluster shares its key tiles out among its CTAs), nothing is put together afterwards
 //   aligned  no more units than workers: a unit is cut into pieces of `chunk` key tiles, a piece to a worker
 //   list     more units than workers: worker w takes an equal piece of the list of all (unit, key tile) pairs, in the order
@@ -358,6 +358,10 @@ constexpr int kTreeMergeShares = 4;        // shares that a warp has in flight
 // their keys.  blockIdx.x stands for the place where a worker's list ends and the next one's begins; the places inside one
 // unit share its work out: an item is 32 rows, one a lane, and eight elements of each, which lie as 2 x 512 bytes in a
 // share.  Loops stay rolled: the kernel runs for a few microseconds, and its instructions come at the pace of their first fetch.
+// What bounds it is the latency of loads that follow one another: with the shares of an item split among a CTA's four
+// warps where there are CTAs for that, 38 shares of 256 rows x 128 (17 MB, out of the L2) took 5.5 us instead of 9.5, 9 of 96
+// x 128 3.8 instead of 4.3.  (Eight warps, or eight shares of a warp in flight, were no faster where it matters: 37.2 us for 38.0
+// of the former's two launches, 18.7 for 17.1 of the latter's.)
 template <typename T>
 __global__ void __launch_bounds__(32 * kTreeMergeWarps) tree_merge_kernel(TreeParams p) {
   pdl_launch_dependents();
@@ -366,18 +370,21 @@ __global__ void __launch_bounds__(32 * kTreeMergeWarps) tree_merge_kernel(TreePa
   if (n.places == 0) return;                             // no unit is cut here
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int first = blockIdx.x - n.place, rows = n.nodes * n.heads, groups = p.padded >> 2;
-  for (int item = (blockIdx.y * kTreeMergeWarps + warp) * n.places + n.place;; item += n.places * gridDim.y * kTreeMergeWarps) {
-    const int row_block = divide(2 * item, groups), row = row_block * 32 + lane, group = 2 * item - row_block * groups;
-    if (row_block * 32 >= rows) break;
-    if (row >= rows) continue;
-    const float2* ml = p.part_ml + row;
+  // With a CTA for every item (a unit in many pieces) an item's shares are split among the CTA's warps, else a warp has an item.
+  const int pairs = (groups + 1) >> 1, items = ((rows + 31) >> 5) * pairs;
+  const bool together = n.places * (int)gridDim.y >= items;
+  const int item0 = together ? blockIdx.y * n.places + n.place : (blockIdx.y * kTreeMergeWarps + warp) * n.places + n.place;
+  __shared__ float left[kTreeMergeWarps - 1][10][32];      // what a warp has of the item: reference, sum, eight sums of values
+  for (int item = item0; item < items; item += n.places * gridDim.y * kTreeMergeWarps) {
+    const int row_block = divide(item, pairs), row = row_block * 32 + lane, group = 2 * (item - row_block * pairs);
+    const float2* ml = p.part_ml + min(row, rows - 1);
     const float4* sums = reinterpret_cast<const float4*>(p.part_o) + ((size_t)row_block * groups + group) * 32 + lane;
     const size_t share_rows = (size_t)p.unit_rows, share_sums = (size_t)(p.unit_rows >> 5) * groups * 32;
     const bool two = group + 1 < groups;
     float m = -INFINITY, l = 0.f;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
 #pragma unroll 1
-    for (int c0 = 0; c0 <= n.places; c0 += kTreeMergeShares) {
+    for (int c0 = together ? warp * kTreeMergeShares : 0; c0 <= n.places; c0 += together ? kTreeMergeWarps * kTreeMergeShares : kTreeMergeShares) {
       float2 v[kTreeMergeShares];
       float4 x[kTreeMergeShares], y[kTreeMergeShares];
       // all of these in flight at once; what lies beyond the last share is the last one again
@@ -407,6 +414,30 @@ __global__ void __launch_bounds__(32 * kTreeMergeWarps) tree_merge_kernel(TreePa
         b.x = fmaf(y[i].x, f, b.x), b.y = fmaf(y[i].y, f, b.y), b.z = fmaf(y[i].z, f, b.z), b.w = fmaf(y[i].w, f, b.w);
       }
     }
+    if (together) {
+      if (warp) {
+        float(*mine)[32] = left[warp - 1];
+        mine[0][lane] = m, mine[1][lane] = l;
+        mine[2][lane] = a.x, mine[3][lane] = a.y, mine[4][lane] = a.z, mine[5][lane] = a.w;
+        mine[6][lane] = b.x, mine[7][lane] = b.y, mine[8][lane] = b.z, mine[9][lane] = b.w;
+      }
+      __syncthreads();      // once at most in a CTA: it has one item then
+      if (warp) return;
+#pragma unroll 1
+      for (int o = 0; o < kTreeMergeWarps - 1; ++o) {
+        const float(*x)[32] = left[o];
+        const float top = fmaxf(m, x[0][lane]), keep = m == -INFINITY ? 0.f : fast_exp2(m - top);
+        const float f = x[0][lane] == -INFINITY ? 0.f : fast_exp2(x[0][lane] - top);
+        m = top;
+        l = (l == 0.f ? 0.f : l * keep) + (x[1][lane] == 0.f ? 0.f : x[1][lane] * f);
+        // a share without a reference has nothing in its sums
+        a.x = fmaf(x[2][lane], f, a.x * keep), a.y = fmaf(x[3][lane], f, a.y * keep);
+        a.z = fmaf(x[4][lane], f, a.z * keep), a.w = fmaf(x[5][lane], f, a.w * keep);
+        b.x = fmaf(x[6][lane], f, b.x * keep), b.y = fmaf(x[7][lane], f, b.y * keep);
+        b.z = fmaf(x[8][lane], f, b.z * keep), b.w = fmaf(x[9][lane], f, b.w * keep);
+      }
+    }
+    if (row >= rows) continue;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int node = divide(row, n.heads), d = 4 * group;
     T* out = static_cast<T*>(p.out) + ((size_t)(n.token + node) * p.heads + n.first_head + row - node * n.heads) * p.size + d;

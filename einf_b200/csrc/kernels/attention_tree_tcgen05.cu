@@ -157,15 +157,12 @@ __device__ __forceinline__ void merge_cluster(const TreeParams& p, const TreeWal
       sum.z += o.z * fc;
       sum.w += o.w * fc;
     }
-    if (4 * lane < D && w.whole) {
+    if (4 * lane < D) {
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const int node = divide(row, u.heads);
       __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) +
           ((size_t)(w.t.first + u.first_node + node) * p.heads + u.first_head + row - node * u.heads) * D + 4 * lane;
       *reinterpret_cast<uint2*>(dst) = make_uint2(pack_pair(sum.x * inv, sum.y * inv), pack_pair(sum.z * inv, sum.w * inv));
-    } else if (4 * lane < D) {
-      *reinterpret_cast<float4*>(tree_share(p, w.share, row, 4 * lane)) = sum;
-      if (lane == 0) p.part_ml[(size_t)w.share * p.unit_rows + row] = make_float2(m, l);
     }
     __syncwarp();
   }
@@ -769,12 +766,12 @@ extern "C" int einf_tree_attention_tcgen05_max_clusters(int cluster) {
   return clusters;
 }
 
-// call: a TreeCall, on the host; a worker is a cluster of 1 to 8 CTAs.  part_o: [2 * workers][256][size] floats, part_ml:
+// call: a TreeCall, on the host; a worker is a CTA or, where every unit has a worker, a cluster of up to 8.  part_o: [2 * workers][256][size] floats, part_ml:
 // [2 * workers][256][2], notes: [workers][8]; none of them where every unit has one worker (whole).
 extern "C" int einf_tree_attention_tcgen05(const char* call, cudaStream_t stream) {
   const TreeCall& c = *reinterpret_cast<const TreeCall*>(call);
   if (c.requests == 0 || c.tokens == 0) return 0;
-  if (!tree_call_fits(c) || c.cluster > 8 || c.dtype != kBFloat16 || (c.size != 64 && c.size != 128) || c.heads / c.kv_heads > kTile ||
+  if (!tree_call_fits(c) || c.cluster > 8 || (c.cluster > 1 && !c.whole) || c.dtype != kBFloat16 || (c.size != 64 && c.size != 128) || c.heads / c.kv_heads > kTile ||
       c.page_size < 8 || c.page_size > 128 || (c.page_size & (c.page_size - 1)) ||
       ((uintptr_t)c.q | (uintptr_t)c.k_cache | (uintptr_t)c.v_cache | (uintptr_t)c.out) % 16)
     return (int)cudaErrorInvalidValue;

@@ -3566,28 +3566,31 @@ def tree_cluster_room(cluster: int) -> int:
     return _tree_room[key]
 
 
-def _tree_workers(units: int, tiles: int, sms: int, room) -> tuple[int, int, bool]:
-    """Workers, CTAs of a worker, and whether every unit has a worker of its own, for that many units of up to so many key tiles
-    each: what takes the least time, by a tile's and a launch's (see the table in attention_tree_tcgen05.cu)."""
-    best = None
+#: microseconds of a key tile, for a unit of one tile of rows and of two; of putting a cluster's shares together; of the second
+#: launch, which puts workers' shares together
+TREE_TILE_US, TREE_CLUSTER_US, TREE_MERGE_US = (1.3, 2.4), 3.5, 4.7
+
+
+def _tree_workers(units: int, tiles: int, two: bool, sms: int, room) -> tuple[int, int, bool]:
+    """Workers, CTAs of a worker, and whether every unit has a worker of its own, for ``units`` of up to ``tiles`` key tiles and
+    one tile of rows or ``two``.
+
+    A unit has a worker of its own, of 1 to 8 CTAs that put their shares together in shared memory, or all units' tiles are laid end
+    to end and cut into a run for each SM, with a second launch that puts the shares together.  The first is right while
+    there are few tiles, the second where whole units leave SMs idle; the constants above tell them apart.  Measured, in
+    microseconds: 2 units of 9 tiles 11.2 in clusters of eight, 12.3 in runs, 17.6 with a CTA each; 32 of 12 14.6 in clusters
+    of four, 16.1 in runs; 12 of 6 17.6, 21.1; 16 of 33 22.3 in clusters of four, 17.2 in runs; 4 of 257 98 in clusters
+    of eight, 38 in runs; 256 of 65 339 with a CTA each, 246 in runs."""
+    tile = TREE_TILE_US[two]
+    workers = min(room(1), sms)
+    each = -(-units * tiles // workers) if units > workers else max(TREE_MIN_TILES, -(-tiles // (workers // units)))
+    best = (tile * each + TREE_MERGE_US, min(workers, max(1, units * -(-tiles // TREE_MIN_TILES))), 1, False)
     for cluster in (1, 2, 4, 8):
-        workers = min(room(cluster), sms // cluster)
-        if workers < 1:
-            continue
-        if units <= workers:
-            cost = TREE_TILE_US * -(-tiles // cluster) + (TREE_CLUSTER_US if cluster > 1 else 0.0)
-            if best is None or cost < best[0]:
+        if units <= min(room(cluster), sms // cluster):
+            cost = tile * -(-tiles // cluster) + (TREE_CLUSTER_US if cluster > 1 else 0.0)
+            if cost < best[0]:
                 best = (cost, units, cluster, True)
-        if cluster in (1, 8) and (units > workers or tiles > TREE_MIN_TILES):
-            each = -(-units * tiles // workers) if units > workers else -(-tiles // (workers // units))
-            cost = TREE_TILE_US * -(-each // cluster) + (TREE_CLUSTER_US if cluster > 1 else 0.0) + TREE_MERGE_US
-            if best is None or cost < best[0]:
-                best = (cost, min(workers, max(1, units * -(-tiles // TREE_MIN_TILES))), cluster, False)
     return best[1:]
-
-
-#: microseconds of a key tile, of putting a cluster's shares together, of the second launch
-TREE_TILE_US, TREE_CLUSTER_US, TREE_MERGE_US = 2.2, 2.0, 6.0
 
 
 @functools.lru_cache(maxsize=4096)
@@ -3596,7 +3599,8 @@ def _tree_plan(tensor_cores: bool, device: int, requests: int, nodes: int, conte
     """The launcher; its workers, the CTAs of each, whether each has whole units; rows of all shares in scratch memory, elements of a row."""
     if tensor_cores:
         units = requests * kv_heads * -(-nodes // (2 * (TREE_TILE // group)))
-        workers, cluster, whole = _tree_workers(units, -(-context // TREE_TILE), _sm_count(), tree_cluster_room)
+        workers, cluster, whole = _tree_workers(units, -(-context // TREE_TILE), min(nodes, 2 * (TREE_TILE // group)) > TREE_TILE // group,
+                                                _sm_count(), tree_cluster_room)
         return "einf_tree_attention_tcgen05", workers, cluster, whole, 0 if whole else 2 * workers * 2 * TREE_TILE, size
     unit_heads = min(group, TREE_ROWS)
     units = requests * kv_heads * -(-group // unit_heads) * -(-nodes // (TREE_ROWS // unit_heads))
