@@ -9,7 +9,9 @@
 // 16-byte words of shared memory for 32 fused multiply-adds, so shared memory bounds the kernel at two thirds of
 // the FMA rate.  Keys that no row of a tile is kept from run without masks; in the other tiles a value is added
 // to the rows that see it and to no others, so that what stands in a masked place (a sibling's value, a row behind the
-// last node) may be anything.
+// last node) may be anything.  With few requests a CTA has two steps of keys, and the time is that of their loads one after the
+// other and of the second launch: 24.3 us for 2 requests of up to 700 keys and 13 nodes with 14 and 2 heads of 64 in float32, where
+// the bytes alone would take 0.2.
 #include "attention_tree.cuh"
 
 namespace einf {

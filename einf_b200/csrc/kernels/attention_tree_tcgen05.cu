@@ -4,10 +4,18 @@
 // A unit is up to two tiles of 128 rows (nodes x the query heads that share a key/value head) over the keys of
 // one request, 128 at a time.  The CTA has two slots, each a tile of rows with its own issuing warp, tensor memory and
 // two softmax warpgroups, one for either half of a tile's keys.  The slots take turns: while one's threads are at their
-// exponentials the other's products have the tensor core.  A unit of two tiles gives each slot one of them, and every tile of keys in shared memory
-// serves both; a unit of one tile gives both slots the same rows and every second tile of keys, and they are put together at the
-// end.  (Scores half a tile at a time, the other half's in the making meanwhile, were no faster: twice the instructions
-// for the scores, which the issuing warps were slower to come by than the tensor core to carry out.)
+// exponentials the other's products have the tensor core.  A unit of two tiles gives each slot one of them, and every
+// tile of keys in shared memory serves both; a unit of one tile gives both slots the same rows and every second tile of keys, and
+// they are put together at the end.  (Scores half a tile at a time, the other half's in the making meanwhile, were no faster:
+// 247 us against 233 below; twice the instructions for the scores, which the issuing warps were slower to come by than the
+// tensor core to carry out.)
+//
+// What bounds it: with many rows the way of a tile from scores to probabilities, 2.2 us for 256 rows x 128 keys x 128 of a head,
+// of which either the tensor core or the exponentials' unit needs half; with few the launch's start (2.5 us until the lengths
+// are known, 3 until the first scores are) and the second launch.  Measured in captured graphs with 28 query and 4
+// key/value heads of 128: 32 requests of up to 8,192 keys and 64 nodes 233 us, which is 0.59 PFLOP/s of the products that
+// count (268 to 276 after seconds without a pause, at the power limit); one of 32,768 keys and 32 nodes 36.5 us, 1.85 TB/s.  With 12 and 2 heads, 8 requests of
+// up to 4,096 keys and 16 nodes: 17.2 us.  With 14 and 2 of 64, one of 1,024 keys and 8 nodes: 10.9 us.
 //
 //   warps 0, 1    K and V producers: TMA-load the pages that the block table names into rings of tiles
 //   warps 2, 3    issue a slot's products: S = Q K^T into tensor memory, then O += P V with P from there, half by half
@@ -405,13 +413,11 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
     auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, bar_wait_likely_done(bar, parity, p.status)) != 0; };
     bool ok = true;
     int queries = 0;               // loads of Q so far
-    int done = 0, other_done = 0;  // this slot's tiles so far, and the other's before this passage
+    int done = 0;                  // this slot's tiles so far
     int before = 0;                // the CTA's tiles before this passage
     for (; any; next_piece()) {
       const TreeUnit u = tree_unit(p, w.t, w.unit);
       const Slot s = slot_of(w, u, g);
-      const int other_tiles = slot_of(w, u, g ^ 1).tiles;
-      const bool turns = s.tiles > 1 || other_tiles > 1;
       if (s.tiles > 0 && ok) {
         if (elect_one()) {
           bar_expect_tx(q_full(g), (uint32_t)(p.unit_nodes / 2 * u.heads) * 128u * L::kBlocks);
@@ -429,14 +435,7 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
 #pragma unroll 1
         for (int j = 0; j < s.tiles && ok; ++j, ++done) {
           const int c = first + j * s.step, k_stage = c % L::kKStages, v_stage = c % L::kVStages;
-          // The slots take turns, so that one's exponentials meet the other's products: slot 1's scores wait for slot 0's
-          // probabilities, slot 0's next scores for slot 1's.  (Each lets the other go one tile, so no phase is missed.)  Left to
-          // themselves they fall into step and have their exponentials at the same time: 286 us against 246 for 32 requests
-          // of 8,192 keys and 64 nodes.  Where neither has a second tile there is nothing to gain: 11.0 us without, 12.2 with
-          // turns for one request of 1,024 keys.
-          if (g) ok = !turns || (wait(p_full(0, 0), (other_done + j) & 1) && wait(p_full(0, 1), (other_done + j) & 1));
-          else if (turns && j > 0 && j <= other_tiles) ok = wait(s_full(1), (other_done + j - 1) & 1);
-          ok = ok && wait(k_full(k_stage), (c / L::kKStages) & 1);
+          ok = wait(k_full(k_stage), (c / L::kKStages) & 1);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           if (elect_one()) {
@@ -474,7 +473,6 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
           // free too.
           ok = ok && wait(o_done(g), done & 1);
         }
-        other_done += other_tiles;
       } while (!last_passage());
     }
   } else {
@@ -486,10 +484,12 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
     const float* pair_xchg = xchg + (g * 2 + (part ^ 1)) * 128 + r;
     const ScoreScale sc = make_score_scale(p.scale, p.softcap);
     bool ok = true;
-    int done = 0;
+    int done = 0, other_done = 0;      // this slot's tiles so far, and the other's before this passage
     for (; any; next_piece()) {
       const TreeUnit u = tree_unit(p, w.t, w.unit);
       const Slot s = slot_of(w, u, g);
+      const int other_tiles = slot_of(w, u, g ^ 1).tiles;
+      const bool turns = s.tiles > 1 || other_tiles > 1;
       const bool warp_live = (warp & 3) * 32 < s.rows;
       const int unit_row = s.first_node * u.heads + r;
       Row row;
@@ -517,6 +517,14 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
         }
 #pragma unroll 1
         for (int j = 0; j < s.tiles; ++j, ++done) {      // `done` counts this slot's tiles
+          // The turns: slot 1's exponentials wait for slot 0's of its tile, slot 0's for slot 1's of the one before.  (Neither
+          // gets ahead by more than a tile, so no phase is missed.)  Left to themselves the slots fall into step and have their
+          // exponentials at the same time, 286 us against 233 for 32 requests of 8,192 keys and 64 nodes; turns from score
+          // product to score product, by the issuing warps, took 244; passed on before the probabilities are all there,
+          // 244 to 306.  Where neither slot has a second tile there is nothing to gain: 11.0 us without, 12.2 with turns for
+          // one request of 1,024 keys.
+          if (warp_live && turns && ok && (g || (j > 0 && j <= other_tiles)))
+            ok = __all_sync(0xffffffffu, bar_wait_likely_done(p_full(g ^ 1, part), (other_done + j - (g ^ 1)) & 1, p.status));
           if (ok) ok = __all_sync(0xffffffffu, bar_wait_likely_done(s_full(g), done & 1, p.status));
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           if (warp_live) {
@@ -610,6 +618,7 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
           if (way == kAsItComes && ok && row.live && !(row.l <= kSumLimit && (row.l * kSumLimit >= 1.f || !some)))
             flags[turn & 3] = 1;
         }
+        other_done += other_tiles;
       } while (!last_passage());
       if (row.l == 0.f) row.m = -INFINITY;      // nothing to put together with others
       // The row's sums: this slot's alone, half of the head to a warp, or, where both slots had the same rows, both slots',
