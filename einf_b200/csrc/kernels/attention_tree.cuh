@@ -128,7 +128,7 @@ __device__ __forceinline__ TreeRequest tree_request(const TreeParams& p, int r) 
   TreeRequest t;
   t.first = max(0, min(p.q_start[r], p.tokens));
   t.nodes = max(0, min(p.q_start[r + 1], p.tokens) - t.first);
-  const long long room = (long long)p.table_width * p.page_size - t.nodes;
+  const long long room = min((long long)p.table_width * p.page_size, 1ll << 27) - t.nodes;      // (2^27: see divide)
   t.cached = p.cached_lens[r];
   if (t.nodes > 0 && (t.cached < 0 || t.cached > room)) {     // places that the block table does not have
     atomicOr(p.status, kStatusBadPage);

@@ -170,9 +170,9 @@ __device__ __forceinline__ ShapeRequest count_tokens(const ShapeParams& p, const
   return s;
 }
 
-// The places of the nodes' tokens.  `hits` takes the nodes whose tokens are the CTA's (room for as many as a mask has bits); then
-// (hit, row) pairs, a token that several nodes have at the first of them: the row's count is the request's and that of the hits with
-// this token on the row's path.
+// The places of the nodes' tokens.  `hits` takes the nodes whose tokens are the CTA's (room for as many as a mask has bits), and the
+// hits of one token are strung together, the lowest node first; then (hit, row) pairs, a token at its first hit: the row's count
+// is the request's and that of the hits with this token on the row's path.
 template <bool HAS_BIAS>
 __device__ __forceinline__ void shape_drafted(const ShapeParams& p, const Walk& w, const ShapeRequest& s, const uint32_t* words, int2* hits) {
   __shared__ int hit_count;
@@ -186,19 +186,32 @@ __device__ __forceinline__ void shape_drafted(const ShapeParams& p, const Walk& 
   }
   __syncthreads();
   const int count = hit_count;
+  // 12 bits: the node, 13 bits above: 1 + where the next hit of its token lies, or 0; the sign: it is not the first.  (What others
+  // look at, the node's bits, does not change.)
+  static_assert(64 * kMostWords <= 1 << 12, "a node in 12 bits");
+  volatile int* entries = reinterpret_cast<volatile int*>(hits);
+  for (int h = threadIdx.x; h < count; h += kShapeThreads) {
+    const int node = entries[2 * h] & 0xfff, token = entries[2 * h + 1];
+    int next = 0, next_node = 1 << 12, before = 0;
+    for (int other = 0; other < count; ++other) {
+      const int n = entries[2 * other] & 0xfff;
+      if (entries[2 * other + 1] != token) continue;
+      before |= n < node;
+      if (n > node && n < next_node) next = other + 1, next_node = n;
+    }
+    entries[2 * h] = node | next << 12 | (before ? 1 << 31 : 0);
+  }
+  __syncthreads();
   for (int item = threadIdx.x; item < count * w.rows; item += kShapeThreads) {
     const int n = item / count, row = w.first_row + n * (int)gridDim.z;
     const int2 hit = hits[item - n * count];
     const uint32_t* path = p.tree_mask + (size_t)row * 2 * p.words;
+    if (hit.x < 0) continue;
     int on_path = 0;
-    bool first = true;
-    for (int other = 0; other < count; ++other) {
-      const int2 h = hits[other];
-      if (h.y != hit.y) continue;
-      first = first && h.x >= hit.x;
-      on_path += path[h.x >> 5] >> (h.x & 31) & 1u;
+    for (int at = hit.x;; at = hits[(at >> 12 & 0x1fff) - 1].x) {
+      on_path += path[(at & 0xfff) >> 5] >> (at & 31) & 1u;
+      if (!(at >> 12 & 0x1fff)) break;
     }
-    if (!first) continue;
     const uint32_t entry = HAS_BIAS ? which[hit.y - w.v0] : 0u;
     float x = shaped(p.logits[(size_t)row * p.vocab + hit.y], words[hit.y - w.v0], on_path, s);
     if (entry) x += p.bias[(size_t)w.request * p.biases + entry - 1];

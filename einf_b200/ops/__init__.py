@@ -3637,7 +3637,7 @@ def tree_attention(
     stand at their request's cached length at least).  ``softcap`` as in :func:`paged_attention_generic`.  A node that sees
     nothing gets zeros, rows that belong to no request keep what they hold.
 
-    Scores, softmax and sums are 32-bit.  ``max_nodes`` and ``max_cached``, the most nodes and cached tokens of a request as
+    A request has up to 2^27 tokens, a launch up to 2^20 nodes x key/value heads.  Scores, softmax and sums are 32-bit.  ``max_nodes`` and ``max_cached``, the most nodes and cached tokens of a request as
     far as the caller knows them, only size the launch: any request's nodes are computed whole."""
     tokens, heads, size = q.shape
     num_pages, kv_heads, page_size, cache_size = k_cache.shape
@@ -3653,6 +3653,8 @@ def tree_attention(
         raise UnsupportedSize(f"tree attention takes heads of up to {MAX_HEAD_SIZE}, not {size}")
     if q_start.shape[0] != requests + 1 or table_rows < requests:
         raise ValueError(f"q_start must hold {requests + 1} entries and block_table a row for each of {requests} requests")
+    if tokens * kv_heads * -(-(heads // kv_heads) // TREE_ROWS) > 1 << 20:
+        raise UnsupportedSize(f"tree attention takes up to {1 << 20} nodes x key/value heads, not {tokens} x {kv_heads}")
     words = _mask_words(tree_mask, tokens)
     if not scale > 0:
         raise ValueError(f"the scale is positive, not {scale}")
@@ -3663,6 +3665,7 @@ def tree_attention(
             raise ValueError(f"a window holds at least one token, not {window}")
         if positions is None or positions.shape != (tokens,):
             raise ValueError("a window needs the position of every node")
+        window = min(window, (1 << 31) - 1)
     device, stream = _current()
     places = (
         _at(q, "q", dtype, device), _at(k_cache, "k_cache", dtype, device), _at(v_cache, "v_cache", dtype, device),
@@ -3867,6 +3870,9 @@ class CacheRows:
             _code(t)
             while _dev(t, "cache") % unit or t.shape[3] * t.element_size() % unit:
                 unit //= 2
+        ends = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in self.caches)
+        if any(end > start for (_, end), (start, _) in zip(ends, ends[1:])):      # threads of one would read what the other's wrote
+            raise ValueError("a cache tensor is given twice, or two of them share memory")
         self.unit = unit
         #: per launch: how many tensors, the unit, what the pages are, and each tensor's address, heads and units of a row
         self.parts = []
@@ -3886,7 +3892,8 @@ def move_accepted(caches: CacheRows, block_table: torch.Tensor, cached_lens: tor
     """Close the gaps that refused nodes leave in the cache: in every tensor of ``caches`` the row at place
     ``cached_lens[r] + path[r, i]`` of request ``r`` goes to place ``cached_lens[r] + i``, for ``i = 1 .. counts[r] - 1`` (all
     int32, as :func:`accept_drafts` writes them), as if every row were read before any is written.  A path's nodes rise; one
-    that does not, or a place without a page, sets the status word and is not moved."""
+    that does not, or a place without a page, sets the status word and is not moved.  The pages behind a request's cached
+    tokens are its own: no other request of the call has them."""
     (requests,), (path_rows, depth), (table_rows, width) = cached_lens.shape, path.shape, block_table.shape
     if path_rows != requests or counts.shape != cached_lens.shape:
         raise ValueError(f"path must be [{requests}, depth] and counts ({requests},)")

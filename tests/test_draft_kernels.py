@@ -268,6 +268,29 @@ def test_a_result_does_not_depend_on_the_call(dev, dtype, size):
     assert int(st) == 0 and all(torch.equal(first, out) for out in outs)
 
 
+@pytest.mark.parametrize("dtype, size", [(torch.float32, 20), (torch.bfloat16, 64)])
+def test_a_window_wider_than_any_context_is_none(dev, dtype, size):
+    from einf_b200 import ops
+
+    gen = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn(s, generator=gen).to(dtype).to(dev) for s in ((5, 4, size), (40, 2, 8, size), (40, 2, 8, size)))
+    mask = torch.tensor([[1], [3], [5], [11], [1]], dtype=torch.int64, device=dev)
+    outs = []
+    for window in (None, 1 << 40, (1 << 31) - 1):
+        out, st = torch.full_like(q, 3.0), status(dev)
+        ops.tree_attention(q, k, v, ints([list(range(40)), list(range(40))], dev), ints([0, 4, 5], dev), ints([300, 0], dev), mask, out, 0.2, st,
+                           positions=ints([300, 301, 301, 302, 0], dev), window=window)
+        assert int(st) == 0
+        outs.append(out.cpu())
+    assert outs[0].isfinite().all()
+    # the same keys, weighed in other orders: sums of up to 304 products in 32 bits, probabilities of bfloat16 rounded
+    # against other references (2^-8 each), outputs rounded once more (2^-8)
+    bound = 304 * 2.0 ** -24 if dtype == torch.float32 else 3 * 2.0 ** -8
+    top = float(v.float().abs().max())
+    for out in outs[1:]:
+        assert ((out.double() - outs[0].double()).abs() <= bound * top).all()
+
+
 def test_bad_pages_and_lengths_set_the_status_word(dev):
     from einf_b200 import ops
 
@@ -363,6 +386,15 @@ def test_shape_logits(dev, vocab, rows_of, capacity, biases, nodes, masks):
     want = shape(dev, case)
     check_logits(case, want)
     assert torch.equal(shape(dev, case, "in place"), want)
+
+
+@pytest.mark.parametrize("vocab", [2003, 2100])
+def test_shape_logits_of_many_nodes_with_few_tokens(dev, vocab):
+    """All hits of a token in one CTA, every node on some row's path."""
+    case = logits_case(dev, vocab, [700, 2], 20, seed=5, nodes=True, masks="shared")
+    case["node_tokens"] = case["node_tokens"] % 5
+    case["tree_mask"][::3] = -1
+    check_logits(case, shape(dev, case))
 
 
 def test_shape_logits_with_one_thing_alone(dev):

@@ -144,6 +144,24 @@ def test_accept_drafts_refuses(on_this_machine, change, error):
     assert on_this_machine == ["einf_accept_drafts"]
 
 
+def test_cache_rows_refuses_what_two_of_them_share(on_this_machine):
+    both = torch.zeros(2, 6, 2, 4, 8)
+    ops.CacheRows([both[1], both[0]])
+    for caches in ([both[0], both[0]], [both[0], both.view(-1)[8:8 + 6 * 2 * 4 * 8].view(6, 2, 4, 8)], [both[1], both[0], both.view(12, 2, 4, 8)[3:9]]):
+        with pytest.raises(ValueError, match="share memory"):
+            ops.CacheRows(caches)
+
+
+def test_tree_attention_of_the_widest_window_and_the_most_nodes(on_this_machine):
+    ops.tree_attention(**attention_arguments(window=1 << 40, positions=ints(5)))
+    assert on_this_machine == ["einf_tree_attention"]
+    many = (1 << 19) + 1
+    with pytest.raises(ops.UnsupportedSize):
+        ops.tree_attention(**attention_arguments(
+            q=torch.zeros(many, 2, 1), out=torch.zeros(many, 2, 1), k_cache=torch.zeros(6, 2, 4, 1), v_cache=torch.zeros(6, 2, 4, 1),
+            tree_mask=torch.zeros(many, 1, dtype=torch.int64)))
+
+
 def test_cache_rows_refuses(on_this_machine):
     good = [torch.zeros(6, 2, 4, 8), torch.zeros(6, 1, 4, 3, dtype=torch.bfloat16)]
     assert ops.CacheRows(good[:1]).unit == 16 and ops.CacheRows(good).unit == 2
@@ -161,7 +179,7 @@ def test_cache_rows_refuses(on_this_machine):
     (dict(path=torch.zeros(2, 4, dtype=torch.int64)), TypeError),
 ])
 def test_move_accepted_refuses(on_this_machine, change, error):
-    caches = ops.CacheRows([torch.zeros(6, 2, 4, 8)] * 200)
+    caches = ops.CacheRows([torch.zeros(6, 2, 4, 8) for _ in range(200)])
     given = dict(caches=caches, block_table=ints(2, 2), cached_lens=ints(2), path=ints(2, 4), counts=ints(2), status=ints(1))
     ops.move_accepted(**given)
     assert on_this_machine == ["einf_move_accepted"] * 2      # 200 tensors: two launches
