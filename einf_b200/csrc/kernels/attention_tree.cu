@@ -13,6 +13,7 @@
 // other and of the second launch: 24.3 us for 2 requests of up to 700 keys and 13 nodes with 14 and 2 heads of 64 in float32, where
 // the bytes alone would take 0.2.
 #include "attention_tree.cuh"
+#include "mma_sync.cuh"
 
 namespace einf {
 
@@ -20,16 +21,21 @@ constexpr int kKeys = 32;
 constexpr int kWarps = 4;
 constexpr int kRowsPerWarp = 8;
 constexpr int kRows = kWarps * kRowsPerWarp;
+constexpr int kPitch = kKeys + 4;      // of a row's probabilities: four lanes a row meet no bank twice
+static_assert(kKeys == 32 && kRowsPerWarp == 8, "four lanes a row, eight keys a lane");
 
 __device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 __device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
   const uint2 v = *reinterpret_cast<const uint2*>(p);
   return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
 }
-// Four elements of a row from d on; zeros behind its end.
+__device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
+__device__ __forceinline__ void store4(__nv_bfloat16* p, float4 v) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_pair(v.x, v.y), pack_pair(v.z, v.w));
+}
+// Four elements of a row from d on, wherever it starts; zeros behind its end.
 template <typename T>
-__device__ __forceinline__ float4 elements(const T* row, int d, int size, bool aligned) {
-  if (aligned) return load4(row + d);
+__device__ __forceinline__ float4 elements(const T* row, int d, int size) {
   return make_float4(d < size ? to_float(row[d]) : 0.f, d + 1 < size ? to_float(row[d + 1]) : 0.f, d + 2 < size ? to_float(row[d + 2]) : 0.f,
                      d + 3 < size ? to_float(row[d + 3]) : 0.f);
 }
@@ -42,7 +48,7 @@ __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams 
   float* ks = smem;                                 // [keys][pitch]
   float* vs = ks + kKeys * pitch;                   // [keys][32 * VEC]
   float* qs = vs + kKeys * 32 * VEC;                // [rows][size4]
-  float* ps = qs + kRows * size4;                   // [rows][keys]
+  float* ps = qs + kRows * size4;                   // [rows][pitch]: scores, then probabilities
   __shared__ long long places[kKeys];               // where a key's row starts in the caches, or -1
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_launch_dependents();
@@ -50,7 +56,7 @@ __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams 
   const T* q = static_cast<const T*>(p.q);
   const T* k_cache = static_cast<const T*>(p.k_cache);
   const T* v_cache = static_cast<const T*>(p.v_cache);
-  const bool aligned = p.size % 4 == 0 && (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) == 0;
+  const bool aligned = p.size % 4 == 0 && (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)p.out) & 15) == 0;
   TreeWalk w;
   bool any = tree_first(p, blockIdx.x, &w);
   if (threadIdx.x == 0) tree_note(p, blockIdx.x, w, any);
@@ -62,22 +68,20 @@ __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams 
     const int pieces = size4 >> 2;                  // of a row, four elements each
     for (int e = threadIdx.x; e < kRows * pieces; e += 32 * kWarps) {
       const int row = divide(e, pieces), d = 4 * (e - row * pieces), node = divide(row, u.heads);
+      const T* from = q + ((size_t)(w.t.first + u.first_node + node) * p.heads + u.first_head + row - node * u.heads) * p.size;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (row < rows)
-        v = elements(q + ((size_t)(w.t.first + u.first_node + node) * p.heads + u.first_head + row - node * u.heads) * p.size, d, p.size, aligned);
+      if (row < rows) v = aligned ? load4(from + d) : elements(from, d, p.size);
       *reinterpret_cast<float4*>(qs + row * size4 + d) = v;
     }
     // elements beyond the head are zeros, once
     for (int e = threadIdx.x; e < kKeys * 32 * VEC; e += 32 * kWarps)
       if (e % (32 * VEC) >= size4) vs[e] = 0.f;
-    float m[kRowsPerWarp], l[kRowsPerWarp], acc[kRowsPerWarp][VEC];
+    const int my_rows = min(kRowsPerWarp, rows - warp * kRowsPerWarp), row = warp * kRowsPerWarp + (lane >> 2);
+    float m = -INFINITY, l = 0.f, acc[kRowsPerWarp][VEC];      // maximum and sum of `row`
 #pragma unroll
-    for (int i = 0; i < kRowsPerWarp; ++i) {
-      m[i] = -INFINITY;
-      l[i] = 0.f;
+    for (int i = 0; i < kRowsPerWarp; ++i)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) acc[i][e] = 0.f;
-    }
     const int keys_end = w.t.cached + w.t.nodes;
     const int* table = p.block_table + (size_t)w.request * p.table_width;
     for (int tile = w.tile_begin; tile < w.tile_end; ++tile) {
@@ -96,8 +100,18 @@ __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams 
       __syncthreads();
       // a key beyond the end, or without a page, is zeros
       constexpr int kAhead = 4;
+      if (!aligned) {
 #pragma unroll 1
-      for (int e0 = threadIdx.x; e0 < kKeys * pieces; e0 += kAhead * 32 * kWarps) {
+        for (int e = threadIdx.x; e < kKeys * pieces; e += 32 * kWarps) {
+          const int key = divide(e, pieces), d = 4 * (e - key * pieces);
+          const long long at = places[key];
+          const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+          *reinterpret_cast<float4*>(ks + key * pitch + d) = at < 0 ? zero : elements(k_cache + at, d, p.size);
+          *reinterpret_cast<float4*>(vs + key * 32 * VEC + d) = at < 0 ? zero : elements(v_cache + at, d, p.size);
+        }
+      }
+#pragma unroll 1
+      for (int e0 = threadIdx.x; aligned && e0 < kKeys * pieces; e0 += kAhead * 32 * kWarps) {
         float4 k4[kAhead], v4[kAhead];
         int key[kAhead], d[kAhead];
 #pragma unroll
@@ -108,8 +122,8 @@ __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams 
           const long long at = key[a] < kKeys ? places[key[a]] : -1;
           k4[a] = v4[a] = make_float4(0.f, 0.f, 0.f, 0.f);
           if (at >= 0) {
-            k4[a] = elements(k_cache + at, d[a], p.size, aligned);
-            v4[a] = elements(v_cache + at, d[a], p.size, aligned);
+            k4[a] = load4(k_cache + at + d[a]);
+            v4[a] = load4(v_cache + at + d[a]);
           }
         }
 #pragma unroll
@@ -120,7 +134,6 @@ __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams 
           }
       }
       __syncthreads();
-      const int my_rows = min(kRowsPerWarp, rows - warp * kRowsPerWarp);
       if (my_rows <= 0) continue;
       float s[kRowsPerWarp];
 #pragma unroll
@@ -136,33 +149,56 @@ __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams 
           s[i] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[i]))));
         }
       }
-      // lane i finds out what row i sees
-      uint32_t mine = 0xffffffffu;
-      if (lane < my_rows && (key0 + kKeys > w.t.cached || p.window > 0)) {
-        const int token = w.t.first + u.first_node + divide(warp * kRowsPerWarp + lane, u.heads), position = tree_position(p, w.t, token);
-        mine = tree_visible(p, w.t, token, tree_lowest(p, position), position, key0);
+      // the scores change hands: four lanes a row, eight keys each
+      float* pr = ps + warp * kRowsPerWarp * kPitch;
+#pragma unroll
+      for (int i = 0; i < kRowsPerWarp; ++i) pr[i * kPitch + lane] = s[i];
+      uint32_t bits = row < rows ? 0xffffffffu : 0u;
+      if (row < rows && (key0 + kKeys > w.t.cached || p.window > 0)) {
+        const int token = w.t.first + u.first_node + divide(row, u.heads), position = tree_position(p, w.t, token);
+        bits = tree_visible(p, w.t, token, tree_lowest(p, position), position, key0);
       }
       __syncwarp();
-      const bool all = __all_sync(0xffffffffu, mine == 0xffffffffu);
-      uint32_t seen[kRowsPerWarp];
+      const bool all = __all_sync(0xffffffffu, row >= rows || bits == 0xffffffffu);
+      float* mine = ps + row * kPitch + 8 * (lane & 3);
+      if (p.softcap > 0.f) {
+#pragma unroll 1
+        for (int c = 0; c < 8; ++c) mine[c] = cap_log2 * tanhf(mine[c] * p.scale / p.softcap);
+      }
+      const float factor = p.softcap > 0.f ? 1.f : scale_log2;
+      float x[8];
+#pragma unroll
+      for (int c = 0; c < 8; c += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(mine + c);
+        x[c] = v.x, x[c + 1] = v.y, x[c + 2] = v.z, x[c + 3] = v.w;
+      }
+      float top = m, sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        x[c] = bits >> (8 * (lane & 3) + c) & 1u ? x[c] * factor : -INFINITY;
+        top = fmaxf(top, x[c]);
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const float keep = m == -INFINITY ? 0.f : exp2f(m - top);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        x[c] = x[c] == -INFINITY ? 0.f : exp2f(x[c] - top);
+        sum += x[c];
+      }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      l = (l == 0.f ? 0.f : l * keep) + sum;
+      m = top;
+#pragma unroll
+      for (int c = 0; c < 8; c += 4) *reinterpret_cast<float4*>(mine + c) = make_float4(x[c], x[c + 1], x[c + 2], x[c + 3]);
 #pragma unroll
       for (int i = 0; i < kRowsPerWarp; ++i) {
-        const int row = warp * kRowsPerWarp + i;
-        const uint32_t bits = row < rows ? __shfl_sync(0xffffffffu, mine, i) : 0u;
-        seen[i] = bits;
-        float x = p.softcap > 0.f ? cap_log2 * tanhf(s[i] * p.scale / p.softcap) : s[i] * scale_log2;
-        if (!(bits >> lane & 1u)) x = -INFINITY;
-        const float top = fmaxf(m[i], warp_max(x));
-        const float keep = m[i] == -INFINITY ? 0.f : exp2f(m[i] - top);
-        const float e = (bits >> lane & 1u) && x != -INFINITY ? exp2f(x - top) : 0.f;
-        l[i] = (l[i] == 0.f ? 0.f : l[i] * keep) + warp_sum(e);
-        m[i] = top;
-        ps[row * kKeys + lane] = e;
+        const float factor_i = __shfl_sync(0xffffffffu, keep, 4 * i);
 #pragma unroll
-        for (int d = 0; d < VEC; ++d) acc[i][d] *= keep;
+        for (int d = 0; d < VEC; ++d) acc[i][d] *= factor_i;
       }
       __syncwarp();
-      const float* pr = ps + warp * kRowsPerWarp * kKeys;
       auto value = [&](int j, float* v) {
         const float* vr = vs + j * 32 * VEC;
         if (VEC == 2) {
@@ -181,7 +217,7 @@ __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams 
         for (int j = 0; j < kKeys; j += 4) {
           float4 e4[kRowsPerWarp];
 #pragma unroll
-          for (int i = 0; i < kRowsPerWarp; ++i) e4[i] = *reinterpret_cast<const float4*>(pr + i * kKeys + j);
+          for (int i = 0; i < kRowsPerWarp; ++i) e4[i] = *reinterpret_cast<const float4*>(pr + i * kPitch + j);
 #pragma unroll
           for (int jj = 0; jj < 4; ++jj) {
             float v[VEC];
@@ -195,9 +231,9 @@ __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams 
           }
         }
       } else {
-        uint32_t some = 0u;
+        uint32_t some = 0u, seen[kRowsPerWarp];
 #pragma unroll
-        for (int i = 0; i < kRowsPerWarp; ++i) some |= seen[i];
+        for (int i = 0; i < kRowsPerWarp; ++i) some |= seen[i] = __shfl_sync(0xffffffffu, bits, 4 * i);
         for (; some; some &= some - 1) {
           const int j = __ffs(some) - 1;
           float v[VEC];
@@ -205,7 +241,7 @@ __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams 
 #pragma unroll
           for (int i = 0; i < kRowsPerWarp; ++i)
             if (seen[i] >> j & 1u) {
-              const float e = pr[i * kKeys + j];
+              const float e = pr[i * kPitch + j];
 #pragma unroll
               for (int d = 0; d < VEC; ++d) acc[i][d] = fmaf(e, v[d], acc[i][d]);
             }
@@ -213,30 +249,51 @@ __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams 
       }
       __syncwarp();
     }
+    if (my_rows <= 0) continue;
+    // the sums take the place of the warp's queries, and go out from there four elements at a time
+    float* left = qs + warp * kRowsPerWarp * size4;
 #pragma unroll
     for (int i = 0; i < kRowsPerWarp; ++i) {
-      const int row = warp * kRowsPerWarp + i;
-      if (row >= rows) break;
-      const size_t at = ((size_t)(w.t.first + u.first_node + row / u.heads) * p.heads + u.first_head + row % u.heads) * p.size;
-      const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+      if (VEC == 2) {
+        if (2 * lane < size4) *reinterpret_cast<float2*>(left + i * size4 + 2 * lane) = make_float2(acc[i][0], acc[i][1]);
+      } else {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const int d = VEC == 2 ? 2 * lane + e : (e >> 2) * 128 + 4 * lane + (e & 3);
-        if (w.whole) {
-          if (d < p.size) static_cast<T*>(p.out)[at + d] = from_float<T>(acc[i][e] * inv);
-        } else if (d < p.padded) {
-          tree_share(p, w.share, row, d)[d & 3] = acc[i][e];
-        }
+        for (int e = 0; e < VEC; e += 4)
+          if (e * 32 + 4 * lane < size4)
+            *reinterpret_cast<float4*>(left + i * size4 + e * 32 + 4 * lane) = make_float4(acc[i][e], acc[i][e + 1], acc[i][e + 2], acc[i][e + 3]);
       }
-      if (!w.whole && lane == 0) p.part_ml[(size_t)w.share * p.unit_rows + row] = make_float2(m[i], l[i]);
     }
+    __syncwarp();
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+    for (int e0 = 0; e0 < my_rows * pieces; e0 += 32) {
+      const int e = min(e0 + lane, my_rows * pieces - 1), i = divide(e, pieces), d = 4 * (e - i * pieces), r = warp * kRowsPerWarp + i;
+      const float f = __shfl_sync(0xffffffffu, inv, 4 * i);
+      float4 v = *reinterpret_cast<const float4*>(left + 4 * e);
+      if (!w.whole) {
+        *reinterpret_cast<float4*>(tree_share(p, w.share, r, d)) = v;
+        continue;
+      }
+      const int node = divide(r, u.heads);
+      T* to = static_cast<T*>(p.out) + ((size_t)(w.t.first + u.first_node + node) * p.heads + u.first_head + r - node * u.heads) * p.size + d;
+      v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+      if (aligned) {
+        store4(to, v);
+      } else {
+        to[0] = from_float<T>(v.x);
+        if (d + 1 < p.size) to[1] = from_float<T>(v.y);
+        if (d + 2 < p.size) to[2] = from_float<T>(v.z);
+        if (d + 3 < p.size) to[3] = from_float<T>(v.w);
+      }
+    }
+    if (!w.whole && (lane & 3) == 0 && row < rows) p.part_ml[(size_t)w.share * p.unit_rows + row] = make_float2(m, l);
   }
 }
 
 template <typename T, int VEC>
 int launch_tree(const TreeParams& p, cudaStream_t stream) {
   const int size4 = (p.size + 3) & ~3;
-  const size_t smem = sizeof(float) * ((size_t)kKeys * (size4 + 4) + kKeys * 32 * VEC + kRows * size4 + kRows * kKeys);
+  const size_t smem = sizeof(float) * ((size_t)kKeys * (size4 + 4) + kKeys * 32 * VEC + kRows * size4 + kRows * kPitch);
   cudaError_t e = cudaFuncSetAttribute(tree_attention_kernel<T, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
   e = launch_pdl(tree_attention_kernel<T, VEC>, dim3(p.workers), dim3(32 * kWarps), smem, stream, p);
