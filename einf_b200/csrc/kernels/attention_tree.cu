@@ -9,9 +9,14 @@
 // 16-byte words of shared memory for 32 fused multiply-adds, so shared memory bounds the kernel at two thirds of
 // the FMA rate.  Keys that no row of a tile is kept from run without masks; in the other tiles a value is added
 // to the rows that see it and to no others, so that what stands in a masked place (a sibling's value, a row behind the
-// last node) may be anything.  With few requests a CTA has two steps of keys, and the time is that of their loads one after the
-// other and of the second launch: 24.3 us for 2 requests of up to 700 keys and 13 nodes with 14 and 2 heads of 64 in float32, where
-// the bytes alone would take 0.2.
+// last node) may be anything.  Between the products the scores change hands, so that a row's softmax is four lanes' work, eight
+// keys each, done once for a warp's eight rows (a row after the other with a key a lane it was 2 us of a tile's 5: shuffles, and as
+// many instructions to fetch again for every row).
+//
+// With few requests a CTA has one tile of keys, 3.2 us: its loads 1.2, scores 1, probabilities 0.4, sums 0.8, each at its latency with a
+// warp on a scheduler; 2.5 us go before it, 4 are the second launch's.  15.4 us for 2 requests of up to 700 keys and 13 nodes
+// with 14 and 2 heads of 64 in float32, where the bytes alone would take 0.2; 226 us for one of 8,192 and 32 with 28 and 4 of 128
+// (17 TFLOP/s: the latency of shared memory between few warps).
 #include "attention_tree.cuh"
 #include "mma_sync.cuh"
 
@@ -213,7 +218,7 @@ __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams 
         }
       };
       if (all) {
-#pragma unroll 1
+#pragma unroll 2
         for (int j = 0; j < kKeys; j += 4) {
           float4 e4[kRowsPerWarp];
 #pragma unroll

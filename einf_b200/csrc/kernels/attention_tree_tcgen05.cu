@@ -14,8 +14,9 @@
 // of which either the tensor core or the exponentials' unit needs half; with few the launch's start (2.5 us until the lengths
 // are known, 3 until the first scores are) and the second launch.  Measured in captured graphs with 28 query and 4
 // key/value heads of 128: 32 requests of up to 8,192 keys and 64 nodes 233 us, which is 0.59 PFLOP/s of the products that
-// count (268 to 276 after seconds without a pause, at the power limit); one of 32,768 keys and 32 nodes 36.5 us, 1.85 TB/s.  With 12 and 2 heads, 8 requests of
-// up to 4,096 keys and 16 nodes: 17.2 us.  With 14 and 2 of 64, one of 1,024 keys and 8 nodes: 10.9 us.
+// count (268 to 276 after seconds without a pause, at the power limit); one of 32,768 keys and 32 nodes 36.5 us, 1.85 TB/s.
+// With 12 and 2 heads, 8 requests of up to 4,096 keys and 16 nodes: 17.2 us.  With 14 and 2 of 64, one of 1,024 keys and 8
+// nodes: 10.9 us.
 //
 //   warps 0, 1    K and V producers: TMA-load the pages that the block table names into rings of tiles
 //   warps 2, 3    issue a slot's products: S = Q K^T into tensor memory, then O += P V with P from there, half by half

@@ -13,7 +13,7 @@
 // one by one at the end, so that a row may be shaped in place.
 //
 // Measured with a vocabulary of 151,936, in captured graphs: 64 rows with histories of up to 4,096 tokens 21.5 us (3.6 TB/s;
-// a plain copy would take 12, the rest is the histories and the starts of the CTAs), 192 rows of eight trees with biases and masks
+// a plain copy would take 12, the rest is the histories and the starts of the CTAs), 143 rows of eight trees with biases and masks
 // 42.0 us (4.2 TB/s; 27 for a copy), one row 3.2 us.
 #include "tcgen05.cuh"
 

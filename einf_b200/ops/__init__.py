@@ -3552,7 +3552,7 @@ def tree_takes_tcgen05(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     )
 
 
-#: key tiles that a worker of a tree attention launch takes at least
+#: key tiles that a worker of a tensor-core launch takes at least: one for either slot
 TREE_MIN_TILES = 2
 
 _tree_room: dict[tuple[int, int], int] = {}
@@ -3595,17 +3595,21 @@ def _tree_workers(units: int, tiles: int, two: bool, sms: int, room) -> tuple[in
 
 @functools.lru_cache(maxsize=4096)
 def _tree_plan(tensor_cores: bool, device: int, requests: int, nodes: int, context: int, group: int, kv_heads: int,
-               size: int) -> tuple[str, int, int, bool, int, int]:
-    """The launcher; its workers, the CTAs of each, whether each has whole units; rows of all shares in scratch memory, elements of a row."""
+               size: int) -> tuple[str, int, int, bool, int, int, int]:
+    """The launcher; its workers, the CTAs of each, whether each has whole units, key tiles that one takes at least; rows of all shares in
+    scratch memory, elements of a row."""
     if tensor_cores:
         units = requests * kv_heads * -(-nodes // (2 * (TREE_TILE // group)))
         workers, cluster, whole = _tree_workers(units, -(-context // TREE_TILE), min(nodes, 2 * (TREE_TILE // group)) > TREE_TILE // group,
                                                 _sm_count(), tree_cluster_room)
-        return "einf_tree_attention_tcgen05", workers, cluster, whole, 0 if whole else 2 * workers * 2 * TREE_TILE, size
+        return "einf_tree_attention_tcgen05", workers, cluster, whole, TREE_MIN_TILES, 0 if whole else 2 * workers * 2 * TREE_TILE, size
     unit_heads = min(group, TREE_ROWS)
     units = requests * kv_heads * -(-group // unit_heads) * -(-nodes // (TREE_ROWS // unit_heads))
-    workers = max(1, min(3 * _sm_count(), units * -(-context // (TREE_KEYS * TREE_MIN_TILES))))
-    return "einf_tree_attention", workers, 1, False, 2 * workers * TREE_ROWS, -(-size // 4) * 4
+    # Two CTAs an SM, each with a tile of keys at least: 15.2 us for 2 requests of 700 keys and 13 nodes (14 and 2 heads of 64,
+    # float32) against 18.9 with one CTA an SM, 16.0 with three and 18.0 with two tiles; 232, 447 and 239 us for one of 8,192 keys and
+    # 32 nodes (28 and 4 heads of 128) with two, one and three.
+    workers = max(1, min(2 * _sm_count(), units * -(-context // TREE_KEYS)))
+    return "einf_tree_attention", workers, 1, False, 1, 2 * workers * TREE_ROWS, -(-size // 4) * 4
 
 
 _TREE_CALL = struct.Struct("<13Q15i2f4x")
@@ -3682,7 +3686,7 @@ def tree_attention(
         context = min(context, max(0, int(max_cached)) + nodes)
     if window:
         context = min(context, window + nodes + page_size)
-    symbol, workers, cluster, whole, shares, padded = _tree_plan(
+    symbol, workers, cluster, whole, min_tiles, shares, padded = _tree_plan(
         tree_takes_tcgen05(q, k_cache, v_cache, out), device, requests, nodes, context, heads // kv_heads, kv_heads, size)
     notes = sums = 0
     if shares:
@@ -3692,7 +3696,7 @@ def tree_attention(
     fn = _fn(symbol, [c_char_p, c_void_p])
     _check(
         fn(_TREE_CALL.pack(*places, sums, sums + 4 * shares * padded, notes, requests, tokens, heads, kv_heads, size, page_size,
-                           num_pages, width, words, int(window or 0), code, workers, cluster, whole, TREE_MIN_TILES, scale,
+                           num_pages, width, words, int(window or 0), code, workers, cluster, whole, min_tiles, scale,
                            softcap or 0.0), stream),
         "tree_attention",
     )
