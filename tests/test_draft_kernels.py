@@ -268,6 +268,51 @@ def test_a_result_does_not_depend_on_the_call(dev, dtype, size):
     assert int(st) == 0 and all(torch.equal(first, out) for out in outs)
 
 
+FAR = (1 << 31) + 5      # elements: offsets beyond 32 bits behind them
+
+
+@pytest.mark.parametrize("heads, kv_heads, size, page", [(12, 2, 128, 16), (4, 2, 48, 5)])
+def test_pages_beyond_32_bits(dev, heads, kv_heads, size, page):
+    """The pages at the end of a cache of more than 2^31 elements give the bits that they give in a small one."""
+    from einf_b200 import ops
+
+    case = Trees(dev, heads, kv_heads, size, page, [9, 30], [77, 400], torch.bfloat16, seed=3)
+    want = case.run()
+    q, k, v, table, *rest = case.arguments()
+    before = FAR // (kv_heads * page * size) + 1
+    far = [torch.empty((before + t.shape[0],) + tuple(t.shape[1:]), dtype=t.dtype, device=dev) for t in (k, v)]
+    for big, t in zip(far, (k, v)):
+        big[before:] = t
+    out, st = torch.full_like(q, 7.0), status(dev)
+    ops.tree_attention(q, *far, torch.where(table < 0, table, table + before), *rest, out, case.scale, st)
+    assert int(st) == 0 and torch.equal(out, want)
+    small, kept, path = [k, v], ints([5, 3], dev), ints([[0, 2, 3, 6, 8], [0, 1, 29, -1, -1]], dev)
+    ops.move_accepted(ops.CacheRows(small), table, rest[1], path, kept, st)
+    ops.move_accepted(ops.CacheRows(far), torch.where(table < 0, table, table + before), rest[1], path, kept, st)
+    assert int(st) == 0
+    for big, t in zip(far, small):
+        assert torch.equal(big[before:].view(torch.int16), t.view(torch.int16))
+
+
+@pytest.mark.parametrize("vocab", [151936, 151935])
+def test_logits_beyond_32_bits(dev, vocab):
+    case = logits_case(dev, vocab, [2, 3], 50, seed=1, biases=4, nodes=True)
+    want = shape(dev, case)
+    before = FAR // vocab + 1
+    big = torch.empty((before + 5, vocab), device=dev)
+    big[before:] = case.pop("logits").to(dev)
+    on, st = {name: t.to(dev) for name, t in case.items()}, status(dev)
+    starts = on.pop("row_start") + before
+    for name in ("tree_mask", "node_tokens"):
+        t = on[name]
+        on[name] = torch.zeros((before + 5,) + tuple(t.shape[1:]), dtype=t.dtype, device=dev)
+        on[name][before:] = t
+    from einf_b200 import ops
+
+    ops.shape_logits(big, big, starts, st, **on)
+    assert int(st) == 0 and torch.equal(big[before:], want)
+
+
 @pytest.mark.parametrize("dtype, size", [(torch.float32, 20), (torch.bfloat16, 64)])
 def test_a_window_wider_than_any_context_is_none(dev, dtype, size):
     from einf_b200 import ops
