@@ -7,15 +7,15 @@
 // exponentials the other's products have the tensor core.  A unit of two tiles gives each slot one of them, and every
 // tile of keys in shared memory serves both; a unit of one tile gives both slots the same rows and every second tile of keys, and
 // they are put together at the end.  (Scores half a tile at a time, the other half's in the making meanwhile, were no faster:
-// 247 us against 233 below; twice the instructions for the scores, which the issuing warps were slower to come by than the
+// 247 us against 221 below; twice the instructions for the scores, which the issuing warps were slower to come by than the
 // tensor core to carry out.)
 //
 // What bounds it: with many rows the way of a tile from scores to probabilities, 2.2 us for 256 rows x 128 keys x 128 of a head,
 // of which either the tensor core or the exponentials' unit needs half; with few the launch's start (2.5 us until the lengths
 // are known, 3 until the first scores are) and the second launch.  Measured in captured graphs with 28 query and 4
-// key/value heads of 128: 32 requests of up to 8,192 keys and 64 nodes 233 us, which is 0.59 PFLOP/s of the products that
-// count (268 to 276 after seconds without a pause, at the power limit); one of 32,768 keys and 32 nodes 36.5 us, 1.85 TB/s.
-// With 12 and 2 heads, 8 requests of up to 4,096 keys and 16 nodes: 17.2 us.  With 14 and 2 of 64, one of 1,024 keys and 8
+// key/value heads of 128: 32 requests of up to 8,192 keys and 64 nodes 221 to 230 us, which is 0.6 PFLOP/s of the products that
+// count (264 to 271 after seconds without a pause, at the power limit); one of 32,768 keys and 32 nodes 35.5 us, 1.9 TB/s.
+// With 12 and 2 heads, 8 requests of up to 4,096 keys and 16 nodes: 16.9 us.  With 14 and 2 of 64, one of 1,024 keys and 8
 // nodes: 10.9 us.
 //
 //   warps 0, 1    K and V producers: TMA-load the pages that the block table names into rings of tiles
@@ -106,6 +106,9 @@ __device__ __forceinline__ float2 ld_peer2(uint32_t local, uint32_t rank) {
   return v;
 }
 __device__ __forceinline__ void both_slots_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
+// A slot's warpgroup passes the turn on to the other slot's of the same keys, which takes it.
+__device__ __forceinline__ void pass_turn(int id) { asm volatile("barrier.cta.arrive %0, 256;" ::"r"(10 + id) : "memory"); }
+__device__ __forceinline__ void take_turn(int id) { asm volatile("barrier.cta.sync %0, 256;" ::"r"(10 + id) : "memory"); }
 // The two warps of a slot with the same rows meet.
 __device__ __forceinline__ void pair_sync(int pair) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(2 + pair) : "memory"); }
 
@@ -181,7 +184,7 @@ __device__ __forceinline__ void merge_cluster(const TreeParams& p, const TreeWal
 struct Row {
   bool live;
   int token, position, lowest;
-  float m, l;               // the reference, a whole number, and the sum of weights
+  float m, l;               // the reference and the sum of weights
 };
 
 // What a slot has of a unit.
@@ -485,7 +488,7 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
     const float* pair_xchg = xchg + (g * 2 + (part ^ 1)) * 128 + r;
     const ScoreScale sc = make_score_scale(p.scale, p.softcap);
     bool ok = true;
-    int done = 0, other_done = 0;      // this slot's tiles so far, and the other's before this passage
+    int done = 0;                      // this slot's tiles so far
     for (; any; next_piece()) {
       const TreeUnit u = tree_unit(p, w.t, w.unit);
       const Slot s = slot_of(w, u, g);
@@ -518,14 +521,14 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
         }
 #pragma unroll 1
         for (int j = 0; j < s.tiles; ++j, ++done) {      // `done` counts this slot's tiles
-          // The turns: slot 1's exponentials wait for slot 0's of its tile, slot 0's for slot 1's of the one before.  (Neither
-          // gets ahead by more than a tile, so no phase is missed.)  Left to themselves the slots fall into step and have their
-          // exponentials at the same time, 286 us against 233 for 32 requests of 8,192 keys and 64 nodes; turns from score
-          // product to score product, by the issuing warps, took 244; passed on before the probabilities are all there,
-          // 244 to 306.  Where neither slot has a second tile there is nothing to gain: 11.0 us without, 12.2 with turns for
-          // one request of 1,024 keys.
-          if (warp_live && turns && ok && (g || (j > 0 && j <= other_tiles)))
-            ok = __all_sync(0xffffffffu, bar_wait_likely_done(p_full(g ^ 1, part), (other_done + j - (g ^ 1)) & 1, p.status));
+          // The turns: slot 1's exponentials wait for slot 0's of its tile, slot 0's for slot 1's of the one before.  Every turn
+          // passed on is taken, whatever else went wrong, and none is passed on before the one it answers was taken.  Left to
+          // themselves the slots fall into step and have their exponentials at the same time, 286 us against 221 for 32
+          // requests of 8,192 keys and 64 nodes; turns from score product to score product, by the issuing warps, took 244; by
+          // the barrier of the probabilities 224 (300 cycles until it is seen); passed on before they are all there 244 to
+          // 306.  Where neither slot has a second tile there is nothing to gain: 11.0 us without, 12.2 with turns for one
+          // request of 1,024 keys.
+          if (turns && (g || (j > 0 && j <= other_tiles))) take_turn(2 * (g ^ 1) + part);
           if (ok) ok = __all_sync(0xffffffffu, bar_wait_likely_done(s_full(g), done & 1, p.status));
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           if (warp_live) {
@@ -603,6 +606,7 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
           }
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           bar_arrive(p_full(g, part));
+          if (turns && (g ? j + 1 < other_tiles : j < other_tiles)) pass_turn(2 * g + part);
         }
         if (ok && s.tiles > 0) {
           ok = __all_sync(0xffffffffu, bar_wait(o_done(g), (done - 1) & 1, p.status));
@@ -619,7 +623,6 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
           if (way == kAsItComes && ok && row.live && !(row.l <= kSumLimit && (row.l * kSumLimit >= 1.f || !some)))
             flags[turn & 3] = 1;
         }
-        other_done += other_tiles;
       } while (!last_passage());
       if (row.l == 0.f) row.m = -INFINITY;      // nothing to put together with others
       // The row's sums: this slot's alone, half of the head to a warp, or, where both slots had the same rows, both slots',

@@ -3568,7 +3568,7 @@ def tree_cluster_room(cluster: int) -> int:
 
 #: microseconds of a key tile, for a unit of one tile of rows and of two; of putting a cluster's shares together; of the second
 #: launch, which puts workers' shares together
-TREE_TILE_US, TREE_CLUSTER_US, TREE_MERGE_US = (1.3, 2.4), 3.5, 4.7
+TREE_TILE_US, TREE_CLUSTER_US, TREE_MERGE_US = (1.3, 2.1), 3.5, 4.7
 
 
 def _tree_workers(units: int, tiles: int, two: bool, sms: int, room) -> tuple[int, int, bool]:
@@ -3578,9 +3578,9 @@ def _tree_workers(units: int, tiles: int, two: bool, sms: int, room) -> tuple[in
     A unit has a worker of its own, of 1 to 8 CTAs that put their shares together in shared memory, or all units' tiles are laid end
     to end and cut into a run for each SM, with a second launch that puts the shares together.  The first is right while
     there are few tiles, the second where whole units leave SMs idle; the constants above tell them apart.  Measured, in
-    microseconds: 2 units of 9 tiles 11.2 in clusters of eight, 12.3 in runs, 17.6 with a CTA each; 32 of 12 14.6 in clusters
-    of four, 16.1 in runs; 12 of 6 17.6, 21.1; 16 of 33 22.3 in clusters of four, 17.2 in runs; 4 of 257 98 in clusters
-    of eight, 38 in runs; 256 of 65 339 with a CTA each, 246 in runs."""
+    microseconds: 2 units of 9 tiles 11.0 in clusters of eight, 12.0 in runs, 17.0 with a CTA each; 32 of 12 14.5 in clusters
+    of four, 16.4 in runs; 12 of 6 17.6 in clusters of eight, 20.7 in runs; 16 of 33 21.5 in clusters of four, 16.9 in runs; 4 of 257
+    86 in clusters of eight, 36 in runs; 256 of 65 294 with a CTA each, 222 in runs."""
     tile = TREE_TILE_US[two]
     workers = min(room(1), sms)
     each = -(-units * tiles // workers) if units > workers else max(TREE_MIN_TILES, -(-tiles // (workers // units)))
