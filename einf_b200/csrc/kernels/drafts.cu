@@ -26,7 +26,8 @@ static_assert(sizeof(WalkParams) == 7 * 8 + 4 * 4, "as packed");
 __global__ void __launch_bounds__(32) accept_drafts_kernel(WalkParams p) {
   __shared__ int child[kWalkNodes];
   __shared__ int walked[kWalkNodes];
-  pdl_launch_dependents();
+  // No early launch of the dependents: where a path is its root alone this is the last kernel of a step, and the next step's read
+  // the step's keys and values before their own wait.
   pdl_wait();
   const int request = blockIdx.x, lane = threadIdx.x;
   const int first = max(0, min(p.q_start[request], p.rows)), nodes = max(0, min(p.q_start[request + 1], p.rows) - first);
@@ -104,7 +105,8 @@ struct MoveParams {
 template <typename Unit>
 __global__ void __launch_bounds__(kMoveThreads) move_accepted_kernel(const __grid_constant__ MoveParams p) {
   __shared__ long long from[kMoveSteps], to[kMoveSteps];     // places: the page in the high half, the row in the low one
-  pdl_launch_dependents();
+  // No early launch of the dependents: the rows are those of cached tokens from here on, which the attention of later steps reads
+  // before its own wait.
   pdl_wait();
   const int request = blockIdx.x;
   const int count = max(0, min(p.call.counts[request], p.call.depth)), cached = p.call.cached_lens[request];

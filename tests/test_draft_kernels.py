@@ -694,3 +694,51 @@ def test_drafted_steps_answer_what_decoding_token_by_token_answers(dev):
             cached[r] += n
             kept_total += n
     assert kept_total > 2 * requests * (steps - 1)      # drafts were kept
+
+
+@pytest.mark.parametrize("size", [64, 128])
+def test_a_decode_step_behind_a_move_reads_the_moved_rows(dev, size):
+    """move_accepted, rope_kv_write and the decode attention one behind the other in a graph, with nothing between them, give what
+    they give with a synchronisation after each: the decode kernel asks for the keys of earlier steps before its own wait."""
+    from einf_b200 import ops
+
+    heads, kv_heads, page, layers, nodes, cached = 12, 2, 16, 64, 40, [600, 33, 250]
+    gen, rng = torch.Generator().manual_seed(size), random.Random(size)
+    width = -(-(max(cached) + nodes + 1) // page)
+    pages = width * len(cached)
+    table = torch.randperm(pages, generator=gen).view(len(cached), width).int().to(dev)
+    paths = [[0] + sorted(rng.sample(range(1, nodes), 30)) for _ in cached]
+    path, counts, lens = ints(paths, dev), ints([31] * len(cached), dev), ints(cached, dev)
+    given = (torch.randn((layers, 2, pages, kv_heads, page, size), generator=gen)).bfloat16().to(dev)
+    caches = torch.empty_like(given)
+    rows = ops.CacheRows(list(caches.flatten(0, 1).unbind(0)))
+    position = ints([c + 31 for c in cached], dev)
+    slots = ints([int(table[r, (c + 31) // page]) * page + (c + 31) % page for r, c in enumerate(cached)], dev)
+    qkv = torch.randn((len(cached), (heads + 2 * kv_heads) * size), generator=gen).bfloat16().to(dev)
+    inv_freq = (100.0 ** (-torch.arange(0, size, 2).float() / size)).to(dev)
+    seq, st = ints(range(len(cached)), dev), status(dev)
+    q = torch.empty((len(cached), heads, size), dtype=torch.bfloat16, device=dev)
+    outs = [torch.zeros_like(q) for _ in range(2 * 3)]
+
+    def step(outs, layers, between):
+        caches.copy_(given)
+        between()
+        ops.move_accepted(rows, table, lens, path, counts, st)
+        for out, layer in zip(outs, layers):
+            between()
+            ops.rope_kv_write(qkv, None, position, inv_freq, slots, q, caches[layer, 0], caches[layer, 1], heads, kv_heads, size, st)
+            between()
+            ops.paged_decode_attention_tcgen05(q, caches[layer, 0], caches[layer, 1], table, seq, position, out, size ** -0.5, None, 4, st)
+
+    for i, layer in enumerate((0, layers // 2, layers - 1)):
+        step(outs[i:i + 1], [layer], torch.cuda.synchronize)
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            step(outs[3 + i:4 + i], [layer], lambda: None)
+        for _ in range(20):
+            outs[3 + i].zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(outs[i], outs[3 + i])
+    assert int(st) == 0

@@ -1,8 +1,11 @@
 """What the operators of drafted trees refuse, how their launches are cut, on a machine without a GPU."""
+import re
+
 import pytest
 import torch
 
 from einf_b200 import ops
+from einf_b200.ops import build
 
 
 @pytest.fixture
@@ -198,3 +201,12 @@ def test_tensors_of_the_cpu_are_refused():
         ops.accept_drafts(ints(6), ints(6), ints(6), ints(3), ints(2, 4), ints(2, 4), ints(2))
     with pytest.raises(ops.KernelError):
         ops.CacheRows([torch.zeros(6, 2, 4, 8)])
+
+
+@pytest.mark.parametrize("source, kernel", [("drafts", "move_accepted_kernel"), ("drafts", "accept_drafts_kernel"), ("pointwise", "advance_decode_kernel")])
+def test_kernels_that_change_what_a_later_step_reads_early_are_waited_for(source, kernel):
+    """Decode kernels read positions, slots and the keys of earlier steps before they wait for the kernel before them: none may
+    start before a kernel has ended that writes these."""
+    text = (build.KERNEL_DIR / f"{source}.cu").read_text()
+    body = re.search(rf"__global__ void[^;{{]*\b{kernel}\(.*?\n}}\n", text, re.S).group(0)
+    assert "pdl_wait();" in body and "pdl_launch_dependents();" not in body
