@@ -742,3 +742,148 @@ def test_a_decode_step_behind_a_move_reads_the_moved_rows(dev, size):
             torch.cuda.synchronize()
             assert torch.equal(outs[i], outs[3 + i])
     assert int(st) == 0
+
+
+# ---------------------------------------------------------------------------
+# Launches cut in the ways that the sizes of tests do not lead to: units over several workers, several units to one, shares that
+# the second launch puts together.
+def cut_over(monkeypatch, workers):
+    from einf_b200 import ops
+
+    def plan(tensor_cores, device, requests, nodes, context, group, kv_heads, size):
+        if tensor_cores:
+            return "einf_tree_attention_tcgen05", workers, 1, False, ops.TREE_MIN_TILES, 2 * workers * 2 * ops.TREE_TILE, size
+        return "einf_tree_attention", workers, 1, False, 1, 2 * workers * ops.TREE_ROWS, -(-size // 4) * 4
+
+    monkeypatch.setattr(ops, "_tree_plan", plan)
+
+
+class Cut(Trees):
+    """Trees that are run several times and stated in 64 bits once."""
+
+    stated: dict = {}
+
+    def check(self, got, window=None, softcap=None):
+        key = (window, softcap)
+        if key not in self.stated:
+            want, bound = ref.tree_attention(self.q, self.k, self.v, self.table, torch.tensor(self.starts), torch.tensor(self.cached),
+                                             self.mask, self.scale, self.positions, window, softcap)
+            want, bound = want[:self.starts[-1]], bound[:self.starts[-1]]
+            if self.q.dtype == torch.bfloat16:      # as in Trees.check
+                bound = bound + self.weights_step(window, softcap) + want.abs() * 2.0 ** -8
+            self.stated = {**self.stated, key: (want, bound * 1.0001)}
+        want, bound = self.stated[key]
+        got, live = got.double().cpu(), self.starts[-1]
+        assert torch.equal(got[live:], torch.full_like(got[live:], 7.0)), "rows of no request were written"
+        assert ((got[:live] - want).abs() <= bound).all()
+
+
+CUTS = [
+    # nodes, cached: one unit, few units, more units than workers
+    ([1], [1500]),
+    ([40], [1290]),
+    ([20, 3, 0, 90, 8], [700, 1500, 40, 300, 900]),
+    ([5, 4, 1, 30, 2, 7, 6, 3], [300, 500, 130, 257, 1, 800, 0, 384]),
+]
+
+
+@pytest.mark.parametrize("dtype, heads, kv_heads, size, page", [
+    (torch.bfloat16, 14, 2, 64, 16), (torch.bfloat16, 12, 2, 128, 16), (torch.bfloat16, 4, 4, 128, 64), (torch.float32, 4, 2, 48, 4)])
+@pytest.mark.parametrize("nodes, cached", CUTS)
+def test_tree_attention_cut_over_workers(dev, monkeypatch, dtype, heads, kv_heads, size, page, nodes, cached):
+    case = Cut(dev, heads, kv_heads, size, page, nodes, cached, dtype, seed=sum(nodes), extra_rows=1)
+    for workers in (1, 2, 3, 7, 148):
+        cut_over(monkeypatch, workers)
+        first = case.run()
+        case.check(first)
+        assert torch.equal(first, case.run())
+
+
+@pytest.mark.parametrize("size", [64, 128])
+@pytest.mark.parametrize("window, softcap", [(200, None), (30, 3.0), (10 ** 9, 20.0)])
+def test_windows_and_caps_cut_over_workers(dev, monkeypatch, size, window, softcap):
+    case = Cut(dev, 12, 2, size, 16, *CUTS[3], torch.bfloat16, seed=4)
+    for workers in (2, 7, 148):
+        cut_over(monkeypatch, workers)
+        case.check(case.run(window=window, **({"softcap": softcap} if softcap else {})), window, softcap)
+
+
+@pytest.mark.parametrize("size", [64, 128])
+@pytest.mark.parametrize("levels", [
+    lambda j: -100.0 if j < 200 else 150.0 + j % 3, lambda j: 150.0 if j < 200 else -100.0, lambda j: -300.0 - j % 5,
+    lambda j: 900.0 if j == 350 else 899.0 if j == 30 else 0.5 * (j % 7)], ids=["rising", "falling", "low", "peaks"])
+def test_scores_that_need_a_second_passage_cut_over_workers(dev, monkeypatch, size, levels):
+    nodes, cached = CUTS[3]
+    case = Cut(dev, 6, 2, size, 16, nodes, cached, torch.bfloat16, seed=6)
+    case.q[:] = 1.0
+    for r, (c, n) in enumerate(zip(cached, nodes)):
+        for j in range(c + n):
+            where, row = case.slot(r, j)
+            case.k[where, :, row] = levels(j) * size ** -0.5
+    for workers in (2, 3, 7, 148):
+        cut_over(monkeypatch, workers)
+        case.check(case.run())
+
+
+@pytest.mark.parametrize("size", [64, 128])
+@pytest.mark.parametrize("workers", [2, 7, 148])
+@pytest.mark.parametrize("bad", [NAN, math.inf])
+def test_values_that_are_not_finite_cut_over_workers(dev, monkeypatch, size, workers, bad):
+    cut_over(monkeypatch, workers)
+    nodes, cached = CUTS[2]
+    case, clean = (Trees(dev, 12, 2, size, 16, nodes, cached, torch.bfloat16, seed=11) for _ in range(2))
+    hit = 5
+    where, row = case.slot(0, cached[0] + hit)
+    case.v[where, 0, row, ::3] = bad
+    got, want = case.run().double().cpu(), clean.run().double().cpu()
+    for j in range(nodes[0]):
+        if int(case.mask[j, 0]) >> hit & 1:
+            assert not got[j, :6, ::3].isfinite().any()
+            got[j, :6, ::3] = want[j, :6, ::3]
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("size", [64, 128])
+@pytest.mark.parametrize("workers", [3, 148])
+def test_graphs_that_share_scratch_memory_at_once(dev, monkeypatch, size, workers):
+    """Two captured launches with shares in scratch memory, replayed side by side, and a third one on another stream meanwhile."""
+    from einf_b200 import ops
+
+    cut_over(monkeypatch, workers)
+    cases = [Trees(dev, 12, 2, size, 16, *CUTS[i], torch.bfloat16, seed=2 + i) for i in (2, 3, 2)]
+    wants, st = [case.run() for case in cases], status(dev)
+    given, outs, streams, graphs = [case.arguments() for case in cases], [torch.zeros_like(w) for w in wants], [torch.cuda.Stream() for _ in cases], []
+    torch.cuda.synchronize()
+    for case, arguments, out in zip(cases[:2], given, outs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops.tree_attention(*arguments, out, case.scale, st)
+        graphs.append(graph)
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        with torch.cuda.stream(streams[2]):
+            ops.tree_attention(*given[2], outs[2], cases[2].scale, st)
+    torch.cuda.synchronize()
+    assert int(st) == 0 and all(torch.equal(want, out) for want, out in zip(wants, outs))
+
+
+@pytest.mark.parametrize("dtype, heads, kv_heads, size, page", [
+    (torch.bfloat16, 14, 2, 64, 16), (torch.bfloat16, 6, 2, 128, 8), (torch.bfloat16, 4, 2, 48, 4), (torch.float32, 4, 2, 20, 5)])
+@pytest.mark.parametrize("requests", [33, 70])
+def test_more_requests_than_a_warp_has_lanes(dev, monkeypatch, dtype, heads, kv_heads, size, page, requests):
+    """A launch's work is counted 32 requests at a time; some of them, the last and a whole 32 among them, have no nodes."""
+    rng = random.Random(requests)
+    nodes = [rng.choice([0, 1, 2, 5]) for _ in range(requests)]
+    cached = [rng.choice([0, 1, 30, 127, 128, 300]) for _ in range(requests)]
+    nodes[-1] = 0
+    if requests > 64:
+        nodes[32:64] = [0] * 32
+    case = Cut(dev, heads, kv_heads, size, page, nodes, cached, dtype, seed=requests, extra_rows=1)
+    for workers in (None, 5, 148):
+        if workers:
+            cut_over(monkeypatch, workers)
+        case.check(case.run())
+        case.check(case.run(window=100), 100)
