@@ -271,14 +271,15 @@ __global__ void __launch_bounds__(kShapeThreads) shape_logits_bulk_kernel(ShapeP
   const float* biases = p.bias + (size_t)w.request * p.biases;
   const int shift = (w.v0 + i0) & 31;                            // parts start on whole words
   uint32_t parity = 0u;                                          // a bit a stage
+  int there = steps;                                             // the first step whose part did not come within the limit
 #pragma unroll 1
   for (int step = 0; step < steps; ++step) {
     const int stage = step % kStages, n = places(step), part0 = (step & (p.parts - 1)) * kPart;
     const Bits bits = ahead;
     ahead = ask_bits(step + 1);
-    if (n > 0) {
+    if (n > 0 && there == steps && !bar_wait_likely_done(saddr(bars + stage), parity >> stage & 1u, p.status)) there = step;
+    if (n > 0 && there == steps) {
       float* out = p.out + (size_t)(w.first_row + (step >> part_shift) * (int)gridDim.z) * p.vocab + w.v0 + part0;
-      bar_wait_likely_done(saddr(bars + stage), parity >> stage & 1u, p.status);
       parity ^= 1u << stage;
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
@@ -316,7 +317,14 @@ __global__ void __launch_bounds__(kShapeThreads) shape_logits_bulk_kernel(ShapeP
       }
     }
     __syncthreads();                                             // the stage is read
-    if (threadIdx.x == 0) fetch(step + kStages);
+    if (threadIdx.x == 0 && there == steps) fetch(step + kStages);
+  }
+  if (!__syncthreads_and(there == steps)) {
+    // A thread that gave up asked for and wrote nothing more; no CTA ends with a copy under way.
+    if (threadIdx.x == 0)
+      for (int step = there; step < min(steps, there + kStages); ++step)
+        if (places(step) > 0) bar_poll(saddr(bars + step % kStages), parity >> (step % kStages) & 1u);
+    return;
   }
   shape_drafted<HAS_BIAS>(p, w, s, words, reinterpret_cast<int2*>(ring));
 }

@@ -210,3 +210,11 @@ def test_kernels_that_change_what_a_later_step_reads_early_are_waited_for(source
     text = (build.KERNEL_DIR / f"{source}.cu").read_text()
     body = re.search(rf"__global__ void[^;{{]*\b{kernel}\(.*?\n}}\n", text, re.S).group(0)
     assert "pdl_wait();" in body and "pdl_launch_dependents();" not in body
+
+
+@pytest.mark.parametrize("source", ["logits.cu", "attention_tree_tcgen05.cu"])
+def test_every_bounded_wait_is_asked_whether_it_ran_out(source):
+    """A kernel goes on from a wait on a barrier only if what it waited for is there."""
+    lines = (build.KERNEL_DIR / source).read_text().splitlines()
+    assert any("bar_wait" in line for line in lines)
+    assert [line for line in lines if re.match(r"\s*bar_wait\w*\(", line)] == []
