@@ -407,6 +407,8 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
       } while (!last_passage());
     }
     if (__any_sync(0xffffffffu, bad) && lane == 0) atomicOr(p.status, kStatusBadPage);
+    // no copy is under way when the CTA leaves: lane j waits for the last one into stage j
+    if (!ok && lane < stages && (lane < stage || round > 0)) bar_poll(full_bar(lane), (lane < stage ? round : round - 1) & 1);
   } else if (warp < 4) {
     // ---- a slot's products: the whole warp goes the way of the lane that issues, so that addresses stay in uniform registers ----
     const int g = warp - 2;

@@ -218,3 +218,10 @@ def test_every_bounded_wait_is_asked_whether_it_ran_out(source):
     lines = (build.KERNEL_DIR / source).read_text().splitlines()
     assert any("bar_wait" in line for line in lines)
     assert [line for line in lines if re.match(r"\s*bar_wait\w*\(", line)] == []
+
+
+@pytest.mark.parametrize("source", ["logits.cu", "attention_tree_tcgen05.cu"])
+def test_no_kernel_leaves_copies_behind(source):
+    """Where a wait has run out, the copies that were asked for are waited for, with a limit, before the CTA ends."""
+    text = (build.KERNEL_DIR / source).read_text()
+    assert re.search(r"// [^\n]*no (?:CTA|copy)\b[^\n]*under way.{0,300}bar_poll\(", text, re.S)
