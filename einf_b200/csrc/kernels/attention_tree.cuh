@@ -173,10 +173,16 @@ struct TreeWalk {
   bool list;
 };
 
-__device__ __forceinline__ int warp_add(int v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+// A launch's units (nodes and heads that the caller holds to this many, unless trees overlap) and its pairs of a unit and a key
+// tile, so that places in the list are 32-bit.  (Pairs are not bounded by memory: all units of a key/value head read the same
+// keys, and requests may share pages.)
+constexpr int kTreeMostUnits = 1 << 20, kTreeMostPairs = 1 << 30;
+
+__device__ __forceinline__ int warp_add(int v) { return __reduce_add_sync(0xffffffffu, v); }
+// Of 64-bit numbers below 2^52, in two sums that 32 bits hold.
+__device__ __forceinline__ long long warp_add(long long v) {
+  const unsigned low = __reduce_add_sync(0xffffffffu, (unsigned)v & 0x3ffffffu);
+  return ((long long)__reduce_add_sync(0xffffffffu, (unsigned)(v >> 26)) << 26) + low;
 }
 __device__ __forceinline__ void tree_piece(const TreeParams& p, int worker, TreeWalk* w, int tile_begin, int available) {
   w->tile_begin = tile_begin;
@@ -186,8 +192,8 @@ __device__ __forceinline__ void tree_piece(const TreeParams& p, int worker, Tree
   w->share = 2 * worker + (w->pieces > 0 ? 1 : 0);
   ++w->pieces;
 }
-// The first piece of a worker; every warp works it out by itself.  False where there is nothing to do.  (Sums are 32-bit: a
-// launch of 2^31 key tiles would read more than there is memory.)
+// The first piece of a worker; every warp works it out by itself.  False where there is nothing to do, or more than a launch
+// takes: then the status word is set, and no worker has a piece.
 __device__ __forceinline__ bool tree_first(const TreeParams& p, int worker, TreeWalk* w) {
   const int lane = threadIdx.x & 31;
   TreeRequest mine = {};
@@ -200,11 +206,17 @@ __device__ __forceinline__ bool tree_first(const TreeParams& p, int worker, Tree
   };
   auto total = [&](auto weight) {
     if (few) return warp_add(weight(mine));
-    int sum = 0;
+    auto sum = weight(TreeRequest{});
     for (int r0 = 0; r0 < p.requests; r0 += 32) sum += warp_add(weight(request(r0 + lane)));
     return sum;
   };
-  const int units = total([](const TreeRequest& t) { return t.units; });
+  auto too_many = [&] {
+    if (lane == 0) atomicOr(p.status, kStatusBadIndex);
+    return false;
+  };
+  const long long all_units = total([](const TreeRequest& t) { return (long long)t.units; });
+  if (all_units > kTreeMostUnits) return too_many();
+  const int units = (int)all_units;
   int chunk = 1, begin, end;
   w->list = false;
   if (p.whole) {
@@ -213,7 +225,9 @@ __device__ __forceinline__ bool tree_first(const TreeParams& p, int worker, Tree
     begin = worker * each;
     end = min(units, begin + each);
   } else {
-    const int pairs = total([](const TreeRequest& t) { return t.units * t.tiles; });
+    const long long all_pairs = total([](const TreeRequest& t) { return (long long)t.units * t.tiles; });
+    if (all_pairs > kTreeMostPairs) return too_many();
+    const int pairs = (int)all_pairs;
     chunk = max(p.min_chunk, (pairs + p.workers - 1) / p.workers);
     if (units > p.workers) {
       w->list = true;

@@ -887,3 +887,36 @@ def test_more_requests_than_a_warp_has_lanes(dev, monkeypatch, dtype, heads, kv_
             cut_over(monkeypatch, workers)
         case.check(case.run())
         case.check(case.run(window=100), 100)
+
+
+@pytest.mark.parametrize("dtype, heads, size", [(torch.float32, 32, 1), (torch.bfloat16, 128, 64)])
+def test_more_tiles_than_a_launch_counts_set_the_status_word(dev, monkeypatch, dtype, heads, size):
+    """One page over and over: more than 2^31 pairs of rows' and keys' tiles, in a few hundred megabytes."""
+    from einf_b200 import ops
+
+    cut_over(monkeypatch, 148)
+    nodes, cached, page = (16384, 1 << 22, 64) if size == 1 else (32768, 1 << 24, 64)
+    k = torch.zeros((1, 1, page, size), dtype=dtype, device=dev)
+    q = torch.zeros((nodes, heads, size), dtype=dtype, device=dev)
+    table = torch.zeros((1, -(-(cached + nodes) // page)), dtype=torch.int32, device=dev)
+    out, st = torch.full_like(q, 7.0), status(dev)
+    ops.tree_attention(q, k, k.clone(), table, ints([0, nodes], dev), ints([cached], dev), torch.ones((nodes, 1), dtype=torch.int64, device=dev),
+                       out, 1.0, st)
+    assert int(st) == ops.STATUS_BAD_INDEX
+    assert (out == 7.0).all()
+
+
+def test_trees_that_overlap_to_more_than_their_nodes_set_the_status_word(dev):
+    """The same rows for every second request, the launch's most units each: counted in 64 bits, and not computed."""
+    from einf_b200 import ops
+
+    nodes, requests = 1 << 20, 8192
+    q = torch.zeros((nodes, 1, 1), device=dev)
+    k = torch.zeros((1, 1, nodes, 1), device=dev)
+    out, st = torch.full_like(q, 7.0), status(dev)
+    starts = torch.tensor([0, nodes] * (requests // 2) + [0], dtype=torch.int32, device=dev)
+    table = torch.zeros((requests, 1), dtype=torch.int32, device=dev)
+    ops.tree_attention(q, k, k.clone(), table, starts, torch.zeros(requests, dtype=torch.int32, device=dev),
+                       torch.zeros((nodes, 1), dtype=torch.int64, device=dev), out, 1.0, st)
+    assert int(st) == ops.STATUS_BAD_INDEX
+    assert (out == 7.0).all()
