@@ -3559,10 +3559,16 @@ _tree_room: dict[tuple[int, int], int] = {}
 
 
 def tree_cluster_room(cluster: int) -> int:
-    """How many clusters of ``cluster`` CTAs of the tensor-core tree attention kernel the device holds at once."""
+    """How many clusters of ``cluster`` CTAs of the tensor-core tree attention kernel the device holds at once; 0 where it cannot
+    say, and an error if it cannot for single CTAs."""
     key = (torch.cuda.current_device(), cluster)
     if key not in _tree_room:
-        _tree_room[key] = int(_fn("einf_tree_attention_tcgen05_max_clusters", [c_int])(cluster))
+        room = int(_fn("einf_tree_attention_tcgen05_max_clusters", [c_int])(cluster))
+        if room < 1:      # not kept: it may have been another call's error
+            if cluster == 1:
+                raise KernelError("the device does not say how many CTAs of the tree attention kernel it holds")
+            return 0
+        _tree_room[key] = room
     return _tree_room[key]
 
 

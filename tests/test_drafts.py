@@ -225,3 +225,17 @@ def test_no_kernel_leaves_copies_behind(source):
     """Where a wait has run out, the copies that were asked for are waited for, with a limit, before the CTA ends."""
     text = (build.KERNEL_DIR / source).read_text()
     assert re.search(r"// [^\n]*no (?:CTA|copy)\b[^\n]*under way.{0,300}bar_poll\(", text, re.S)
+
+
+def test_a_device_that_does_not_say_what_it_holds_is_asked_again(monkeypatch):
+    answers = {1: [0, 148], 4: [0, 36]}
+    monkeypatch.setattr(ops, "_fn", lambda symbol, argtypes, variant="": lambda cluster: answers[cluster].pop(0))
+    monkeypatch.setattr(ops, "_tree_room", {})
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    with pytest.raises(ops.KernelError):
+        ops.tree_cluster_room(1)
+    assert [ops.tree_cluster_room(1) for _ in range(2)] == [148, 148]
+    assert [ops.tree_cluster_room(4) for _ in range(3)] == [0, 36, 36]
+    # larger clusters that it does not hold are not chosen
+    workers, cluster, whole = ops._tree_workers(2, 9, False, 148, lambda c: 148 if c == 1 else 0)
+    assert cluster == 1 and workers >= 1
