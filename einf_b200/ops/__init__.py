@@ -3714,10 +3714,10 @@ SHAPE_PART = 2048      # places of the vocabulary that a CTA of shape_logits has
 
 
 @functools.lru_cache(maxsize=4096)
-def _shape_pieces(rows: int, requests: int, vocab: int, capacity: int) -> tuple[int, int]:
+def _shape_pieces(device: int, rows: int, requests: int, vocab: int, capacity: int) -> tuple[int, int]:
     """Parts of the vocabulary to a CTA of :func:`shape_logits`, and how many CTAs take a request's rows in turn.  A CTA reads
     its request's whole history: more parts to it where the history is longer than they are, as long as the device
-    is filled; the rows are shared out where it is not."""
+    is filled; the rows are shared out where it is not.  (``device`` is the current one: what is remembered is its.)"""
     full, parts, ways = 4 * _sm_count(), 1, 1
     while parts < 4 and SHAPE_PART * parts * rows <= capacity * requests and requests * -(-vocab // (2 * SHAPE_PART * parts)) >= full:
         parts *= 2
@@ -3823,7 +3823,7 @@ def shape_logits(
         raise UnsupportedSize(f"shape_logits takes up to 65535 requests, not {requests}")
     fn = _fn("einf_shape_logits", [c_char_p, c_void_p])
     _check(
-        fn(_SHAPE_CALL.pack(*places, rows, vocab, requests, capacity, words, biases, masks, mask_words, *_shape_pieces(rows, requests, vocab, capacity)),
+        fn(_SHAPE_CALL.pack(*places, rows, vocab, requests, capacity, words, biases, masks, mask_words, *_shape_pieces(device, rows, requests, vocab, capacity)),
            stream),
         "shape_logits",
     )

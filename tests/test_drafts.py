@@ -1,5 +1,6 @@
 """What the operators of drafted trees refuse, how their launches are cut, on a machine without a GPU."""
 import re
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -239,3 +240,17 @@ def test_a_device_that_does_not_say_what_it_holds_is_asked_again(monkeypatch):
     # larger clusters that it does not hold are not chosen
     workers, cluster, whole = ops._tree_workers(2, 9, False, 148, lambda c: 148 if c == 1 else 0)
     assert cluster == 1 and workers >= 1
+
+
+def test_a_launch_is_cut_for_the_device_that_it_is_on(on_this_machine, monkeypatch):
+    """What is remembered of one device's launches is not taken for another's."""
+    cuts = []
+    monkeypatch.setattr(ops, "_SHAPE_CALL", SimpleNamespace(pack=lambda *values: cuts.append(values[-2:]) or b""))
+    ops._shape_pieces.cache_clear()
+    for device, sms in ((-1, 148), (-2, 1), (-1, 148)):
+        monkeypatch.setattr(ops, "_current", lambda: (device, 0))
+        monkeypatch.setattr(ops, "_sm_count", lambda: sms)
+        monkeypatch.setattr(ops, "_at", lambda t, name, dtype, device: t.data_ptr())
+        ops.shape_logits(torch.zeros(8, 5000), torch.zeros(8, 5000), ints(2), ints(1))
+    ops._shape_pieces.cache_clear()
+    assert cuts[0] == cuts[2] != cuts[1]
