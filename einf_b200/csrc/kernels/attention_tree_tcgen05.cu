@@ -40,6 +40,7 @@ constexpr int kTile = 128;                     // rows of a slot, keys of a tile
 constexpr int kSlice = kTile * 128;            // a [128 rows x 64] bfloat16 slice: 16 KB
 constexpr int kTreeThreads = 640;
 constexpr float kSumLimit = 1.15292150e18f;    // 2^60
+constexpr float kLowest = -3.40282347e38f;
 constexpr int kHalf = kTile / 2;               // keys of a softmax thread
 constexpr int kTmemColumns = 512;              // S: 2 x 128 columns, O: 2 x D
 
@@ -566,6 +567,8 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
 #pragma unroll
                 for (int c = 0; c < 16; c += 4) top = max3(top, max3(v[c], v[c + 1], v[c + 2]), v[c + 3]);
               }
+              // under a cap a score of -inf is one as any other, the lowest: no row that sees one is without a reference
+              if (sc.tanh_in != 0.f && (seen[0] | seen[1])) top = fmaxf(top, kLowest);
               best = fmaxf(best, top);
               if (way == kAsItComes) {
                 // The row's reference: the maximum of the tile (the scale is positive and the cap grows with the score: the
@@ -594,10 +597,11 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
               for (int c0 = 0; c0 < kHalf; c0 += 16) {
                 float v[16];
                 uint32_t packed[8];
-                scores(c0, v, true);
+                scores(c0, v, sc.tanh_in == 0.f);
                 if (sc.tanh_in != 0.f) {
+                  const uint32_t bits = (c0 < 32 ? seen[0] : seen[1]) >> (c0 & 31);
 #pragma unroll
-                  for (int c = 0; c < 16; ++c) v[c] = v[c] == -INFINITY ? -INFINITY : __fdividef(capped(v[c], sc), sc.scale_log2);
+                  for (int c = 0; c < 16; ++c) v[c] = bits >> c & 1u ? __fdividef(capped(v[c], sc), sc.scale_log2) : -INFINITY;
                 }
                 exps(v, packed, scale2, shift2, &sum2);
                 tmem_st8(s_row + (c0 >> 1), packed);

@@ -920,3 +920,40 @@ def test_trees_that_overlap_to_more_than_their_nodes_set_the_status_word(dev):
                        torch.zeros((nodes, 1), dtype=torch.int64, device=dev), out, 1.0, st)
     assert int(st) == ops.STATUS_BAD_INDEX
     assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype, heads, kv_heads, size, page", [
+    (torch.float32, 4, 2, 48, 4), (torch.bfloat16, 4, 2, 48, 4), (torch.bfloat16, 14, 2, 64, 16), (torch.bfloat16, 12, 2, 128, 16)])
+@pytest.mark.parametrize("softcap", [3.0, 100.0])
+@pytest.mark.parametrize("workers", [None, 7])
+def test_infinite_scores_are_capped(dev, monkeypatch, dtype, heads, kv_heads, size, page, softcap, workers):
+    """A score of minus or plus infinity is the cap's lowest or highest, for rows that see nothing else too; one that is no number
+    stays none."""
+    if workers:
+        cut_over(monkeypatch, workers)
+    nodes, cached = [12, 1, 30, 4], [150, 0, 390, 300]
+    case = Trees(dev, heads, kv_heads, size, page, nodes, cached, dtype, seed=11)
+    case.q[:, :, 1] = case.q[:, :, 1].abs() + 0.5
+    key_size = float((case.k[~case.k.isnan()]).abs().max())
+    for r, (c, n) in enumerate(zip(cached, nodes)):
+        for j in range(c + n):
+            where, row = case.slot(r, j)
+            if r == 1 or j % 7 == 3 or (r == 3 and j < 256):
+                case.k[where, :, row, 1] = -math.inf
+            elif j % 31 == 5:
+                case.k[where, :, row, 1] = math.inf
+    where, row = case.slot(0, cached[0] + 5)
+    case.k[where, :, row, 1] = NAN
+    got = case.run(softcap=softcap).double().cpu()
+    statement = (case.table, torch.tensor(case.starts), torch.tensor(case.cached), case.mask, case.scale, None, None, softcap)
+    want, _ = ref.tree_attention(case.q, case.k, case.v, *statement)
+    assert torch.equal(got.isnan(), want.isnan()) and want.isnan().any() and want[12].isfinite().all()
+    # A finite score is a sum of `size` rounded products, the cap's own error 8 units of the cap; a weight is off by as much
+    # and 4 units more, a result by twice the worst of them and a unit for every sum, of the values' size.
+    eps, count = 2.0 ** -24, max(c + n for c, n in zip(cached, nodes))
+    worst = (size + 4) * eps * key_size * float(case.q.abs().max()) * size * case.scale + 8 * eps * softcap + 4 * eps * (2 * softcap + 1)
+    bound = (2 * worst + (2 * count + count / 16 + 8) * eps) * float(case.v[~case.v.isnan()].abs().max())
+    if dtype == torch.bfloat16:      # the weights as the second product's operand, and the result
+        sizes, _ = ref.tree_attention(case.q, case.k, case.v.abs(), *statement)
+        bound = bound + sizes * 2.0 ** -8 * 1.01 + want.abs() * 2.0 ** -8
+    assert ((got - want).abs() <= bound)[want.isfinite()].all()
