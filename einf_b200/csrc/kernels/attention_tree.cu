@@ -83,6 +83,7 @@ __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams 
       if (e % (32 * VEC) >= size4) vs[e] = 0.f;
     const int my_rows = min(kRowsPerWarp, rows - warp * kRowsPerWarp), row = warp * kRowsPerWarp + (lane >> 2);
     float m = -INFINITY, l = 0.f, acc[kRowsPerWarp][VEC];      // maximum and sum of `row`
+    bool some = false;                                         // it has seen a key
 #pragma unroll
     for (int i = 0; i < kRowsPerWarp; ++i)
 #pragma unroll
@@ -171,6 +172,7 @@ __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams 
         for (int c = 0; c < 8; ++c) mine[c] = cap_log2 * tanhf(mine[c] * p.scale / p.softcap);
       }
       const float factor = p.softcap > 0.f ? 1.f : scale_log2;
+      some = some || bits != 0u;
       float x[8];
 #pragma unroll
       for (int c = 0; c < 8; c += 4) {
@@ -269,7 +271,8 @@ __global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams 
       }
     }
     __syncwarp();
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (m == -INFINITY && l == 0.f && some) l = 1.f;
+    const float inv = tree_inverse(m, l);
 #pragma unroll 1
     for (int e0 = 0; e0 < my_rows * pieces; e0 += 32) {
       const int e = min(e0 + lane, my_rows * pieces - 1), i = divide(e, pieces), d = 4 * (e - i * pieces), r = warp * kRowsPerWarp + i;

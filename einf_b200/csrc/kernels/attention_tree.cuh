@@ -365,6 +365,17 @@ __device__ __forceinline__ void tree_note(const TreeParams& p, int worker, const
   p.notes[worker] = n;
 }
 
+// A row's reference m and sum of weights l: where m is -inf, l is 0 for a row that saw no key, 1 for one whose scores were all -inf (its
+// softmax is no number), and no number for one that saw a score that is none.  What two shares of a row's keys come to:
+__device__ __forceinline__ float tree_sums(float m_a, float l_a, float factor_a, float m_b, float l_b, float factor_b) {
+  if (m_a == -INFINITY && m_b == -INFINITY) return l_a + l_b;
+  return (l_a == 0.f ? 0.f : l_a * factor_a) + (l_b == 0.f ? 0.f : l_b * factor_b);
+}
+// What a row's sums are multiplied by in the end.
+__device__ __forceinline__ float tree_inverse(float m, float l) {
+  return l == 0.f ? 0.f : m == -INFINITY ? NAN : 1.f / l;
+}
+
 constexpr int kTreeMergeWarps = 4;
 constexpr int kTreeMergeShares = 4;        // shares that a warp has in flight
 
@@ -416,13 +427,13 @@ __global__ void __launch_bounds__(32 * kTreeMergeWarps) tree_merge_kernel(TreePa
       const float keep = m == -INFINITY ? 0.f : fast_exp2(m - top);
       m = top;
       // a sum of weights that is not a number stays one, whatever the reference beside it
-      l = l == 0.f ? 0.f : l * keep;
+      l = l == 0.f ? 0.f : top == -INFINITY ? l : l * keep;
       a.x *= keep, a.y *= keep, a.z *= keep, a.w *= keep;
       b.x *= keep, b.y *= keep, b.z *= keep, b.w *= keep;
 #pragma unroll
       for (int i = 0; i < kTreeMergeShares; ++i) {
         const float f = v[i].x == -INFINITY || c0 + i > n.places ? 0.f : fast_exp2(v[i].x - top);
-        l += v[i].y == 0.f || c0 + i > n.places ? 0.f : v[i].y * f;
+        l += v[i].y == 0.f || c0 + i > n.places ? 0.f : top == -INFINITY ? v[i].y : v[i].y * f;
         if (f == 0.f) continue;                          // a share without a reference has nothing in its sums
         a.x = fmaf(x[i].x, f, a.x), a.y = fmaf(x[i].y, f, a.y), a.z = fmaf(x[i].z, f, a.z), a.w = fmaf(x[i].w, f, a.w);
         b.x = fmaf(y[i].x, f, b.x), b.y = fmaf(y[i].y, f, b.y), b.z = fmaf(y[i].z, f, b.z), b.w = fmaf(y[i].w, f, b.w);
@@ -442,8 +453,8 @@ __global__ void __launch_bounds__(32 * kTreeMergeWarps) tree_merge_kernel(TreePa
         const float(*x)[32] = left[o];
         const float top = fmaxf(m, x[0][lane]), keep = m == -INFINITY ? 0.f : fast_exp2(m - top);
         const float f = x[0][lane] == -INFINITY ? 0.f : fast_exp2(x[0][lane] - top);
+        l = tree_sums(m, l, keep, x[0][lane], x[1][lane], f);
         m = top;
-        l = (l == 0.f ? 0.f : l * keep) + (x[1][lane] == 0.f ? 0.f : x[1][lane] * f);
         // a share without a reference has nothing in its sums
         a.x = fmaf(x[2][lane], f, a.x * keep), a.y = fmaf(x[3][lane], f, a.y * keep);
         a.z = fmaf(x[4][lane], f, a.z * keep), a.w = fmaf(x[5][lane], f, a.w * keep);
@@ -452,7 +463,7 @@ __global__ void __launch_bounds__(32 * kTreeMergeWarps) tree_merge_kernel(TreePa
       }
     }
     if (row >= rows) continue;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = tree_inverse(m, l);
     const int node = divide(row, n.heads), d = 4 * group;
     T* out = static_cast<T*>(p.out) + ((size_t)(n.token + node) * p.heads + n.first_head + row - node * n.heads) * p.size + d;
     const float v[8] = {a.x * inv, a.y * inv, a.z * inv, a.w * inv, b.x * inv, b.y * inv, b.z * inv, b.w * inv};

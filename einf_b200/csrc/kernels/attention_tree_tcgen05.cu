@@ -157,7 +157,7 @@ __device__ __forceinline__ void merge_cluster(const TreeParams& p, const TreeWal
     const float2 ml = lane < p.cluster ? ld_peer2(base + L::kSumsMl + row * 8, lane) : make_float2(-INFINITY, 0.f);
     const float m = warp_max(ml.x);
     const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - m);
-    const float l = warp_sum(ml.y == 0.f ? 0.f : ml.y * f);
+    const float l = warp_sum(ml.y == 0.f ? 0.f : m == -INFINITY ? ml.y : ml.y * f);
     const uint32_t at = base + L::kSums + (row * L::kPitch + (4 * lane) % D) * 4;      // (D = 64: the upper lanes repeat the lower)
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
@@ -171,7 +171,7 @@ __device__ __forceinline__ void merge_cluster(const TreeParams& p, const TreeWal
       sum.w += o.w * fc;
     }
     if (4 * lane < D) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = tree_inverse(m, l);
       const int node = divide(row, u.heads);
       __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) +
           ((size_t)(w.t.first + u.first_node + node) * p.heads + u.first_head + row - node * u.heads) * D + 4 * lane;
@@ -619,18 +619,20 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         }
         pair_sync(pair);      // both have read what the other left
-        *my_xchg = way == kForMaxima ? best : row.l;
+        *my_xchg = way == kForMaxima ? best : row.l == 0.f && some ? -1.f : row.l;
         pair_sync(pair);
         if (way == kForMaxima) {
           best = fmaxf(best, *pair_xchg);
           row.m = best == -INFINITY ? 0.f : score_log2(best, sc);
         } else {
-          row.l = *my_xchg + *pair_xchg;
+          const float a = *my_xchg, b = *pair_xchg;
+          row.l = (a < 0.f ? 0.f : a) + (b < 0.f ? 0.f : b);
+          if (row.l == 0.f && a + b < 0.f) row.l = -1.f;      // the row has seen keys, and scores of -inf alone
           if (way == kAsItComes && ok && row.live && !(row.l <= kSumLimit && (row.l * kSumLimit >= 1.f || !some)))
             flags[turn & 3] = 1;
         }
       } while (!last_passage());
-      if (row.l == 0.f) row.m = -INFINITY;      // nothing to put together with others
+      if (row.l <= 0.f) row.m = -INFINITY, row.l = -row.l;      // nothing to put together with others
       // The row's sums: this slot's alone, half of the head to a warp, or, where both slots had the same rows, both slots',
       // a quarter of the head to a warp.
       float m = row.m, l = row.l, mine = 1.f, other = 0.f;
@@ -644,12 +646,12 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const _
         m = fmaxf(row.m, m_other);
         mine = row.m == -INFINITY ? 0.f : fast_exp2(row.m - m);
         other = m_other == -INFINITY ? 0.f : fast_exp2(m_other - m);
-        l = (l == 0.f ? 0.f : l * mine) + (l_other == 0.f ? 0.f : l_other * other);
+        l = tree_sums(row.m, l, mine, m_other, l_other, other);
         d0 = (g * 2 + part) * (D / 4);
         d1 = d0 + D / 4;
       }
       const bool write = row.live && ok, not_all_finite = flags[4 + (pieces & 3)] != 0;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = tree_inverse(m, l);
       const uint32_t o_other = tmem_o(g ^ 1) + lane_addr;
       float* left = reinterpret_cast<float*>(smem_raw + L::kSums) + unit_row * L::kPitch;
       __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + ((size_t)row.token * p.heads + u.first_head + (row.live ? r - node * u.heads : 0)) * D;

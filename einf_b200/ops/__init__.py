@@ -3645,7 +3645,8 @@ def tree_attention(
     ``tree_mask[node, k // 64]`` (int64) is set: its ancestors and itself, in a tree.  With ``window`` it sees
     only what stands less than ``window`` before its position (``positions``, int32 per node, then needed; nodes
     stand at their request's cached length at least).  ``softcap`` as in :func:`paged_attention_generic`.  A node that sees
-    nothing gets zeros, rows that belong to no request keep what they hold.
+    nothing gets zeros (one that sees scores of minus infinity alone NaN, as their softmax), rows that belong to no request keep
+    what they hold.
 
     A request has up to 2^27 tokens, a launch up to 2^20 nodes x key/value heads; one with more work than is counted (over 2^30
     tiles of rows and keys where workers share rows, trees that overlap) sets ``STATUS_BAD_INDEX`` and computes nothing.  Scores,

@@ -957,3 +957,39 @@ def test_infinite_scores_are_capped(dev, monkeypatch, dtype, heads, kv_heads, si
         sizes, _ = ref.tree_attention(case.q, case.k, case.v.abs(), *statement)
         bound = bound + sizes * 2.0 ** -8 * 1.01 + want.abs() * 2.0 ** -8
     assert ((got - want).abs() <= bound)[want.isfinite()].all()
+
+
+@pytest.mark.parametrize("dtype, heads, kv_heads, size, page", [
+    (torch.float32, 4, 2, 48, 4), (torch.bfloat16, 4, 2, 48, 4), (torch.bfloat16, 14, 2, 64, 16), (torch.bfloat16, 12, 2, 128, 16)])
+@pytest.mark.parametrize("workers", [None, 1, 2, 7, 148])
+def test_rows_whose_scores_are_all_minus_infinity_are_no_numbers(dev, monkeypatch, dtype, heads, kv_heads, size, page, workers):
+    """As their softmax: not zeros, which is what a row gets that sees nothing.  Keys with such a score count for nothing beside others,
+    wherever a row's shares begin and end."""
+    if workers:
+        cut_over(monkeypatch, workers)
+    nodes, cached = [12, 1, 30, 4, 3, 9], [150, 0, 390, 300, 700, 0]
+    case = Trees(dev, heads, kv_heads, size, page, nodes, cached, dtype, seed=12)
+    case.q[:, :, 1] = case.q[:, :, 1].abs() + 0.5
+    key_size = float((case.k[~case.k.isnan()]).abs().max())
+    for r, (c, n) in enumerate(zip(cached, nodes)):
+        for j in range(c + n):
+            where, row = case.slot(r, j)
+            if r in (1, 4) or (r == 0 and j < 140) or (r == 2 and j >= 128) or (r == 3 and not 256 <= j < 260):
+                case.k[where, :, row, 1] = -math.inf
+    case.mask[50 + 3] = 0      # of the last request, which has no cached tokens: one node sees nothing
+    got = case.run().double().cpu()
+    statement = (case.table, torch.tensor(case.starts), torch.tensor(case.cached), case.mask, case.scale)
+    want, _ = ref.tree_attention(case.q, case.k, case.v, *statement)
+    assert torch.equal(got.isnan(), want.isnan())
+    assert want[12].isnan().all() and want[47:50].isnan().all() and int(want.isnan().any(-1).any(-1).sum()) == 4
+    assert (want[53] == 0).all() and (got[53] == 0).all()
+    # as the bound of other rows: a score is a sum of `size` rounded products, a weight is off by as much and by two units of
+    # how far it lies below the row's highest
+    eps, count = 2.0 ** -24, max(c + n for c, n in zip(cached, nodes))
+    highest = key_size * float(case.q.abs().max()) * size * case.scale
+    worst = (size + 4) * eps * highest + 2 * eps * 2 * highest + 4 * eps
+    bound = (2 * worst + (2 * count + count / 16 + 8) * eps) * float(case.v[~case.v.isnan()].abs().max())
+    if dtype == torch.bfloat16:
+        sizes, _ = ref.tree_attention(case.q, case.k, case.v.abs(), *statement)
+        bound = bound + sizes * 2.0 ** -8 * 1.01 + want.abs() * 2.0 ** -8
+    assert ((got - want).abs() <= bound)[want.isfinite()].all()
