@@ -24,8 +24,9 @@
 //
 // The two warpgroups of a slot agree on nothing while they run: a row's reference is the maximum of its first tile,
 // and stays.  What that leaves to be done comes out at the end of a piece: a row with a sum of
-// weights above 2^60 (scores far above the reference; an overflow is such a sum too), or one that saw keys and has less
-// than 2^-60, sends the piece through again, once for the rows' maxima and once against those.
+// weights above 2^40 (scores far above the reference; an overflow is such a sum too), or one that saw keys and has less
+// than 2^-40, sends the piece through again, once for the rows' maxima and once against those.  So sums hold values of up to 2^86
+// times their weights, and down to 2^-86 nothing of them is lost.
 //
 // Tiles with keys that some row does not see (the drafted ones, a window) run with masks of 64 bits a thread.  There a
 // value that is not finite must not meet a weight of zero, so the V producer looks over such a tile and clears the
@@ -39,7 +40,7 @@ namespace einf {
 constexpr int kTile = 128;                     // rows of a slot, keys of a tile
 constexpr int kSlice = kTile * 128;            // a [128 rows x 64] bfloat16 slice: 16 KB
 constexpr int kTreeThreads = 640;
-constexpr float kSumLimit = 1.15292150e18f;    // 2^60
+constexpr float kSumLimit = 1099511627776.f;   // 2^40
 constexpr float kLowest = -3.40282347e38f;
 constexpr int kHalf = kTile / 2;               // keys of a softmax thread
 constexpr int kTmemColumns = 512;              // S: 2 x 128 columns, O: 2 x D

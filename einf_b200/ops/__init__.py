@@ -3650,7 +3650,7 @@ def tree_attention(
 
     A request has up to 2^27 tokens, a launch up to 2^20 nodes x key/value heads; one with more work than is counted (over 2^30
     tiles of rows and keys where workers share rows, trees that overlap) sets ``STATUS_BAD_INDEX`` and computes nothing.  Scores,
-    softmax and sums are 32-bit.  ``max_nodes`` and ``max_cached``, the most nodes and cached tokens of a request as
+    softmax and sums are 32-bit, with room for values of up to 2^86.  ``max_nodes`` and ``max_cached``, the most nodes and cached tokens of a request as
     far as the caller knows them, only size the launch: any request's nodes are computed whole."""
     tokens, heads, size = q.shape
     num_pages, kv_heads, page_size, cache_size = k_cache.shape

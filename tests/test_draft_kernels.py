@@ -993,3 +993,27 @@ def test_rows_whose_scores_are_all_minus_infinity_are_no_numbers(dev, monkeypatc
         sizes, _ = ref.tree_attention(case.q, case.k, case.v.abs(), *statement)
         bound = bound + sizes * 2.0 ** -8 * 1.01 + want.abs() * 2.0 ** -8
     assert ((got - want).abs() <= bound)[want.isfinite()].all()
+
+
+@pytest.mark.parametrize("dtype, heads, kv_heads, size, page", [
+    (torch.float32, 4, 2, 48, 4), (torch.bfloat16, 14, 2, 64, 16), (torch.bfloat16, 12, 2, 128, 16)])
+@pytest.mark.parametrize("workers", [None, 7])
+@pytest.mark.parametrize("power, level", [(83, 35.0), (83, 26.0), (-83, -35.0), (-83, -26.0)])
+def test_large_and_small_values_beside_scores_far_apart(dev, monkeypatch, dtype, heads, kv_heads, size, page, workers, power, level):
+    """What weighs a row's keys against the first it sees has room for values of 2^83 times the weights of scores far above, and loses
+    nothing of values of 2^-83 times those of scores far below."""
+    if workers:
+        cut_over(monkeypatch, workers)
+    nodes, cached = ([9, 40], [700, 390]) if level > 0 else ([300, 200], [0, 0])
+    case = Trees(dev, heads, kv_heads, size, page, nodes, cached, dtype, seed=13)
+    case.q[:] = 1.0
+    case.v = (case.v.float() * 2.0 ** power).to(dtype)
+    for r, (c, n) in enumerate(zip(cached, nodes)):
+        for j in range(c + n):
+            where, row = case.slot(r, j)
+            case.k[where, :, row] = (0.0 if j < 130 else level - j % 3) * size ** -0.5
+    if level < 0:       # a node sees itself and one before it: nothing of the first tiles
+        for i in range(sum(nodes)):
+            k = i % 300
+            case.mask[i] = torch.tensor(words_of(1 << k | 1 << max(k - 1, 0), case.mask.shape[1]))
+    case.check(case.run())
