@@ -3654,7 +3654,7 @@ def tree_attention(
     far as the caller knows them, only size the launch: any request's nodes are computed whole."""
     tokens, heads, size = q.shape
     num_pages, kv_heads, page_size, cache_size = k_cache.shape
-    requests, (table_rows, width) = cached_lens.shape[0], block_table.shape
+    (requests,), (table_rows, width) = cached_lens.shape, block_table.shape
     dtype = q.dtype
     if out.shape != q.shape or v_cache.shape != k_cache.shape or cache_size != size:
         raise ValueError(f"q {tuple(q.shape)}, out {tuple(out.shape)} and caches {tuple(k_cache.shape)}, {tuple(v_cache.shape)} do not "
@@ -3664,8 +3664,9 @@ def tree_attention(
         raise UnsupportedSize(f"{heads} query heads are not a multiple of {kv_heads} key/value heads")
     if not 1 <= size <= MAX_HEAD_SIZE:
         raise UnsupportedSize(f"tree attention takes heads of up to {MAX_HEAD_SIZE}, not {size}")
-    if q_start.shape[0] != requests + 1 or table_rows < requests:
-        raise ValueError(f"q_start must hold {requests + 1} entries and block_table a row for each of {requests} requests")
+    if q_start.shape != (requests + 1,) or table_rows < requests:
+        raise ValueError(f"q_start is {tuple(q_start.shape)}, expected ({requests + 1},), and block_table needs a row for each of "
+                         f"{requests} requests")
     if tokens * kv_heads * -(-(heads // kv_heads) // TREE_ROWS) > 1 << 20:
         raise UnsupportedSize(f"tree attention takes up to {1 << 20} nodes x key/value heads, not {tokens} x {kv_heads}")
     words = _mask_words(tree_mask, tokens)
@@ -3766,8 +3767,8 @@ def shape_logits(
     if out.shape != logits.shape:
         raise ValueError(f"logits {tuple(logits.shape)}, out {tuple(out.shape)}")
     requests = rows if row_start is None else row_start.shape[0] - 1
-    if requests < 0:
-        raise ValueError("row_start must hold one more entry than there are requests")
+    if requests < 0 or (row_start is not None and row_start.dim() != 1):
+        raise ValueError("row_start must be [requests + 1]")
     if (history is None) != (history_lens is None) or (prompt_lens is not None and history is None):
         raise ValueError("a history comes with its lengths")
     if (node_tokens is None) != (tree_mask is None):
@@ -3800,7 +3801,7 @@ def shape_logits(
     device, stream = _current()
     for t, name in ((history_lens, "history_lens"), (prompt_lens, "prompt_lens"), (repetition, "repetition"), (presence, "presence"),
                     (frequency, "frequency")):
-        if t is not None and t.shape[0] != requests:
+        if t is not None and t.shape != (requests,):
             raise ValueError(f"{name} is {tuple(t.shape)}, expected ({requests},)")
     i32, f32 = torch.int32, torch.float32
     places = (
@@ -3845,8 +3846,8 @@ def accept_drafts(node_tokens: torch.Tensor, targets: torch.Tensor, parents: tor
     (rows,), (requests,), (path_rows, depth) = node_tokens.shape, counts.shape, path.shape
     if targets.shape != node_tokens.shape or parents.shape != node_tokens.shape:
         raise ValueError("node_tokens, targets and parents must be [rows]")
-    if q_start.shape[0] != requests + 1:
-        raise ValueError(f"q_start must hold {requests + 1} entries")
+    if q_start.shape != (requests + 1,):
+        raise ValueError(f"q_start is {tuple(q_start.shape)}, expected ({requests + 1},)")
     if path_rows != requests or depth < 1 or answer.shape != path.shape:
         raise ValueError(f"path {tuple(path.shape)} and answer {tuple(answer.shape)} must be [{requests}, depth]")
     device, stream = _current()

@@ -254,3 +254,27 @@ def test_a_launch_is_cut_for_the_device_that_it_is_on(on_this_machine, monkeypat
         ops.shape_logits(torch.zeros(8, 5000), torch.zeros(8, 5000), ints(2), ints(1))
     ops._shape_pieces.cache_clear()
     assert cuts[0] == cuts[2] != cuts[1]
+
+
+@pytest.mark.parametrize("change", [dict(q_start=ints(3, 1)), dict(q_start=ints(3, 2)), dict(cached_lens=ints(2, 1)), dict(cached_lens=ints(2, 2)),
+                                    dict(window=3, positions=ints(5, 1))])
+def test_tree_attention_looks_at_whole_shapes(on_this_machine, change):
+    with pytest.raises(ValueError):
+        ops.tree_attention(**attention_arguments(**change))
+    assert on_this_machine == []
+
+
+@pytest.mark.parametrize("name", ["history_lens", "prompt_lens", "repetition", "presence", "frequency"])
+@pytest.mark.parametrize("shape", [(2, 1), (2, 2)])
+def test_shape_logits_looks_at_whole_shapes(on_this_machine, name, shape):
+    with pytest.raises(ValueError):
+        ops.shape_logits(**logits_arguments(**{name: (ints if name.endswith("lens") else torch.ones)(*shape)}))
+    with pytest.raises(ValueError):
+        ops.shape_logits(**logits_arguments(row_start=ints(3, 2)))
+    assert on_this_machine == []
+
+
+def test_accept_drafts_looks_at_whole_shapes(on_this_machine):
+    with pytest.raises(ValueError):
+        ops.accept_drafts(ints(6), ints(6), ints(6), ints(3, 2), ints(2, 4), ints(2, 4), ints(2))
+    assert on_this_machine == []
