@@ -3786,6 +3786,8 @@ def shape_logits(
         words = _mask_words(tree_mask, rows)
         if words > 64:
             raise UnsupportedSize(f"shape_logits takes masks of up to 64 words (4096 nodes), not {words}")
+        if rows * 64 * words >= 1 << 31:      # a request's rows x its nodes are counted in 32 bits
+            raise UnsupportedSize(f"shape_logits takes fewer than 2^31 rows x nodes, not {rows} x {64 * words}")
     if bias is not None:
         if bias.dim() != 2 or bias.shape[0] != requests or bias_ids.shape != bias.shape:
             raise ValueError(f"bias_ids {tuple(bias_ids.shape)} and bias {tuple(bias.shape)} must be [{requests}, n]")

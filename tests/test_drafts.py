@@ -278,3 +278,16 @@ def test_accept_drafts_looks_at_whole_shapes(on_this_machine):
     with pytest.raises(ValueError):
         ops.accept_drafts(ints(6), ints(6), ints(6), ints(3, 2), ints(2, 4), ints(2, 4), ints(2))
     assert on_this_machine == []
+
+
+@pytest.mark.parametrize("rows, words", [((1 << 19), 64), ((1 << 25), 1)])
+def test_shape_logits_refuses_more_rows_and_nodes_than_it_counts(on_this_machine, rows, words):
+    def given(rows):
+        return dict(logits=torch.zeros(1, 2).expand(rows, 2), out=torch.zeros(1, 2).expand(rows, 2), row_start=ints(2), status=ints(1),
+                    node_tokens=ints(1).expand(rows), tree_mask=torch.zeros(1, words, dtype=torch.int64).expand(rows, words))
+
+    with pytest.raises(ops.UnsupportedSize):
+        ops.shape_logits(**given(rows))
+    with pytest.raises(ValueError, match="contiguous"):      # a row less is not too many
+        ops.shape_logits(**given(rows - 1))
+    assert on_this_machine == []
