@@ -114,9 +114,10 @@ __device__ __forceinline__ void take_turn(int id) { asm volatile("barrier.cta.sy
 // The two warps of a slot with the same rows meet.
 __device__ __forceinline__ void pair_sync(int pair) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(2 + pair) : "memory"); }
 
-// 16 scores of a row to 2^(scale s - m): packed, and added to `sum`.  (Taken from the exponentials' unit, 16 a cycle, three of
-// eight by a polynomial of the fourth degree made tree-sized launches 4 per cent slower: while a slot's threads are at this the
-// other slot's products run, and it is the way from scores to weights, not the unit, that a tile waits for.)
+// 16 scores of a row to 2^(scale s - m): packed, and added to `sum`.  Packed they are bfloat16, up to 2^-8 off each, as the second
+// product's operands have one type and the values are bfloat16; the sum takes them as they are, in 32 bits.  (Taken from the
+// exponentials' unit, 16 a cycle, three of eight by a polynomial of the fourth degree made tree-sized launches 4 per cent slower: while
+// a slot's threads are at this the other slot's products run, and it is the way from scores to weights, not the unit, that a tile waits for.)
 __device__ __forceinline__ void exps(const float* v, uint32_t* packed, float2 scale2, float2 shift2, float2* sum) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {

@@ -3646,11 +3646,13 @@ def tree_attention(
     only what stands less than ``window`` before its position (``positions``, int32 per node, then needed; nodes
     stand at their request's cached length at least).  ``softcap`` as in :func:`paged_attention_generic`.  A node that sees
     nothing gets zeros (one that sees scores of minus infinity alone NaN, as their softmax), rows that belong to no request keep
-    what they hold.
+    what they hold.  Layers with a sink, kept first positions, chunks, values of another size or latent rows are not taken, nor a
+    scale that is not positive.
 
     A request has up to 2^27 tokens, a launch up to 2^20 nodes x key/value heads; one with more work than is counted (over 2^30
     tiles of rows and keys where workers share rows, trees that overlap) sets ``STATUS_BAD_INDEX`` and computes nothing.  Scores,
-    softmax and sums are 32-bit, with room for values of up to 2^86.  ``max_nodes`` and ``max_cached``, the most nodes and cached tokens of a request as
+    softmax and sums are 32-bit, with room for values of up to 2^86; on the tensor cores (:func:`tree_takes_tcgen05`) the
+    probabilities are rounded to bfloat16 before they meet the values, as in the prompt kernel.  ``max_nodes`` and ``max_cached``, the most nodes and cached tokens of a request as
     far as the caller knows them, only size the launch: any request's nodes are computed whole."""
     tokens, heads, size = q.shape
     num_pages, kv_heads, page_size, cache_size = k_cache.shape
@@ -3758,11 +3760,13 @@ def shape_logits(
 
     ``history`` (int32 ``[requests, capacity]``) holds the first ``history_lens[r]`` tokens of a request, of which the first
     ``prompt_lens[r]`` (None: none) are its prompt.  For drafted trees ``node_tokens`` (int32 ``[rows]``) are the rows' own
-    tokens and ``tree_mask`` their ancestors and themselves, as in :func:`tree_attention`: these count as answered.
+    tokens and ``tree_mask`` their ancestors and themselves, as in :func:`tree_attention`: these count as answered, the root
+    among them, so that the history of such a call ends before the root (at the cached tokens); a root in both counts twice.
     ``bias_ids`` (int32 ``[requests, n]``, negative: none) and ``bias`` (float32) are added to single tokens, the last entry
     of a token that stands twice.  ``allowed`` (int32 ``[masks, (vocab + 31) // 32]``) has bit ``v % 32`` of word
     ``v // 32`` set for tokens that may come; row ``i`` has mask ``i``, or mask ``allowed_rows[i]`` (int32, negative: none).
-    A token outside the vocabulary and a mask that is not there set the status word and count for nothing."""
+    A token outside the vocabulary and a mask that is not there set the status word and count for nothing; rows that belong to
+    no request are not written."""
     rows, vocab = logits.shape
     if out.shape != logits.shape:
         raise ValueError(f"logits {tuple(logits.shape)}, out {tuple(out.shape)}")

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from einf_b200 import ops
+from einf_b200.engine import ModelRunner, StepError
 from einf_b200.ops import build
 
 
@@ -291,3 +292,10 @@ def test_shape_logits_refuses_more_rows_and_nodes_than_it_counts(on_this_machine
     with pytest.raises(ValueError, match="contiguous"):      # a row less is not too many
         ops.shape_logits(**given(rows - 1))
     assert on_this_machine == []
+
+
+def test_a_bad_index_fails_the_step():
+    ModelRunner.check_status(0)
+    with pytest.raises(StepError, match="an index outside what it points into") as caught:
+        ModelRunner.check_status(ops.STATUS_BAD_INDEX)
+    assert "page" not in str(caught.value)
