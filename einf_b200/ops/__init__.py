@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 import struct
 from ctypes import c_char_p, c_float, c_int, c_longlong, c_void_p
 from typing import Optional, Sequence, Tuple
@@ -3647,7 +3648,7 @@ def tree_attention(
     stand at their request's cached length at least).  ``softcap`` as in :func:`paged_attention_generic`.  A node that sees
     nothing gets zeros (one that sees scores of minus infinity alone NaN, as their softmax), rows that belong to no request keep
     what they hold.  Layers with a sink, kept first positions, chunks, values of another size or latent rows are not taken, nor a
-    scale that is not positive.
+    scale that is not positive and finite.
 
     A request has up to 2^27 tokens, a launch up to 2^20 nodes x key/value heads; one with more work than is counted (over 2^30
     tiles of rows and keys where workers share rows, trees that overlap) sets ``STATUS_BAD_INDEX`` and computes nothing.  Scores,
@@ -3672,10 +3673,10 @@ def tree_attention(
     if tokens * kv_heads * -(-(heads // kv_heads) // TREE_ROWS) > 1 << 20:
         raise UnsupportedSize(f"tree attention takes up to {1 << 20} nodes x key/value heads, not {tokens} x {kv_heads}")
     words = _mask_words(tree_mask, tokens)
-    if not scale > 0:
-        raise ValueError(f"the scale is positive, not {scale}")
-    if softcap is not None and not softcap > 0:
-        raise ValueError(f"a soft cap is positive, not {softcap}")
+    if not 0 < scale < math.inf:
+        raise ValueError(f"the scale is positive and finite, not {scale}")
+    if softcap is not None and not 0 < softcap < math.inf:
+        raise ValueError(f"a soft cap is positive and finite, not {softcap}")
     if window is not None:
         if window < 1:
             raise ValueError(f"a window holds at least one token, not {window}")

@@ -299,3 +299,11 @@ def test_a_bad_index_fails_the_step():
     with pytest.raises(StepError, match="an index outside what it points into") as caught:
         ModelRunner.check_status(ops.STATUS_BAD_INDEX)
     assert "page" not in str(caught.value)
+
+
+@pytest.mark.parametrize("change", [dict(softcap=float("inf")), dict(scale=float("inf")), dict(scale=float("nan"))])
+def test_tree_attention_refuses_scales_and_caps_that_are_not_finite(on_this_machine, change):
+    """The kernels differ in what becomes of them: uncapped scores in one, no numbers in the other."""
+    with pytest.raises(ValueError, match="finite"):
+        ops.tree_attention(**attention_arguments(**change))
+    assert on_this_machine == []
