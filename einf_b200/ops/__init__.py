@@ -3691,7 +3691,7 @@ def tree_attention(
         _at(positions, "positions", torch.int32, device) if window else 0, _at(out, "out", dtype, device),
         _at(status, "status", torch.int32, device),
     )
-    if tokens == 0 or requests == 0:
+    if tokens == 0 or requests == 0 or heads == 0:
         return
     nodes = min(tokens, 64 * words if max_nodes is None else max(1, int(max_nodes)))
     context = width * page_size

@@ -307,3 +307,8 @@ def test_tree_attention_refuses_scales_and_caps_that_are_not_finite(on_this_mach
     with pytest.raises(ValueError, match="finite"):
         ops.tree_attention(**attention_arguments(**change))
     assert on_this_machine == []
+
+
+def test_tree_attention_without_heads_has_nothing_to_do(on_this_machine):
+    ops.tree_attention(**attention_arguments(q=torch.zeros(5, 0, 48), out=torch.zeros(5, 0, 48)))
+    assert on_this_machine == []
