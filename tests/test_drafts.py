@@ -312,3 +312,12 @@ def test_tree_attention_refuses_scales_and_caps_that_are_not_finite(on_this_mach
 def test_tree_attention_without_heads_has_nothing_to_do(on_this_machine):
     ops.tree_attention(**attention_arguments(q=torch.zeros(5, 0, 48), out=torch.zeros(5, 0, 48)))
     assert on_this_machine == []
+
+
+def test_a_status_without_a_word_is_refused(on_this_machine):
+    caches = ops.CacheRows([torch.zeros(6, 2, 4, 8)])
+    for call in (lambda: ops.tree_attention(**attention_arguments(status=ints(0))), lambda: ops.shape_logits(**logits_arguments(status=ints(0))),
+                 lambda: ops.move_accepted(caches, ints(2, 2), ints(2), ints(2, 4), ints(2), ints(0))):
+        with pytest.raises(ValueError, match="status"):
+            call()
+    assert on_this_machine == []
