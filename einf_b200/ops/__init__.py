@@ -3529,11 +3529,9 @@ def _current() -> tuple[int, int]:
     return torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream
 
 
-def _status_at(status: torch.Tensor, device: int) -> int:
-    """The address of the status word: a kernel writes there without looking whether there is one."""
-    if status.numel() < 1:
-        raise ValueError("status must hold a word")
-    return _at(status, "status", torch.int32, device)
+def _no_status() -> int:
+    """In the place of an empty tensor's address: a kernel writes the status without looking whether there is a word."""
+    raise ValueError("status must hold a word")
 
 
 def _mask_words(tree_mask: torch.Tensor, rows: int) -> int:
@@ -3696,7 +3694,7 @@ def tree_attention(
         _at(block_table, "block_table", torch.int32, device), _at(q_start, "q_start", torch.int32, device),
         _at(cached_lens, "cached_lens", torch.int32, device), _at(tree_mask, "tree_mask", torch.int64, device),
         _at(positions, "positions", torch.int32, device) if window else 0, _at(out, "out", dtype, device),
-        _status_at(status, device),
+        _at(status, "status", torch.int32, device) or _no_status(),
     )
     if tokens == 0 or requests == 0 or heads == 0:
         return
@@ -3819,7 +3817,7 @@ def shape_logits(
             raise ValueError(f"{name} is {tuple(t.shape)}, expected ({requests},)")
     i32, f32 = torch.int32, torch.float32
     places = (
-        _at(logits, "logits", f32, device), _at(out, "out", f32, device), _status_at(status, device),
+        _at(logits, "logits", f32, device), _at(out, "out", f32, device), _at(status, "status", i32, device) or _no_status(),
         0 if history_lens is None else _at(history_lens, "history_lens", i32, device),
         0 if prompt_lens is None else _at(prompt_lens, "prompt_lens", i32, device),
         0 if repetition is None else _at(repetition, "repetition", f32, device),
@@ -3932,7 +3930,7 @@ def move_accepted(caches: CacheRows, block_table: torch.Tensor, cached_lens: tor
         raise ValueError(f"the caches are on cuda:{caches.device}, and the current device is cuda:{device}")
     call = _MOVE_CALL.pack(
         _at(block_table, "block_table", torch.int32, device), _at(cached_lens, "cached_lens", torch.int32, device),
-        _at(path, "path", torch.int32, device), _at(counts, "counts", torch.int32, device), _status_at(status, device),
+        _at(path, "path", torch.int32, device), _at(counts, "counts", torch.int32, device), _at(status, "status", torch.int32, device) or _no_status(),
         requests, depth, width, 0)
     if requests == 0 or depth < 2:
         return
