@@ -14,8 +14,8 @@
 // many instructions to fetch again for every row).
 //
 // With few requests a CTA has one tile of keys, 3.2 us: its loads 1.2, scores 1, probabilities 0.4, sums 0.8, each at its latency with a
-// warp on a scheduler; 2.5 us go before it, 4 are the second launch's.  15.4 us for 2 requests of up to 700 keys and 13 nodes
-// with 14 and 2 heads of 64 in float32, where the bytes alone would take 0.2; 226 us for one of 8,192 and 32 with 28 and 4 of 128
+// warp on a scheduler; 2.5 us go before it, 4 are the second launch's.  15.7 us for 2 requests of up to 700 keys and 13 nodes
+// with 14 and 2 heads of 64 in float32, where the bytes alone would take 0.2; 223 us for one of 8,192 and 32 with 28 and 4 of 128
 // (17 TFLOP/s: the latency of shared memory between few warps).
 #include "attention_tree.cuh"
 #include "mma_sync.cuh"
@@ -45,9 +45,11 @@ __device__ __forceinline__ float4 elements(const T* row, int d, int size) {
                      d + 3 < size ? to_float(row[d + 3]) : 0.f);
 }
 
-// VEC: elements of the head that a lane has (2, 4 or 8: heads of up to 64, 128, 256)
+// VEC: elements of the head that a lane has (2, 4 or 8: heads of up to 64, 128, 256).  Launches have two CTAs an SM, and the compiler is
+// told so: left to itself it took registers for one of three or four, and the products' loop came out up to a fifth slower with every
+// change around it (one request of 8,192 keys and 32 nodes, 28 and 4 heads of 128 in float32: 223 us; 272 without, 229 for four).
 template <typename T, int VEC>
-__global__ void __launch_bounds__(32 * kWarps) tree_attention_kernel(TreeParams p) {
+__global__ void __launch_bounds__(32 * kWarps, 2) tree_attention_kernel(TreeParams p) {
   extern __shared__ __align__(16) float smem[];
   const int size4 = (p.size + 3) & ~3, pitch = size4 + 4;
   float* ks = smem;                                 // [keys][pitch]
