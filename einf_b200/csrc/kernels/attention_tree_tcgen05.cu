@@ -10,13 +10,13 @@
 // 247 us against 221 below; twice the instructions for the scores, which the issuing warps were slower to come by than the
 // tensor core to carry out.)
 //
-// What bounds it: with many rows the way of a tile from scores to probabilities, 2.2 us for 256 rows x 128 keys x 128 of a head,
-// of which either the tensor core or the exponentials' unit needs half; with few the launch's start (2.5 us until the lengths
-// are known, 3 until the first scores are) and the second launch.  Measured in captured graphs with 28 query and 4
-// key/value heads of 128: 32 requests of up to 8,192 keys and 64 nodes 221 to 230 us, which is 0.6 PFLOP/s of the products that
-// count (264 to 271 after seconds without a pause, at the power limit); one of 32,768 keys and 32 nodes 35.5 us, 1.9 TB/s.
-// With 12 and 2 heads, 8 requests of up to 4,096 keys and 16 nodes: 16.9 us.  With 14 and 2 of 64, one of 1,024 keys and 8
-// nodes: 10.9 us.
+// What bounds it: with many rows a slot's way from one score product to the next, 3,900 cycles for 256 rows x 128 keys x 128 of a head,
+// of which the slots' products take 2,050 of the tensor core and their exponentials 2,050 of their unit: the two hardly overlap.  With
+// few rows the launch's start (2.5 us until the lengths are known, 3 until the first scores are) and the second launch.  Measured in
+// captured graphs with 28 query and 4 key/value heads of 128: 32 requests of up to 8,192 keys and 64 nodes 220 to 230 us, which is
+// 0.6 PFLOP/s of the products that count (265 to 271 after seconds without a pause, at the power limit and 1.42 GHz); one of 32,768
+// keys and 32 nodes 35.6 us, 1.9 TB/s; 8 of 4,096 and 64 52 us, 29 with a window of 1,024 and 180 with a cap.  With 12 and 2 heads, 8
+// requests of up to 4,096 keys and 16 nodes: 17.4 us.  With 14 and 2 of 64, one of 1,024 keys and 8 nodes: 10.9 us.
 //
 //   warps 0, 1    K and V producers: TMA-load the pages that the block table names into rings of tiles
 //   warps 2, 3    issue a slot's products: S = Q K^T into tensor memory, then O += P V with P from there, half by half

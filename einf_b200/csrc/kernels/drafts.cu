@@ -1,7 +1,7 @@
 // After the step that verified a draft: the longest path of the tree that the model agrees with, and the keys and
 // values of its nodes moved to where the cache goes on.  Both are a few kilobytes and bound by the latency of their
 // loads: each is one launch for all requests (and, for the move, all layers).  In captured graphs: paths of 64 trees of
-// 64 nodes 2.8 us, of one tree of 8 2.0 us; the rows of 32 paths of 6 nodes in all layers' caches 4.6 us, of one of three 3.1 us.
+// 64 nodes 2.7 us, of one tree of 8 2.0 us; the rows of 32 paths of 6 nodes in all layers' caches 3.9 us, of one of three 2.9 us.
 #include "common.cuh"
 
 namespace einf {

@@ -12,9 +12,10 @@
 // The nodes of a request share the counts.  A row's path is a few tokens: their places are left out of the walk and done
 // one by one at the end, so that a row may be shaped in place.
 //
-// Measured with a vocabulary of 151,936, in captured graphs: 64 rows with histories of up to 4,096 tokens 21.5 us (3.6 TB/s;
-// a plain copy would take 12, the rest is the histories and the starts of the CTAs), 143 rows of eight trees with biases and masks
-// 42.0 us (4.2 TB/s; 27 for a copy), one row 3.2 us.
+// Measured with a vocabulary of 151,936, in captured graphs: 64 rows with histories of up to 4,096 tokens 21.5 us (3.7 TB/s;
+// a plain copy would take 12: all of a row's parts are asked for at once and then wait for the counts, and each of a request's CTAs
+// reads its whole history), 143 rows of eight trees with biases and masks 42.6 us (4.2 TB/s; 27 for a copy; the CTAs of the request
+// with the most rows end alone), one row 3.3 us.
 #include "tcgen05.cuh"
 
 namespace einf {
